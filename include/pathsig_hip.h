@@ -241,6 +241,82 @@ int pathsig_set_option(const char *name, int64_t value);
 int pathsig_profile_enable(int on);
 float pathsig_profile_sweep_ms(void);
 
+/*
+ * Linear attention with a decay for each head (no counterpart in the reference).  For every sequence b and head h
+ *     S_t = exp(log_decay[h]) S_(t-1) + k_t v_t^T,     out_t = scale * S_t^T q_t,      t = 0 .. n_b - 1,
+ * with a [Dk, Dv] state S in 32 bits that starts from `state` (NULL: from zero).
+ *   q [B, L, H, Dk], k [B, L, Hkv, Dk], v [B, L, Hkv, Dv], H a multiple of Hkv: head h reads keys and values of head
+ *   h / (H / Hkv).  The channels of a head lie side by side; the other strides are given in elements.
+ *   log_decay [H] float32 (not positive in a memory that fades; exp(0) = 1 is a plain sum);
+ *   lengths [B] int32 or NULL: n_b = lengths[b] clamped to 0 .. L (NULL: L).  Rows from n_b on are not read, whatever they
+ *   hold; out and the gradients get zeros there.  The final state is S after token n_b - 1 (the initial state if n_b = 0).
+ *   out [B, L, H, Dv] in the type of q, state and final_state [B, H, Dk, Dv] float32, all dense.
+ * Types: PATHSIG_F32 and PATHSIG_BF16 for q, k, v, out and their gradients.  Dk and Dv from 1 to PATHSIG_MAX_HEAD_DIM.
+ */
+#define PATHSIG_BF16 2
+#define PATHSIG_MAX_HEAD_DIM 256
+
+typedef struct pathsig_linattn {
+    int dtype;
+    int64_t B, L, H, Hkv, Dk, Dv;
+    int64_t q_stride[3], k_stride[3], v_stride[3]; /* of a sequence, a token, a head */
+    float scale;
+    const float *log_decay;
+    const int32_t *lengths;
+} pathsig_linattn;
+
+size_t pathsig_linattn_forward_workspace(const pathsig_linattn *call);
+/* `state` and `final_state` may be NULL, and may be the same buffer. */
+int pathsig_linattn_forward(const pathsig_linattn *call, const void *q, const void *k, const void *v, const float *state,
+                            void *out, float *final_state, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Its backward.  grad_out is a dense [B, L, H, Dv], grad_final_state [B, H, Dk, Dv] float32 or NULL (zero).
+ *   grad_q [B, L, H, Dk], grad_k [B, L, Hkv, Dk], grad_v [B, L, Hkv, Dv] dense, in the type of q (sums over the heads that share
+ *   a key); grad_log_decay [H] and grad_state [B, H, Dk, Dv] float32, each NULL where it is not wanted.
+ */
+size_t pathsig_linattn_backward_workspace(const pathsig_linattn *call, int want_log_decay);
+int pathsig_linattn_backward(const pathsig_linattn *call, const void *q, const void *k, const void *v, const float *state,
+                             const void *grad_out, const float *grad_final_state, void *grad_q, void *grad_k, void *grad_v,
+                             float *grad_log_decay, float *grad_state, void *workspace, size_t workspace_bytes,
+                             void *stream);
+
+/* One token of every sequence: L = 1, no lengths; `state` is updated in place.  The token strides are not read. */
+int pathsig_linattn_step(const pathsig_linattn *call, const void *q, const void *k, const void *v, float *state, void *out,
+                         void *stream);
+
+/*
+ * Norms before and after a block, on rows of C channels (no counterpart in the reference):
+ *     joined = x / sqrt(mean(x^2) + eps) * weight * act(gate),   out = residual + scale * joined,
+ *     next   = out / sqrt(mean(out^2) + eps) * next_weight.
+ * weight, gate, scale, residual may be NULL (then 1, 1, 1 and 0), next too (then it is not computed; next_weight may be
+ * NULL with it).  `next` is computed from `out` before that is rounded to its type.
+ *   x, gate, residual: rows of C channels side by side, row strides in elements; out, next and all gradients dense;
+ *   weight, scale, next_weight [C], all of the type param_dtype: PATHSIG_F32 or that of x;
+ *   statistics [2, rows] float32 (written by the forward unless NULL, read by the backward): 1 / sqrt(...) of x and of out.
+ */
+#define PATHSIG_MAX_NORM_CHANNELS 8192
+#define PATHSIG_GATE_SILU 0    /* act(g) = g / (1 + exp(-g)) */
+#define PATHSIG_GATE_SIGMOID 1 /* act(g) = 1 / (1 + exp(-g)) */
+#define PATHSIG_GATE_LINEAR 2  /* act(g) = g */
+
+typedef struct pathsig_norm {
+    int dtype, param_dtype, activation;
+    int64_t rows, C;
+    int64_t x_stride, gate_stride, residual_stride;
+    float eps;
+    const void *x, *gate, *residual, *weight, *scale, *next_weight;
+} pathsig_norm;
+
+int pathsig_norm_forward(const pathsig_norm *call, void *out, void *next, float *statistics, void *stream);
+
+/* grad_out and grad_next [rows, C] dense, one of them may be NULL (zero).  Each gradient may be NULL where it is not wanted;
+ * those of weight, scale and next_weight are in param_dtype. */
+size_t pathsig_norm_backward_workspace(const pathsig_norm *call);
+int pathsig_norm_backward(const pathsig_norm *call, const float *statistics, const void *grad_out, const void *grad_next,
+                          void *grad_x, void *grad_gate, void *grad_residual, void *grad_weight, void *grad_scale,
+                          void *grad_next_weight, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

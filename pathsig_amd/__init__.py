@@ -9,5 +9,6 @@ _ensure_loaded()
 
 from .modules import LogSignature, Signature  # noqa: E402
 from .projections import projections  # noqa: E402
+from . import sequence  # noqa: E402,F401  (layers of sequence models; not in the reference)
 
 __all__ = ["Signature", "LogSignature", "projections"]

@@ -25,11 +25,45 @@ _PTR = ctypes.c_void_p
 _SIZE = ctypes.c_size_t
 
 
+class LinearAttentionCall(ctypes.Structure):
+    """`pathsig_linattn` of include/pathsig_hip.h."""
+    _fields_ = [("dtype", _INT), ("B", _I64), ("L", _I64), ("H", _I64), ("Hkv", _I64), ("Dk", _I64), ("Dv", _I64),
+                ("q_stride", _I64 * 3), ("k_stride", _I64 * 3), ("v_stride", _I64 * 3), ("scale", ctypes.c_float),
+                ("log_decay", _PTR), ("lengths", _PTR)]
+
+
+class NormCall(ctypes.Structure):
+    """`pathsig_norm` of include/pathsig_hip.h."""
+    _fields_ = [("dtype", _INT), ("param_dtype", _INT), ("activation", _INT), ("rows", _I64), ("C", _I64),
+                ("x_stride", _I64), ("gate_stride", _I64), ("residual_stride", _I64), ("eps", ctypes.c_float),
+                ("x", _PTR), ("gate", _PTR), ("residual", _PTR), ("weight", _PTR), ("scale", _PTR),
+                ("next_weight", _PTR)]
+
+
 def _declare(lib: ctypes.CDLL) -> None:
     lib.pathsig_abi_version.restype = _INT
     lib.pathsig_abi_version.argtypes = []
     lib.pathsig_last_error.restype = ctypes.c_char_p
     lib.pathsig_last_error.argtypes = []
+
+    _CALL = ctypes.POINTER(LinearAttentionCall)
+    lib.pathsig_linattn_forward_workspace.restype = _SIZE
+    lib.pathsig_linattn_forward_workspace.argtypes = [_CALL]
+    lib.pathsig_linattn_forward.restype = _INT
+    lib.pathsig_linattn_forward.argtypes = [_CALL] + [_PTR] * 7 + [_SIZE, _PTR]
+    lib.pathsig_linattn_backward_workspace.restype = _SIZE
+    lib.pathsig_linattn_backward_workspace.argtypes = [_CALL, _INT]
+    lib.pathsig_linattn_backward.restype = _INT
+    lib.pathsig_linattn_backward.argtypes = [_CALL] + [_PTR] * 12 + [_SIZE, _PTR]
+    lib.pathsig_linattn_step.restype = _INT
+    lib.pathsig_linattn_step.argtypes = [_CALL] + [_PTR] * 6
+    _NORM = ctypes.POINTER(NormCall)
+    lib.pathsig_norm_forward.restype = _INT
+    lib.pathsig_norm_forward.argtypes = [_NORM] + [_PTR] * 4
+    lib.pathsig_norm_backward_workspace.restype = _SIZE
+    lib.pathsig_norm_backward_workspace.argtypes = [_NORM]
+    lib.pathsig_norm_backward.restype = _INT
+    lib.pathsig_norm_backward.argtypes = [_NORM] + [_PTR] * 10 + [_SIZE, _PTR]
 
     lib.pathsig_set_option.restype = _INT
     lib.pathsig_set_option.argtypes = [ctypes.c_char_p, _I64]

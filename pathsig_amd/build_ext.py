@@ -1,5 +1,5 @@
 """Compiles pathsig_amd/csrc/*.hip for gfx950 into pathsig_amd/libpathsig_hip.so with hipcc, and the torch
-operator registration csrc/torch_ops.cpp into pathsig_amd/libpathsig_torch.so with g++.
+operator registrations csrc/torch_ops.cpp and csrc/torch_seq.cpp into pathsig_amd/libpathsig_torch.so with g++.
 
 Run `python pathsig_amd/build_ext.py` (or `__graft_entry__.build()`).  The first library needs no torch headers:
 it is a plain C-ABI shared object declared in include/pathsig_hip.h.  The second one links against it and against
@@ -27,8 +27,11 @@ UNITS = ([("dense_kernels.hip", f"dense_kernels_g{g}.o", [f"-DPSIG_GROUP={g}"]) 
             ("words_chunks.hip", "words_chunks.o", []),
             ("logsig_kernels.hip", "logsig_kernels.o", []), ("chain_kernels.hip", "chain_kernels.o", []),
             ("logsig_rows.hip", "logsig_rows_f32.o", ["-DPSIG_ROWS_TYPE=float"]),
+            ("seq_attention.hip", "seq_attention.o", []), ("seq_norms.hip", "seq_norms.o", []),
             ("logsig_rows.hip", "logsig_rows_f64.o", ["-DPSIG_ROWS_TYPE=double"]), ("dense_kernels.hip", "dense_kernels.o", []),
             ("api.hip", "api.o", [])])
+
+TORCH_UNITS = ["torch_ops.cpp", "torch_seq.cpp"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
@@ -92,17 +95,32 @@ def build_torch_ops(verbose: bool = False, out_dir: pathlib.Path | None = None) 
     lib_dirs = cpp_extension.library_paths()
     pkg = PKG if out_dir is None else pathlib.Path(out_dir)
     torch_lib = pkg / TORCH_LIB.name
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *includes,
-           str(CSRC / "torch_ops.cpp"), "-o", str(torch_lib),
-           *[f"-L{d}" for d in lib_dirs], "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python",
+    obj_dir = CSRC if out_dir is None else pathlib.Path(out_dir) / "obj"
+    obj_dir.mkdir(parents=True, exist_ok=True)
+    flags = ["-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *includes]
+
+    def compile_one(name: str) -> str:
+        obj = str(obj_dir / name.replace(".cpp", ".o"))
+        cmd = ["g++", *flags, "-c", str(CSRC / name), "-o", obj]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            sys.stderr.write(res.stdout + res.stderr)
+            raise RuntimeError(f"g++ failed on {name}")
+        return obj
+
+    with concurrent.futures.ThreadPoolExecutor(max_workers=len(TORCH_UNITS)) as pool:
+        objs = list(pool.map(compile_one, TORCH_UNITS))
+    cmd = ["g++", "-shared", "-fPIC", *objs, "-o", str(torch_lib), *[f"-L{d}" for d in lib_dirs], "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python",
            f"-L{pkg}", "-lpathsig_hip", "-Wl,-rpath,$ORIGIN", *[f"-Wl,-rpath,{d}" for d in lib_dirs]]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
-        raise RuntimeError("g++ failed on torch_ops.cpp")
+        raise RuntimeError("g++ failed to link the operator registration")
     return torch_lib
 
 

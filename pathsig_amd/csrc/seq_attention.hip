@@ -1,0 +1,470 @@
+// Linear attention with a decay for each head: whole sequences, their gradients, and single tokens (pathsig_linattn_* of
+// pathsig_hip.h).
+//
+// Recurrence of a head, state S [Dk, Dv]:  S_t = e^g S_(t-1) + k_t v_t^T,  o_t = scale S_t^T q_t.
+// Gradients, with R_t = dL/dS_t through the outputs from t on:  R_t = e^g R_(t+1) + scale q_t do_t^T,
+//   dq_t = scale S_t do_t,   dk_t = R_t v_t,   dv_t = R_t^T k_t,   dS_(-1) = e^g R_0,
+//   dg = sum over t of scale do_t^T T_t^T q_t with T_t = dS_t/dg = e^g (T_(t-1) + S_(t-1)), and <dS_end, T_end>.
+// So all three gradients are the forward's recurrence with other tensors in the places of q, k and v: dq with (do, v, k),
+// dv backwards in time with (k, q, do), dk backwards in time with (v, do, q).
+#include <algorithm>
+
+#include "seq_common.hpp"
+
+namespace psig {
+namespace seq {
+namespace {
+
+// a [B, L, heads, D] tensor; heads[h / group] is read for head h
+template <typename T>
+struct View {
+    const T *p;
+    int64_t sb, st, sh;
+    int group;
+};
+
+struct StateRef {
+    float *p;  // [B, H, rows, columns] dense; element (a, c) of a head at a * row + c * column
+    int64_t row, column;
+};
+
+template <typename T>
+struct Sweep {
+    View<T> q, k, v;
+    StateRef first, last;  // p may be NULL
+    void *out;             // [B, L, H, Dv] dense, T or float
+    const float *log_decay;
+    const int32_t *lengths;
+    int64_t L;
+    int H, Dk, Dv;
+    float in_scale, out_scale;
+};
+
+__device__ __forceinline__ int64_t length_of(const int32_t *lengths, int64_t b, int64_t L) {
+    if (!lengths) return L;
+    const int64_t n = lengths[b];
+    return n < 0 ? 0 : n > L ? L : n;
+}
+
+__device__ __forceinline__ float decay_of(const float *log_decay, int h) {
+    // (minus infinity forgets everything at once; a finite stand-in keeps 0 * g at 0)
+    return fmaxf(log_decay[h], -1e30f);
+}
+
+// One lane per column of the state, the column in LDS.
+template <typename T, typename O, bool REVERSE>
+__global__ __launch_bounds__(64) void scan_kernel(const Sweep<T> a) {
+    __shared__ float S[PATHSIG_MAX_HEAD_DIM][64];
+    const int lane = threadIdx.x, h = blockIdx.y;
+    const int64_t b = blockIdx.z;
+    const int c = blockIdx.x * 64 + lane;
+    const bool mine = c < a.Dv;
+    const int64_t n = length_of(a.lengths, b, a.L);
+    const float decay = expf(decay_of(a.log_decay, h));
+    const int64_t head = (b * a.H + h) * a.Dk * a.Dv;
+    for (int r = 0; r < a.Dk; ++r) S[r][lane] = mine && a.first.p ? a.first.p[head + r * a.first.row + c * a.first.column] : 0.f;
+    const T *q = a.q.p + b * a.q.sb + (h / a.q.group) * a.q.sh;
+    const T *k = a.k.p + b * a.k.sb + (h / a.k.group) * a.k.sh;
+    const T *v = a.v.p + b * a.v.sb + (h / a.v.group) * a.v.sh;
+    O *out = (O *)a.out;
+    for (int64_t i = 0; i < n; ++i) {
+        const int64_t t = REVERSE ? n - 1 - i : i;
+        const float vc = mine ? to_float(v[t * a.v.st + c]) * a.in_scale : 0.f;
+        float o = 0.f;
+        for (int r = 0; r < a.Dk; ++r) {
+            float s = S[r][lane];
+            s = (REVERSE ? s : s * decay) + to_float(k[t * a.k.st + r]) * vc;
+            o += to_float(q[t * a.q.st + r]) * s;
+            S[r][lane] = REVERSE ? s * decay : s;
+        }
+        if (mine && out) out[((b * a.L + t) * a.H + h) * a.Dv + c] = from_float<O>(o * a.out_scale);
+    }
+    if (out && mine)
+        for (int64_t t = n; t < a.L; ++t) out[((b * a.L + t) * a.H + h) * a.Dv + c] = from_float<O>(0.f);
+    if (a.last.p && mine)
+        for (int r = 0; r < a.Dk; ++r) a.last.p[head + r * a.last.row + c * a.last.column] = S[r][lane];
+}
+
+// dL/dg: the state and its derivative side by side.
+template <typename T>
+__global__ __launch_bounds__(32) void decay_scan_kernel(const Sweep<T> a, const T *grad_out, const float *grad_final, float *partial) {
+    __shared__ float S[PATHSIG_MAX_HEAD_DIM][32], D[PATHSIG_MAX_HEAD_DIM][32];
+    const int lane = threadIdx.x, h = blockIdx.y;
+    const int64_t b = blockIdx.z;
+    const int c = blockIdx.x * 32 + lane;
+    const bool mine = c < a.Dv;
+    const int64_t n = length_of(a.lengths, b, a.L);
+    const float decay = expf(decay_of(a.log_decay, h));
+    const int64_t head = (b * a.H + h) * a.Dk * a.Dv;
+    for (int r = 0; r < a.Dk; ++r) {
+        S[r][lane] = mine && a.first.p ? a.first.p[head + (int64_t)r * a.Dv + c] : 0.f;
+        D[r][lane] = 0.f;
+    }
+    const T *q = a.q.p + b * a.q.sb + (h / a.q.group) * a.q.sh;
+    const T *k = a.k.p + b * a.k.sb + (h / a.k.group) * a.k.sh;
+    const T *v = a.v.p + b * a.v.sb + (h / a.v.group) * a.v.sh;
+    double total = 0;
+    for (int64_t t = 0; t < n; ++t) {
+        const float vc = mine ? to_float(v[t * a.v.st + c]) : 0.f;
+        const float go = mine ? to_float(grad_out[((b * a.L + t) * a.H + h) * a.Dv + c]) * a.out_scale : 0.f;
+        float o = 0.f;
+        for (int r = 0; r < a.Dk; ++r) {
+            const float s = S[r][lane], d = decay * (D[r][lane] + s);
+            D[r][lane] = d;
+            S[r][lane] = s * decay + to_float(k[t * a.k.st + r]) * vc;
+            o += to_float(q[t * a.q.st + r]) * d;
+        }
+        total += o * go;
+    }
+    if (grad_final && mine)
+        for (int r = 0; r < a.Dk; ++r) total += D[r][lane] * grad_final[head + (int64_t)r * a.Dv + c];
+    float sum = (float)total;
+    for (int m = 1; m < 32; m <<= 1) sum += __shfl_xor(sum, m);
+    if (lane == 0) partial[((int64_t)blockIdx.x * gridDim.z + b) * a.H + h] = sum;
+}
+
+__global__ void decay_sum_kernel(const float *partial, int64_t rows, int H, float *out) {
+    const int h = blockIdx.x;
+    double s = 0;
+    for (int64_t i = threadIdx.x; i < rows; i += 64) s += partial[i * H + h];
+    for (int m = 1; m < 64; m <<= 1) s += __shfl_xor(s, m);
+    if (threadIdx.x == 0) out[h] = (float)s;
+}
+
+// [rows, H, D] float -> [rows, H / group, D]: the gradient of a key is the sum over the heads that read it
+template <typename T>
+__global__ void group_sum_kernel(const float *in, T *out, int64_t rows, int Hkv, int group, int D) {
+    const int64_t n = rows * Hkv * D;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t head = i / D;
+        const float *p = in + head * group * D + i % D;
+        float s = 0.f;
+        for (int g = 0; g < group; ++g) s += p[(int64_t)g * D];
+        out[i] = from_float<T>(s);
+    }
+}
+
+// One token.  A block has a head of a sequence: TX threads along Dv, the rows of the state dealt to the 256 / TX groups of
+// threads, so that the state is read and written once, in lines.  Bound by that.
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void step_kernel(const Sweep<T> a, float *state, int tx_log2) {
+    __shared__ float qs[PATHSIG_MAX_HEAD_DIM], ks[PATHSIG_MAX_HEAD_DIM];
+    __shared__ float meet[256 * VEC];
+    using V = Pack<float, VEC>;
+    const int h = blockIdx.x, tid = threadIdx.x;
+    const int64_t b = blockIdx.y;
+    const T *q = a.q.p + b * a.q.sb + (h / a.q.group) * a.q.sh;
+    const T *k = a.k.p + b * a.k.sb + (h / a.k.group) * a.k.sh;
+    const T *v = a.v.p + b * a.v.sb + (h / a.v.group) * a.v.sh;
+    if (tid < a.Dk) {
+        qs[tid] = to_float(q[tid]) * a.out_scale;
+        ks[tid] = to_float(k[tid]);
+    }
+    __syncthreads();
+    const float decay = expf(decay_of(a.log_decay, h));
+    const int TX = 1 << tx_log2, TY = 256 >> tx_log2;
+    const int tx = tid & (TX - 1), ty = tid >> tx_log2;
+    float *S = state + (b * a.H + h) * a.Dk * a.Dv;
+    T *out = (T *)a.out + (b * a.H + h) * a.Dv;
+    for (int c0 = 0; c0 < a.Dv; c0 += TX * VEC) {
+        const int c = c0 + tx * VEC;
+        const bool mine = c < a.Dv;
+        float vc[VEC], o[VEC] = {};
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) vc[e] = mine ? to_float(v[c + e]) : 0.f;
+        if (mine) {
+#pragma unroll 8
+            for (int r = ty; r < a.Dk; r += TY) {
+                V s = *(const V *)(S + (int64_t)r * a.Dv + c);
+                const float kr = ks[r], qr = qs[r];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    s.v[e] = s.v[e] * decay + kr * vc[e];
+                    o[e] += qr * s.v[e];
+                }
+                *(V *)(S + (int64_t)r * a.Dv + c) = s;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) meet[tid * VEC + e] = o[e];
+        __syncthreads();
+        for (int i = tid; i < TX * VEC; i += 256) {
+            if (c0 + i >= a.Dv) continue;
+            float s = 0.f;
+            for (int y = 0; y < TY; ++y) s += meet[y * TX * VEC + i];
+            out[c0 + i] = from_float<T>(s);
+        }
+        __syncthreads();
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------
+int check_call(const pathsig_linattn *c) {
+    if (!c) {
+        set_error("call must not be NULL");
+        return PATHSIG_ERR_ARGUMENT;
+    }
+    if (c->dtype != PATHSIG_F32 && c->dtype != PATHSIG_BF16) {
+        set_error("dtype must be PATHSIG_F32 or PATHSIG_BF16");
+        return PATHSIG_ERR_ARGUMENT;
+    }
+    if (c->B < 0 || c->L < 0 || c->H < 1 || c->Hkv < 1 || c->H % c->Hkv) {
+        set_error("sizes must not be negative and H a multiple of Hkv (got B %lld, L %lld, H %lld, Hkv %lld)", (long long)c->B,
+                  (long long)c->L, (long long)c->H, (long long)c->Hkv);
+        return PATHSIG_ERR_ARGUMENT;
+    }
+    if (c->Dk < 1 || c->Dv < 1) {
+        set_error("Dk and Dv must be at least 1 (got %lld, %lld)", (long long)c->Dk, (long long)c->Dv);
+        return PATHSIG_ERR_ARGUMENT;
+    }
+    if (c->Dk > PATHSIG_MAX_HEAD_DIM || c->Dv > PATHSIG_MAX_HEAD_DIM) {
+        set_error("Dk and Dv must be at most %d (got %lld, %lld)", PATHSIG_MAX_HEAD_DIM, (long long)c->Dk, (long long)c->Dv);
+        return PATHSIG_ERR_UNSUPPORTED;
+    }
+    if (c->H > 65535 || c->B > 65535 || c->L > 0x7fffffff) {
+        set_error("at most 65535 sequences and heads and 2^31 - 1 tokens (got B %lld, H %lld, L %lld)", (long long)c->B,
+                  (long long)c->H, (long long)c->L);
+        return PATHSIG_ERR_UNSUPPORTED;
+    }
+    for (int i = 0; i < 3; ++i)
+        if (c->q_stride[i] < 0 || c->k_stride[i] < 0 || c->v_stride[i] < 0) {
+            set_error("strides must not be negative");
+            return PATHSIG_ERR_ARGUMENT;
+        }
+    if (!c->log_decay) {
+        set_error("log_decay must not be NULL");
+        return PATHSIG_ERR_ARGUMENT;
+    }
+    return PATHSIG_OK;
+}
+
+template <typename T>
+View<T> view(const void *p, const int64_t *stride, int64_t group) {
+    return {(const T *)p, stride[0], stride[1], stride[2], (int)group};
+}
+
+template <typename T>
+View<T> dense(const void *p, int64_t L, int64_t H, int64_t D) {
+    return {(const T *)p, L * H * D, H * D, D, 1};
+}
+
+template <typename T>
+Sweep<T> sweep(const pathsig_linattn *c) {
+    Sweep<T> a = {};
+    a.log_decay = c->log_decay;
+    a.lengths = c->lengths;
+    a.L = c->L;
+    a.H = (int)c->H;
+    a.Dk = (int)c->Dk;
+    a.Dv = (int)c->Dv;
+    a.in_scale = 1.f;
+    a.out_scale = 1.f;
+    return a;
+}
+
+template <typename T, typename O, bool REVERSE>
+void run_scan(const Sweep<T> &a, int64_t B, hipStream_t stream) {
+    scan_kernel<T, O, REVERSE><<<dim3((unsigned)ceil_div(a.Dv, 64), a.H, (unsigned)B), 64, 0, stream>>>(a);
+}
+
+template <typename T>
+int forward_t(const pathsig_linattn *c, const void *q, const void *k, const void *v, const float *state, void *out, float *final_state,
+              hipStream_t stream) {
+    Sweep<T> a = sweep<T>(c);
+    const int64_t group = c->H / c->Hkv;
+    a.q = view<T>(q, c->q_stride, 1);
+    a.k = view<T>(k, c->k_stride, group);
+    a.v = view<T>(v, c->v_stride, group);
+    a.first = {const_cast<float *>(state), c->Dv, 1};
+    a.last = {final_state, c->Dv, 1};
+    a.out = out;
+    a.out_scale = c->scale;
+    run_scan<T, T, false>(a, c->B, stream);
+    return launch_status("linear attention");
+}
+
+struct BackwardLayout {
+    size_t wide_k, wide_v, decay, total;  // byte offsets
+};
+
+size_t place(size_t &total, size_t bytes) {
+    const size_t at = total;
+    total += (bytes + 255) / 256 * 256;
+    return at;
+}
+
+BackwardLayout backward_layout(const pathsig_linattn *c, bool want_decay) {
+    BackwardLayout l = {};
+    const size_t tokens = (size_t)c->B * c->L * c->H;
+    if (c->H != c->Hkv) {
+        l.wide_k = place(l.total, tokens * c->Dk * sizeof(float));
+        l.wide_v = place(l.total, tokens * c->Dv * sizeof(float));
+    }
+    if (want_decay) l.decay = place(l.total, (size_t)ceil_div(c->Dv, 32) * c->B * c->H * sizeof(float));
+    return l;
+}
+
+template <typename T>
+int backward_t(const pathsig_linattn *c, const void *q, const void *k, const void *v, const float *state, const void *grad_out,
+               const float *grad_final, void *grad_q, void *grad_k, void *grad_v, float *grad_decay, float *grad_state, char *ws,
+               hipStream_t stream) {
+    const int64_t group = c->H / c->Hkv;
+    const View<T> vq = view<T>(q, c->q_stride, 1), vk = view<T>(k, c->k_stride, group), vv = view<T>(v, c->v_stride, group),
+                  vdo = dense<T>(grad_out, c->L, c->H, c->Dv);
+    const BackwardLayout l = backward_layout(c, grad_decay != nullptr);
+    // dq: the forward with (do, v, k) and the transposed state
+    Sweep<T> a = sweep<T>(c);
+    std::swap(a.Dk, a.Dv);
+    a.q = vdo;
+    a.k = vv;
+    a.v = vk;
+    a.first = {const_cast<float *>(state), 1, c->Dv};
+    a.out = grad_q;
+    a.out_scale = c->scale;
+    run_scan<T, T, false>(a, c->B, stream);
+    // dv: backwards in time with (k, q, do)
+    a = sweep<T>(c);
+    a.q = vk;
+    a.k = vq;
+    a.v = vdo;
+    a.first = {const_cast<float *>(grad_final), c->Dv, 1};
+    a.last = {grad_state, c->Dv, 1};
+    a.in_scale = c->scale;
+    a.out = group > 1 ? (void *)(ws + l.wide_v) : grad_v;
+    if (group > 1)
+        run_scan<T, float, true>(a, c->B, stream);
+    else
+        run_scan<T, T, true>(a, c->B, stream);
+    // dk: backwards in time with (v, do, q) and the transposed gradient of the state
+    std::swap(a.Dk, a.Dv);
+    a.q = vv;
+    a.k = vdo;
+    a.v = vq;
+    a.first = {const_cast<float *>(grad_final), 1, c->Dv};
+    a.last = {nullptr, 0, 0};
+    a.out = group > 1 ? (void *)(ws + l.wide_k) : grad_k;
+    if (group > 1)
+        run_scan<T, float, true>(a, c->B, stream);
+    else
+        run_scan<T, T, true>(a, c->B, stream);
+    if (group > 1) {
+        const int64_t rows = c->B * c->L;
+        const unsigned blocks_k = (unsigned)std::min<int64_t>(ceil_div(rows * c->Hkv * c->Dk, 256), 4096);
+        const unsigned blocks_v = (unsigned)std::min<int64_t>(ceil_div(rows * c->Hkv * c->Dv, 256), 4096);
+        group_sum_kernel<T><<<blocks_k, 256, 0, stream>>>((const float *)(ws + l.wide_k), (T *)grad_k, rows, (int)c->Hkv, (int)group, (int)c->Dk);
+        group_sum_kernel<T><<<blocks_v, 256, 0, stream>>>((const float *)(ws + l.wide_v), (T *)grad_v, rows, (int)c->Hkv, (int)group, (int)c->Dv);
+    }
+    if (grad_decay) {
+        a = sweep<T>(c);
+        a.q = vq;
+        a.k = vk;
+        a.v = vv;
+        a.first = {const_cast<float *>(state), c->Dv, 1};
+        a.out_scale = c->scale;
+        const int64_t slices = ceil_div(c->Dv, 32);
+        decay_scan_kernel<T><<<dim3((unsigned)slices, a.H, (unsigned)c->B), 32, 0, stream>>>(a, (const T *)grad_out, grad_final,
+                                                                                           (float *)(ws + l.decay));
+        decay_sum_kernel<<<a.H, 64, 0, stream>>>((const float *)(ws + l.decay), slices * c->B, a.H, grad_decay);
+    }
+    return launch_status("linear attention, backward");
+}
+
+template <typename T>
+int step_t(const pathsig_linattn *c, const void *q, const void *k, const void *v, float *state, void *out, hipStream_t stream) {
+    Sweep<T> a = sweep<T>(c);
+    const int64_t group = c->H / c->Hkv;
+    a.q = view<T>(q, c->q_stride, 1);
+    a.k = view<T>(k, c->k_stride, group);
+    a.v = view<T>(v, c->v_stride, group);
+    a.out = out;
+    a.out_scale = c->scale;
+    const dim3 grid((unsigned)c->H, (unsigned)c->B);
+    const int vec = c->Dv % 4 == 0 && aligned16(state) ? 4 : 1;
+    int tx_log2 = 0;
+    while (tx_log2 < 6 && ((int64_t)vec << tx_log2) < c->Dv) ++tx_log2;
+    if (vec == 4)
+        step_kernel<T, 4><<<grid, 256, 0, stream>>>(a, state, tx_log2);
+    else
+        step_kernel<T, 1><<<grid, 256, 0, stream>>>(a, state, tx_log2);
+    return launch_status("linear attention, step");
+}
+
+}  // namespace
+}  // namespace seq
+}  // namespace psig
+
+using namespace psig;
+using namespace psig::seq;
+
+extern "C" {
+
+size_t pathsig_linattn_forward_workspace(const pathsig_linattn *call) {
+    if (check_call(call) != PATHSIG_OK) return 0;
+    return 0;
+}
+
+int pathsig_linattn_forward(const pathsig_linattn *call, const void *q, const void *k, const void *v, const float *state,
+                            void *out, float *final_state, void *workspace, size_t workspace_bytes, void *stream) {
+    if (const int rc = check_call(call)) return rc;
+    if (call->B == 0) return PATHSIG_OK;
+    if (call->L > 0 && (!q || !k || !v || !out)) {
+        set_error("q, k, v and out must not be NULL");
+        return PATHSIG_ERR_ARGUMENT;
+    }
+    const size_t need = pathsig_linattn_forward_workspace(call);
+    if (need > 0 && (!workspace || workspace_bytes < need)) {
+        set_error("linear attention: workspace of %zu bytes needed, got %zu", need, workspace ? workspace_bytes : (size_t)0);
+        return PATHSIG_ERR_WORKSPACE;
+    }
+    if (call->dtype == PATHSIG_F32) return forward_t<float>(call, q, k, v, state, out, final_state, (hipStream_t)stream);
+    return forward_t<bf16>(call, q, k, v, state, out, final_state, (hipStream_t)stream);
+}
+
+size_t pathsig_linattn_backward_workspace(const pathsig_linattn *call, int want_log_decay) {
+    if (check_call(call) != PATHSIG_OK) return 0;
+    return backward_layout(call, want_log_decay != 0).total;
+}
+
+int pathsig_linattn_backward(const pathsig_linattn *call, const void *q, const void *k, const void *v, const float *state,
+                             const void *grad_out, const float *grad_final_state, void *grad_q, void *grad_k, void *grad_v,
+                             float *grad_log_decay, float *grad_state, void *workspace, size_t workspace_bytes,
+                             void *stream) {
+    if (const int rc = check_call(call)) return rc;
+    if (call->B > 0 && call->L > 0 && (!q || !k || !v || !grad_out || !grad_q || !grad_k || !grad_v)) {
+        set_error("q, k, v, grad_out, grad_q, grad_k and grad_v must not be NULL");
+        return PATHSIG_ERR_ARGUMENT;
+    }
+    const size_t need = backward_layout(call, grad_log_decay != nullptr).total;
+    if (need > 0 && (!workspace || workspace_bytes < need)) {
+        set_error("linear attention backward: workspace of %zu bytes needed, got %zu", need, workspace ? workspace_bytes : (size_t)0);
+        return PATHSIG_ERR_WORKSPACE;
+    }
+    if (call->B == 0) {
+        if (!grad_log_decay) return PATHSIG_OK;
+        decay_sum_kernel<<<(unsigned)call->H, 64, 0, (hipStream_t)stream>>>(nullptr, 0, (int)call->H, grad_log_decay);
+        return launch_status("linear attention, backward");
+    }
+    if (call->dtype == PATHSIG_F32)
+        return backward_t<float>(call, q, k, v, state, grad_out, grad_final_state, grad_q, grad_k, grad_v, grad_log_decay,
+                                 grad_state, (char *)workspace, (hipStream_t)stream);
+    return backward_t<bf16>(call, q, k, v, state, grad_out, grad_final_state, grad_q, grad_k, grad_v, grad_log_decay,
+                            grad_state, (char *)workspace, (hipStream_t)stream);
+}
+
+int pathsig_linattn_step(const pathsig_linattn *call, const void *q, const void *k, const void *v, float *state, void *out,
+                         void *stream) {
+    if (const int rc = check_call(call)) return rc;
+    if (call->L != 1 || call->lengths) {
+        set_error("a step has one token of every sequence: L must be 1 and lengths NULL");
+        return PATHSIG_ERR_ARGUMENT;
+    }
+    if (call->B == 0) return PATHSIG_OK;
+    if (!q || !k || !v || !state || !out) {
+        set_error("q, k, v, state and out must not be NULL");
+        return PATHSIG_ERR_ARGUMENT;
+    }
+    if (call->dtype == PATHSIG_F32) return step_t<float>(call, q, k, v, state, out, (hipStream_t)stream);
+    return step_t<bf16>(call, q, k, v, state, out, (hipStream_t)stream);
+}
+
+}  // extern "C"

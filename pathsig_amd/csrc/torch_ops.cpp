@@ -21,10 +21,11 @@
 #include <tuple>
 #include <vector>
 
-#include "pathsig_hip.h"
+#include "torch_common.hpp"
 
 namespace {
 
+using namespace psig_torch;
 using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
@@ -33,17 +34,6 @@ int dtype_code(const Tensor &t, const char *what) {
     if (t.scalar_type() == at::kFloat) return PATHSIG_F32;
     if (t.scalar_type() == at::kDouble) return PATHSIG_F64;
     TORCH_CHECK(false, what, " must be float32 or float64");
-}
-
-void *ptr(const Tensor &t) { return t.defined() && t.numel() > 0 ? t.data_ptr() : nullptr; }
-
-void check_rc(int rc) { TORCH_CHECK(rc == PATHSIG_OK, "pathsig: ", pathsig_last_error(), " (error ", rc, ")"); }
-
-void *stream_of(const Tensor &t) { return (void *)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
-
-Tensor scratch(size_t nbytes, const Tensor &like) {
-    if (nbytes == 0) return Tensor();
-    return at::empty({(int64_t)nbytes}, like.options().dtype(at::kByte));
 }
 
 void check_words_arg(const Tensor &encoded_words) {
@@ -333,11 +323,6 @@ Tensor logsig_backward_kept_hip(const Tensor &logsig_in, const Tensor &cache_in,
 }
 
 // ---- autograd (`src/pathsig/ops.py:231-297`) ---------------------------------------------------------------
-template <typename Signature>
-auto typed_op(const char *name) {
-    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Signature>();
-}
-
 using SigForward = Tensor(const Tensor &, int64_t, bool, const Tensor &, at::IntArrayRef, bool, const Tensor &);
 using SigForwardKeep = std::tuple<Tensor, Tensor>(const Tensor &, int64_t, bool, const Tensor &, at::IntArrayRef, bool,
                                                   const Tensor &);
@@ -493,18 +478,6 @@ std::tuple<Tensor, Tensor> sig_to_logsig_keep_autograd(const Tensor &signature, 
 // The backward of these nodes looks at its tensors in the same way: an upstream gradient can be a batched tensor
 // (is_grads_batched), a view whose sign bit is still to be applied, or one that a mode is watching, and saved-tensor
 // hooks can hand back anything.
-bool plain(const Tensor &t) {
-    using c10::DispatchKey;
-    if (!t.defined() || !t.is_cuda() || t._fw_grad(/*level=*/0).defined()) return false;
-    if (at::impl::torch_function_mode_enabled()) return false;
-    const auto tls = c10::impl::tls_local_dispatch_key_set();
-    const c10::DispatchKeySet ordinary({DispatchKey::CUDA, DispatchKey::ADInplaceOrView, DispatchKey::AutogradCUDA,
-                                        DispatchKey::AutogradOther, DispatchKey::BackendSelect, DispatchKey::AutocastCUDA,
-                                        DispatchKey::AutocastCPU});
-    const c10::DispatchKeySet rest = ((t.key_set() | tls.included_) - tls.excluded_) - ordinary;
-    return (rest.raw_repr() & ~c10::full_backend_mask) == 0;
-}
-
 bool plain_call(const Tensor &path) { return plain(path) && path.scalar_type() != at::kHalf; }
 
 // the signature with its hand-over, as SignatureKeepFunction, without a second dispatch
@@ -664,12 +637,6 @@ bool no_keep() {
 }
 
 // The functions of the extension.  All arguments positional; None when the call is not one for this way.
-bool tensor_arg(PyObject *obj, Tensor &out) {
-    if (!THPVariable_CheckExact(obj)) return false;
-    out = THPVariable_Unpack(obj);
-    return true;
-}
-
 bool ints_arg(PyObject *obj, std::vector<int64_t> &out) {
     if (!PyList_Check(obj)) return false;
     const Py_ssize_t n = PyList_GET_SIZE(obj);
@@ -742,6 +709,9 @@ PyObject *py_logsignature(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
 PyMethodDef kMethods[] = {
     {"signature", (PyCFunction)(void (*)(void))py_signature, METH_FASTCALL, nullptr},
     {"logsignature", (PyCFunction)(void (*)(void))py_logsignature, METH_FASTCALL, nullptr},
+    {"linear_attention", (PyCFunction)(void (*)(void))psig_torch::py_linear_attention, METH_FASTCALL, nullptr},
+    {"linear_attention_step", (PyCFunction)(void (*)(void))psig_torch::py_linear_attention_step, METH_FASTCALL, nullptr},
+    {"norm_join", (PyCFunction)(void (*)(void))psig_torch::py_norm_join, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "libpathsig_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
