@@ -251,10 +251,12 @@ float pathsig_profile_sweep_ms(void);
  *   lengths [B] int32 or NULL: n_b = lengths[b] clamped to 0 .. L (NULL: L).  Rows from n_b on are not read, whatever they
  *   hold; out and the gradients get zeros there.  The final state is S after token n_b - 1 (the initial state if n_b = 0).
  *   out [B, L, H, Dv] in the type of q, state and final_state [B, H, Dk, Dv] float32, all dense.
- * Types: PATHSIG_F32 and PATHSIG_BF16 for q, k, v, out and their gradients.  Dk and Dv from 1 to PATHSIG_MAX_HEAD_DIM.
+ * Types: PATHSIG_F32 and PATHSIG_BF16 for q, k, v, out and their gradients.  Dk and Dv from 1 to PATHSIG_MAX_HEAD_DIM, tokens up
+ * to PATHSIG_MAX_TOKEN_STRIDE elements apart.
  */
 #define PATHSIG_BF16 2
 #define PATHSIG_MAX_HEAD_DIM 256
+#define PATHSIG_MAX_TOKEN_STRIDE (1 << 24)
 
 typedef struct pathsig_linattn {
     int dtype;

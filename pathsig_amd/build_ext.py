@@ -27,6 +27,7 @@ UNITS = ([("dense_kernels.hip", f"dense_kernels_g{g}.o", [f"-DPSIG_GROUP={g}"]) 
             ("words_chunks.hip", "words_chunks.o", []),
             ("logsig_kernels.hip", "logsig_kernels.o", []), ("chain_kernels.hip", "chain_kernels.o", []),
             ("logsig_rows.hip", "logsig_rows_f32.o", ["-DPSIG_ROWS_TYPE=float"]),
+            *[("seq_chunks.hip", f"seq_chunks_{n}.o", [f"-DPSIG_KEY_TILES={n}"]) for n in (8, 4, 2, 1)],
             ("seq_attention.hip", "seq_attention.o", []), ("seq_norms.hip", "seq_norms.o", []),
             ("logsig_rows.hip", "logsig_rows_f64.o", ["-DPSIG_ROWS_TYPE=double"]), ("dense_kernels.hip", "dense_kernels.o", []),
             ("api.hip", "api.o", [])])

@@ -7,87 +7,44 @@
 //   dg = sum over t of scale do_t^T T_t^T q_t with T_t = dS_t/dg = e^g (T_(t-1) + S_(t-1)), and <dS_end, T_end>.
 // So all three gradients are the forward's recurrence with other tensors in the places of q, k and v: dq with (do, v, k),
 // dv backwards in time with (k, q, do), dk backwards in time with (v, do, q).
+//
+// A sweep over whole sequences is cut into pieces where there are fewer heads of sequences than the device takes at once: the
+// states that the pieces add from zero (k and v read once more), a scan over the pieces, and all pieces at once from their
+// states.
 #include <algorithm>
 
-#include "seq_common.hpp"
+#include "seq_attention.hpp"
 
 namespace psig {
 namespace seq {
 namespace {
 
-// a [B, L, heads, D] tensor; heads[h / group] is read for head h
-template <typename T>
-struct View {
-    const T *p;
-    int64_t sb, st, sh;
-    int group;
-};
-
-struct StateRef {
-    float *p;  // [B, H, rows, columns] dense; element (a, c) of a head at a * row + c * column
-    int64_t row, column;
-};
-
-template <typename T>
-struct Sweep {
-    View<T> q, k, v;
-    StateRef first, last;  // p may be NULL
-    void *out;             // [B, L, H, Dv] dense, T or float
-    const float *log_decay;
-    const int32_t *lengths;
-    int64_t L;
-    int H, Dk, Dv;
-    float in_scale, out_scale;
-};
-
-__device__ __forceinline__ int64_t length_of(const int32_t *lengths, int64_t b, int64_t L) {
-    if (!lengths) return L;
-    const int64_t n = lengths[b];
-    return n < 0 ? 0 : n > L ? L : n;
-}
-
-__device__ __forceinline__ float decay_of(const float *log_decay, int h) {
-    // (minus infinity forgets everything at once; a finite stand-in keeps 0 * g at 0)
-    return fmaxf(log_decay[h], -1e30f);
-}
-
-// One lane per column of the state, the column in LDS.
-template <typename T, typename O, bool REVERSE>
-__global__ __launch_bounds__(64) void scan_kernel(const Sweep<T> a) {
-    __shared__ float S[PATHSIG_MAX_HEAD_DIM][64];
-    const int lane = threadIdx.x, h = blockIdx.y;
-    const int64_t b = blockIdx.z;
-    const int c = blockIdx.x * 64 + lane;
-    const bool mine = c < a.Dv;
+// starts[s] holds what piece s - 1 adds; in place becomes the state in front of piece s.
+__global__ __launch_bounds__(256) void join_kernel(const Sweep a) {
+    const int64_t plane = (int64_t)a.Dk * a.Dv;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= plane) return;
+    const int h = blockIdx.y;
+    const int64_t b = blockIdx.z, head = (b * a.H + h) * plane, stride = a.B * a.H * plane;
     const int64_t n = length_of(a.lengths, b, a.L);
-    const float decay = expf(decay_of(a.log_decay, h));
-    const int64_t head = (b * a.H + h) * a.Dk * a.Dv;
-    for (int r = 0; r < a.Dk; ++r) S[r][lane] = mine && a.first.p ? a.first.p[head + r * a.first.row + c * a.first.column] : 0.f;
-    const T *q = a.q.p + b * a.q.sb + (h / a.q.group) * a.q.sh;
-    const T *k = a.k.p + b * a.k.sb + (h / a.k.group) * a.k.sh;
-    const T *v = a.v.p + b * a.v.sb + (h / a.v.group) * a.v.sh;
-    O *out = (O *)a.out;
-    for (int64_t i = 0; i < n; ++i) {
-        const int64_t t = REVERSE ? n - 1 - i : i;
-        const float vc = mine ? to_float(v[t * a.v.st + c]) * a.in_scale : 0.f;
-        float o = 0.f;
-        for (int r = 0; r < a.Dk; ++r) {
-            float s = S[r][lane];
-            s = (REVERSE ? s : s * decay) + to_float(k[t * a.k.st + r]) * vc;
-            o += to_float(q[t * a.q.st + r]) * s;
-            S[r][lane] = REVERSE ? s * decay : s;
-        }
-        if (mine && out) out[((b * a.L + t) * a.H + h) * a.Dv + c] = from_float<O>(o * a.out_scale);
+    const float g2 = decay_of(a.log_decay, h) * kLog2e;
+    // (element i of `first` where its rows are the columns of `starts`)
+    const int64_t at = a.first.row == a.starts.row ? i : (i % a.Dv) * a.Dk + i / a.Dv;
+    float *const p = a.starts.p + head + i;
+    float x = a.first.p ? a.first.p[head + at] : 0.f;
+    p[0] = x;
+    const float full = exp2f(g2 * (float)a.piece);
+#pragma unroll 8
+    for (int s = 1; s < a.pieces; ++s) {
+        const int64_t left = n - (s - 1) * a.piece;  // tokens from the piece before on
+        x = x * (left >= a.piece ? full : left > 0 ? exp2f(g2 * (float)left) : 1.f) + p[s * stride];
+        p[s * stride] = x;
     }
-    if (out && mine)
-        for (int64_t t = n; t < a.L; ++t) out[((b * a.L + t) * a.H + h) * a.Dv + c] = from_float<O>(0.f);
-    if (a.last.p && mine)
-        for (int r = 0; r < a.Dk; ++r) a.last.p[head + r * a.last.row + c * a.last.column] = S[r][lane];
 }
 
 // dL/dg: the state and its derivative side by side.
 template <typename T>
-__global__ __launch_bounds__(32) void decay_scan_kernel(const Sweep<T> a, const T *grad_out, const float *grad_final, float *partial) {
+__global__ __launch_bounds__(32) void decay_scan_kernel(const Sweep a, const T *grad_out, const float *grad_final, float *partial) {
     __shared__ float S[PATHSIG_MAX_HEAD_DIM][32], D[PATHSIG_MAX_HEAD_DIM][32];
     const int lane = threadIdx.x, h = blockIdx.y;
     const int64_t b = blockIdx.z;
@@ -100,9 +57,9 @@ __global__ __launch_bounds__(32) void decay_scan_kernel(const Sweep<T> a, const 
         S[r][lane] = mine && a.first.p ? a.first.p[head + (int64_t)r * a.Dv + c] : 0.f;
         D[r][lane] = 0.f;
     }
-    const T *q = a.q.p + b * a.q.sb + (h / a.q.group) * a.q.sh;
-    const T *k = a.k.p + b * a.k.sb + (h / a.k.group) * a.k.sh;
-    const T *v = a.v.p + b * a.v.sb + (h / a.v.group) * a.v.sh;
+    const T *q = (const T *)a.q.p + b * a.q.sb + (h / a.q.group) * a.q.sh;
+    const T *k = (const T *)a.k.p + b * a.k.sb + (h / a.k.group) * a.k.sh;
+    const T *v = (const T *)a.v.p + b * a.v.sb + (h / a.v.group) * a.v.sh;
     double total = 0;
     for (int64_t t = 0; t < n; ++t) {
         const float vc = mine ? to_float(v[t * a.v.st + c]) : 0.f;
@@ -147,15 +104,15 @@ __global__ void group_sum_kernel(const float *in, T *out, int64_t rows, int Hkv,
 // One token.  A block has a head of a sequence: TX threads along Dv, the rows of the state dealt to the 256 / TX groups of
 // threads, so that the state is read and written once, in lines.  Bound by that.
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void step_kernel(const Sweep<T> a, float *state, int tx_log2) {
+__global__ __launch_bounds__(256) void step_kernel(const Sweep a, float *state, int tx_log2) {
     __shared__ float qs[PATHSIG_MAX_HEAD_DIM], ks[PATHSIG_MAX_HEAD_DIM];
     __shared__ float meet[256 * VEC];
     using V = Pack<float, VEC>;
     const int h = blockIdx.x, tid = threadIdx.x;
     const int64_t b = blockIdx.y;
-    const T *q = a.q.p + b * a.q.sb + (h / a.q.group) * a.q.sh;
-    const T *k = a.k.p + b * a.k.sb + (h / a.k.group) * a.k.sh;
-    const T *v = a.v.p + b * a.v.sb + (h / a.v.group) * a.v.sh;
+    const T *q = (const T *)a.q.p + b * a.q.sb + (h / a.q.group) * a.q.sh;
+    const T *k = (const T *)a.k.p + b * a.k.sb + (h / a.k.group) * a.k.sh;
+    const T *v = (const T *)a.v.p + b * a.v.sb + (h / a.v.group) * a.v.sh;
     if (tid < a.Dk) {
         qs[tid] = to_float(q[tid]) * a.out_scale;
         ks[tid] = to_float(k[tid]);
@@ -226,6 +183,10 @@ int check_call(const pathsig_linattn *c) {
                   (long long)c->H, (long long)c->L);
         return PATHSIG_ERR_UNSUPPORTED;
     }
+    if (std::max({c->q_stride[1], c->k_stride[1], c->v_stride[1]}) > PATHSIG_MAX_TOKEN_STRIDE || c->H * std::max(c->Dk, c->Dv) > PATHSIG_MAX_TOKEN_STRIDE) {
+        set_error("tokens may be at most %d elements apart", PATHSIG_MAX_TOKEN_STRIDE);
+        return PATHSIG_ERR_UNSUPPORTED;
+    }
     for (int i = 0; i < 3; ++i)
         if (c->q_stride[i] < 0 || c->k_stride[i] < 0 || c->v_stride[i] < 0) {
             set_error("strides must not be negative");
@@ -238,21 +199,21 @@ int check_call(const pathsig_linattn *c) {
     return PATHSIG_OK;
 }
 
-template <typename T>
-View<T> view(const void *p, const int64_t *stride, int64_t group) {
-    return {(const T *)p, stride[0], stride[1], stride[2], (int)group};
+View view(const void *p, const int64_t *stride, int64_t group, int element) {
+    const int64_t E = 16 / element;
+    return {p, stride[0], stride[1], stride[2], (int)group, aligned16(p) && stride[0] % E == 0 && stride[1] % E == 0 && stride[2] % E == 0};
 }
 
-template <typename T>
-View<T> dense(const void *p, int64_t L, int64_t H, int64_t D) {
-    return {(const T *)p, L * H * D, H * D, D, 1};
+View dense(const void *p, int64_t L, int64_t H, int64_t D, int element) {
+    const int64_t stride[3] = {L * H * D, H * D, D};
+    return view(p, stride, 1, element);
 }
 
-template <typename T>
-Sweep<T> sweep(const pathsig_linattn *c) {
-    Sweep<T> a = {};
+Sweep sweep_of(const pathsig_linattn *c) {
+    Sweep a = {};
     a.log_decay = c->log_decay;
     a.lengths = c->lengths;
+    a.B = c->B;
     a.L = c->L;
     a.H = (int)c->H;
     a.Dk = (int)c->Dk;
@@ -262,29 +223,63 @@ Sweep<T> sweep(const pathsig_linattn *c) {
     return a;
 }
 
-template <typename T, typename O, bool REVERSE>
-void run_scan(const Sweep<T> &a, int64_t B, hipStream_t stream) {
-    scan_kernel<T, O, REVERSE><<<dim3((unsigned)ceil_div(a.Dv, 64), a.H, (unsigned)B), 64, 0, stream>>>(a);
+// Pieces of a sweep whose state has Dv columns: as many as bring the blocks to two for each of the 256 compute units, of whole
+// chunks, and not below 256 tokens, where what a piece costs (its state written and read, 4 Dk Dv bytes each) would be half of
+// what its tokens do.
+void cut(const pathsig_linattn *c, int64_t Dv, int64_t *piece, int *pieces) {
+    const int64_t blocks = c->B * c->H * ceil_div(Dv, 128);
+    const int64_t want = std::max<int64_t>(1, std::min(512 / std::max<int64_t>(blocks, 1), c->L / 256));
+    *piece = std::max<int64_t>(ceil_div(ceil_div(c->L, want), 64) * 64, 64);
+    *pieces = (int)std::max<int64_t>(ceil_div(c->L, *piece), 1);
+}
+
+size_t starts_bytes(const pathsig_linattn *c, int64_t Dv) {
+    int64_t piece;
+    int pieces;
+    cut(c, Dv, &piece, &pieces);
+    return pieces > 1 ? (size_t)pieces * c->B * c->H * c->Dk * c->Dv * sizeof(float) : 0;
+}
+
+template <typename T>
+void chunks(const Sweep &a, bool fold, hipStream_t stream) {
+    if (a.Dk <= 32) return launch_chunks<T, 1>(a, fold, stream);
+    if (a.Dk <= 64) return launch_chunks<T, 2>(a, fold, stream);
+    if (a.Dk <= 128) return launch_chunks<T, 4>(a, fold, stream);
+    launch_chunks<T, 8>(a, fold, stream);
+}
+
+// joined: `starts` already holds the states in front of the pieces
+template <typename T>
+void run_sweep(Sweep &a, const pathsig_linattn *c, float *starts, bool joined, hipStream_t stream) {
+    if (!joined) {
+        cut(c, a.Dv, &a.piece, &a.pieces);
+        a.starts = {starts, a.Dv, 1};
+        if (a.pieces > 1) {
+            chunks<T>(a, true, stream);
+            join_kernel<<<dim3((unsigned)ceil_div((int64_t)a.Dk * a.Dv, 256), a.H, (unsigned)a.B), 256, 0, stream>>>(a);
+        }
+    }
+    chunks<T>(a, false, stream);
 }
 
 template <typename T>
 int forward_t(const pathsig_linattn *c, const void *q, const void *k, const void *v, const float *state, void *out, float *final_state,
-              hipStream_t stream) {
-    Sweep<T> a = sweep<T>(c);
+              float *starts, hipStream_t stream) {
+    Sweep a = sweep_of(c);
     const int64_t group = c->H / c->Hkv;
-    a.q = view<T>(q, c->q_stride, 1);
-    a.k = view<T>(k, c->k_stride, group);
-    a.v = view<T>(v, c->v_stride, group);
+    a.q = view(q, c->q_stride, 1, sizeof(T));
+    a.k = view(k, c->k_stride, group, sizeof(T));
+    a.v = view(v, c->v_stride, group, sizeof(T));
     a.first = {const_cast<float *>(state), c->Dv, 1};
     a.last = {final_state, c->Dv, 1};
     a.out = out;
     a.out_scale = c->scale;
-    run_scan<T, T, false>(a, c->B, stream);
+    run_sweep<T>(a, c, starts, false, stream);
     return launch_status("linear attention");
 }
 
 struct BackwardLayout {
-    size_t wide_k, wide_v, decay, total;  // byte offsets
+    size_t starts, wide_k, wide_v, decay, total;  // byte offsets
 };
 
 size_t place(size_t &total, size_t bytes) {
@@ -296,6 +291,7 @@ size_t place(size_t &total, size_t bytes) {
 BackwardLayout backward_layout(const pathsig_linattn *c, bool want_decay) {
     BackwardLayout l = {};
     const size_t tokens = (size_t)c->B * c->L * c->H;
+    l.starts = place(l.total, std::max(starts_bytes(c, c->Dk), starts_bytes(c, c->Dv)));
     if (c->H != c->Hkv) {
         l.wide_k = place(l.total, tokens * c->Dk * sizeof(float));
         l.wide_v = place(l.total, tokens * c->Dv * sizeof(float));
@@ -309,11 +305,12 @@ int backward_t(const pathsig_linattn *c, const void *q, const void *k, const voi
                const float *grad_final, void *grad_q, void *grad_k, void *grad_v, float *grad_decay, float *grad_state, char *ws,
                hipStream_t stream) {
     const int64_t group = c->H / c->Hkv;
-    const View<T> vq = view<T>(q, c->q_stride, 1), vk = view<T>(k, c->k_stride, group), vv = view<T>(v, c->v_stride, group),
-                  vdo = dense<T>(grad_out, c->L, c->H, c->Dv);
+    const View vq = view(q, c->q_stride, 1, sizeof(T)), vk = view(k, c->k_stride, group, sizeof(T)),
+               vv = view(v, c->v_stride, group, sizeof(T)), vdo = dense(grad_out, c->L, c->H, c->Dv, sizeof(T));
     const BackwardLayout l = backward_layout(c, grad_decay != nullptr);
+    float *const starts = (float *)(ws + l.starts);
     // dq: the forward with (do, v, k) and the transposed state
-    Sweep<T> a = sweep<T>(c);
+    Sweep a = sweep_of(c);
     std::swap(a.Dk, a.Dv);
     a.q = vdo;
     a.k = vv;
@@ -321,32 +318,35 @@ int backward_t(const pathsig_linattn *c, const void *q, const void *k, const voi
     a.first = {const_cast<float *>(state), 1, c->Dv};
     a.out = grad_q;
     a.out_scale = c->scale;
-    run_scan<T, T, false>(a, c->B, stream);
+    run_sweep<T>(a, c, starts, false, stream);
     // dv: backwards in time with (k, q, do)
-    a = sweep<T>(c);
+    a = sweep_of(c);
     a.q = vk;
     a.k = vq;
     a.v = vdo;
     a.first = {const_cast<float *>(grad_final), c->Dv, 1};
     a.last = {grad_state, c->Dv, 1};
     a.in_scale = c->scale;
+    a.reverse = 1;
+    a.out_float = group > 1;
     a.out = group > 1 ? (void *)(ws + l.wide_v) : grad_v;
-    if (group > 1)
-        run_scan<T, float, true>(a, c->B, stream);
-    else
-        run_scan<T, T, true>(a, c->B, stream);
+    run_sweep<T>(a, c, starts, false, stream);
     // dk: backwards in time with (v, do, q) and the transposed gradient of the state
-    std::swap(a.Dk, a.Dv);
-    a.q = vv;
-    a.k = vdo;
-    a.v = vq;
-    a.first = {const_cast<float *>(grad_final), 1, c->Dv};
-    a.last = {nullptr, 0, 0};
-    a.out = group > 1 ? (void *)(ws + l.wide_k) : grad_k;
-    if (group > 1)
-        run_scan<T, float, true>(a, c->B, stream);
-    else
-        run_scan<T, T, true>(a, c->B, stream);
+    Sweep k_sweep = a;
+    std::swap(k_sweep.Dk, k_sweep.Dv);
+    k_sweep.q = vv;
+    k_sweep.k = vdo;
+    k_sweep.v = vq;
+    k_sweep.first = {const_cast<float *>(grad_final), 1, c->Dv};
+    k_sweep.last = {nullptr, 0, 0};
+    k_sweep.out = group > 1 ? (void *)(ws + l.wide_k) : grad_k;
+    // the states in front of the pieces are those of dv, transposed, as long as both are cut alike
+    int64_t piece;
+    int pieces;
+    cut(c, c->Dk, &piece, &pieces);
+    const bool joined = piece == a.piece;
+    if (joined) k_sweep.starts = {starts, 1, c->Dv};
+    run_sweep<T>(k_sweep, c, starts, joined, stream);
     if (group > 1) {
         const int64_t rows = c->B * c->L;
         const unsigned blocks_k = (unsigned)std::min<int64_t>(ceil_div(rows * c->Hkv * c->Dk, 256), 4096);
@@ -355,7 +355,7 @@ int backward_t(const pathsig_linattn *c, const void *q, const void *k, const voi
         group_sum_kernel<T><<<blocks_v, 256, 0, stream>>>((const float *)(ws + l.wide_v), (T *)grad_v, rows, (int)c->Hkv, (int)group, (int)c->Dv);
     }
     if (grad_decay) {
-        a = sweep<T>(c);
+        a = sweep_of(c);
         a.q = vq;
         a.k = vk;
         a.v = vv;
@@ -371,11 +371,11 @@ int backward_t(const pathsig_linattn *c, const void *q, const void *k, const voi
 
 template <typename T>
 int step_t(const pathsig_linattn *c, const void *q, const void *k, const void *v, float *state, void *out, hipStream_t stream) {
-    Sweep<T> a = sweep<T>(c);
+    Sweep a = sweep_of(c);
     const int64_t group = c->H / c->Hkv;
-    a.q = view<T>(q, c->q_stride, 1);
-    a.k = view<T>(k, c->k_stride, group);
-    a.v = view<T>(v, c->v_stride, group);
+    a.q = view(q, c->q_stride, 1, sizeof(T));
+    a.k = view(k, c->k_stride, group, sizeof(T));
+    a.v = view(v, c->v_stride, group, sizeof(T));
     a.out = out;
     a.out_scale = c->scale;
     const dim3 grid((unsigned)c->H, (unsigned)c->B);
@@ -400,7 +400,7 @@ extern "C" {
 
 size_t pathsig_linattn_forward_workspace(const pathsig_linattn *call) {
     if (check_call(call) != PATHSIG_OK) return 0;
-    return 0;
+    return starts_bytes(call, call->Dv);
 }
 
 int pathsig_linattn_forward(const pathsig_linattn *call, const void *q, const void *k, const void *v, const float *state,
@@ -416,8 +416,8 @@ int pathsig_linattn_forward(const pathsig_linattn *call, const void *q, const vo
         set_error("linear attention: workspace of %zu bytes needed, got %zu", need, workspace ? workspace_bytes : (size_t)0);
         return PATHSIG_ERR_WORKSPACE;
     }
-    if (call->dtype == PATHSIG_F32) return forward_t<float>(call, q, k, v, state, out, final_state, (hipStream_t)stream);
-    return forward_t<bf16>(call, q, k, v, state, out, final_state, (hipStream_t)stream);
+    if (call->dtype == PATHSIG_F32) return forward_t<float>(call, q, k, v, state, out, final_state, (float *)workspace, (hipStream_t)stream);
+    return forward_t<bf16>(call, q, k, v, state, out, final_state, (float *)workspace, (hipStream_t)stream);
 }
 
 size_t pathsig_linattn_backward_workspace(const pathsig_linattn *call, int want_log_decay) {

@@ -1,0 +1,62 @@
+// Sweeps of linear attention over whole sequences: what the entry points (seq_attention.hip) and the kernels of the chunked form
+// (seq_chunks.hip, compiled once for each width of the keys) share.
+#pragma once
+
+#include "seq_common.hpp"
+
+namespace psig {
+namespace seq {
+
+// a [B, L, heads, D] tensor; heads[h / group] is read for head h
+struct View {
+    const void *p;
+    int64_t sb, st, sh;
+    int group;
+    int vectors;  // rows start at multiples of 16 bytes
+};
+
+struct StateRef {
+    float *p;  // [B, H, Dk * Dv]; element (a, c) of a head at a * row + c * column
+    int64_t row, column;
+};
+
+// One pass of the recurrence over all tokens, S <- decay S + in_scale k v^T, out = out_scale S^T q, or backwards in time, where
+// the decay comes after the token: S <- S + in_scale k v^T, out = out_scale S^T q, S <- decay S.  Dk and Dv are the rows and
+// columns of this pass' state, whichever tensors are in the places of k and v.
+struct Sweep {
+    View q, k, v;
+    StateRef first, last;  // p may be NULL
+    void *out;             // [B, L, H, Dv] dense
+    int out_float;         // float32 instead of the type of q
+    const float *log_decay;
+    const int32_t *lengths;
+    int64_t B, L;
+    int H, Dk, Dv;
+    float in_scale, out_scale;
+    int reverse;
+    // the sequence in pieces of `piece` tokens: states in front of each, [pieces][B][H][Dk * Dv], in first's order of rows
+    // and columns of `starts`
+    int64_t piece;
+    int pieces;
+    StateRef starts;
+};
+
+__device__ __forceinline__ int64_t length_of(const int32_t *lengths, int64_t b, int64_t L) {
+    if (!lengths) return L;
+    const int64_t n = lengths[b];
+    return n < 0 ? 0 : n > L ? L : n;
+}
+
+__device__ __forceinline__ float decay_of(const float *log_decay, int h) {
+    // (minus infinity forgets everything at once; a finite stand-in keeps 0 * g at 0)
+    return fmaxf(log_decay[h], -1e30f);
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// seq_chunks.hip, for keys of up to 32 DKT channels.  fold: only the states that the pieces add, from zero, into starts[s + 1].
+template <typename T, int DKT>
+void launch_chunks(const Sweep &a, bool fold, hipStream_t stream);
+
+}  // namespace seq
+}  // namespace psig

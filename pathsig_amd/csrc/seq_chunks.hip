@@ -1,0 +1,473 @@
+// Linear attention over whole sequences in chunks, on matrix instructions.
+//
+// In a chunk of C tokens that starts from the state S, with l = e^g and token i of the chunk counted from 0:
+//     o_i = l^(i+1) S^T q_i + sum over j <= i of l^(i-j) (q_i . k_j) v_j,
+//     S' = l^C S + sum over j of l^(C-1-j) k_j v_j^T.
+// Backwards in time the decay comes after the token: exponents i and C - j in place of i + 1 and C - 1 - j.
+//
+// A block has a head of a sequence (or of a piece of it) and up to 128 columns of its state; wave w has the 32 columns from
+// 32 w on, its part of the state in accumulator registers from the first chunk to the last.  All products are 32 x 32 tiles
+// laid out so that nothing crosses lanes:
+//   * scores transposed, K Q^T: a lane has one token i and sixteen j.  Decays and the causal mask are then factors of a lane's
+//     registers, and the rounded scores are, as they stand, the right operand of V^T P;
+//   * answers transposed, S^T Q^T + V^T P: the state's accumulators, rounded, are, as they stand, the left operand;
+//   * an accumulator holds rows 8 (r / 4) + 4 (lane / 32) + r % 4.  Operands are read in that order of the contracted index
+//     ("accumulator order"): Q and K rows from LDS, where the channels of 16 are stored so that a lane's eight lie side by side,
+//     V^T and K^T with transposing reads of four rows each.
+// The scores are computed by every wave (a quarter of its matrix instructions) instead of exchanged through LDS behind a
+// barrier.  Rounding in bf16: scores and the state's copy to bf16 for the products with V and Q (relative 2^-8 a term, like the
+// rounding of the answers), the state itself and what is added to it stay in 32 bits: l^(C-1-j) v_j is split into three bf16
+// terms, which hold all 24 bits.
+//
+// A first chunk that is not full is filled from the front with tokens of zeros, so that the factors l^(C-1-j) hold for every
+// chunk and none of them is a quotient.
+#include <algorithm>
+
+#include "seq_attention.hpp"
+
+namespace psig {
+namespace seq {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// eight elements of an operand, a lane's share of sixteen steps of the contracted index
+template <typename T>
+struct FragOf;
+template <>
+struct FragOf<bf16> {
+    using type = bf16x8;
+};
+template <>
+struct FragOf<float> {
+    using type = f32x8;
+};
+template <typename T>
+using Frag = typename FragOf<T>::type;
+
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(f32x8 a, f32x8 b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+}
+
+template <typename T>
+__device__ __forceinline__ Frag<T> rounded(f32x8 x) {
+    return __builtin_convertvector(x, Frag<T>);
+}
+__device__ __forceinline__ f32x8 widened(bf16x8 x) { return __builtin_convertvector(x, f32x8); }
+__device__ __forceinline__ f32x8 widened(f32x8 x) { return x; }
+
+template <int Half>
+__device__ __forceinline__ f32x8 half_of(f32x16 x) {
+    if constexpr (Half == 0)
+        return __builtin_shufflevector(x, x, 0, 1, 2, 3, 4, 5, 6, 7);
+    else
+        return __builtin_shufflevector(x, x, 8, 9, 10, 11, 12, 13, 14, 15);
+}
+
+// row of accumulator register r
+__device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r / 4) + 4 * half + r % 4; }
+
+// A tile of rows of D channels in LDS, in units of 16 bytes.  Units of a row are exchanged by a pattern of the row number: rows
+// read at one unit by 16 lanes, and four neighbouring rows read at 64 neighbouring bytes (the transposing reads), each fall
+// into different banks.  The pattern repeats after 16 rows, so every address is a lane's base, exclusive-or a constant, plus a
+// constant.
+template <typename T, int D>
+struct Tile;
+
+template <int D>
+struct Tile<bf16, D> {
+    static constexpr int kUnits = D / 8, kPerUnit = 8, kRow = D * 2, kColumnBases = 2;
+    static __device__ __forceinline__ int swizzle(int row) {
+        if constexpr (kUnits >= 16) return ((row & 3) << 2) | ((row >> 2) & 3);
+        if constexpr (kUnits == 8) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+        return (row >> 2) & 3;
+    }
+    // Channels of a group of sixteen are stored in fours as 0, 2 | 1, 3: a unit is what one half of the lanes contracts
+    static __device__ __forceinline__ void store(char *lds, int row, int unit, u32x4 x) {
+        const int at = row * kRow + (((unit & ~1) ^ swizzle(row)) * 16) + (unit & 1) * 8;
+        *(u32x2 *)(lds + at) = u32x2{x[0], x[1]};
+        *(u32x2 *)(lds + (at ^ 16)) = u32x2{x[2], x[3]};
+    }
+    static __device__ __forceinline__ int row_base(int ln, int half) { return ln * kRow + ((half ^ swizzle(ln)) * 16); }
+    // channels 16 kk .. 16 kk + 15 of row 32 tile + lane % 32, in accumulator order
+    static __device__ __forceinline__ bf16x8 row(const char *lds, int base, int tile, int kk) {
+        return *(const bf16x8 *)(lds + (base ^ (kk * 32)) + tile * 32 * kRow);
+    }
+    // (a group of sixteen lanes reads four rows of sixteen channels, each lane four channels of one row, and gets four rows of one
+    // channel)
+    static __device__ __forceinline__ void column_bases(int (&base)[kColumnBases], int lane) {
+        const int half = lane >> 5, part = (lane >> 4) & 1, r = (lane & 15) >> 2, four = lane & 3;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const int j = 8 * g + 4 * half + r;
+            base[g] = j * kRow + (((2 * part + (four & 1)) ^ swizzle(j)) * 16) + (four >> 1) * 8;
+        }
+    }
+    // channel 32 m + lane % 32 of rows 16 kk .. 16 kk + 15, in accumulator order
+    static __device__ __forceinline__ bf16x8 column(const char *lds, const int (&base)[kColumnBases], int m, int kk) {
+        s16x4 got[2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const char *const p = lds + (base[g] ^ (m * 64)) + kk * 16 * kRow;
+            got[g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
+        }
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(got[0], got[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+};
+
+template <int D>
+struct Tile<float, D> {
+    static constexpr int kUnits = D / 4, kPerUnit = 4, kRow = D * 4, kColumnBases = 1;
+    static __device__ __forceinline__ constexpr int swizzle(int row) {
+        return (((row & 4) << 1) | ((row & 8) >> 1) | (row & 3)) & (kUnits - 1);
+    }
+    static __device__ __forceinline__ void store(char *lds, int row, int unit, u32x4 x) {
+        *(u32x4 *)(lds + row * kRow + ((unit ^ swizzle(row)) * 16)) = x;
+    }
+    static __device__ __forceinline__ int row_base(int ln, int half) { return ln * kRow + ((half ^ swizzle(ln)) * 16); }
+    static __device__ __forceinline__ f32x8 row(const char *lds, int base, int tile, int kk) {
+        const f32x4 a = *(const f32x4 *)(lds + (base ^ (kk * 64)) + tile * 32 * kRow);
+        const f32x4 b = *(const f32x4 *)(lds + (base ^ (kk * 64 + 32)) + tile * 32 * kRow);
+        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    static __device__ __forceinline__ void column_bases(int (&base)[kColumnBases], int lane) {
+        const int ln = lane & 31, half = lane >> 5;
+        base[0] = 4 * half * kRow + (((ln >> 2) ^ swizzle(4 * half)) * 16) + (ln & 3) * 4;
+    }
+    static __device__ __forceinline__ f32x8 column(const char *lds, const int (&base)[kColumnBases], int m, int kk) {
+        f32x8 x;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int j = acc_row(e, 0);
+            x[e] = *(const float *)(lds + (base[0] ^ (m * 128) ^ (swizzle(j) * 16)) + (16 * kk + j) * kRow);
+        }
+        return x;
+    }
+};
+
+// The units of a tile of ROWS rows that one of THREADS threads fetches: registers between the load from memory and the store to
+// LDS.
+template <typename T, int D, int ROWS, int THREADS>
+struct Fetch {
+    using L = Tile<T, D>;
+    static constexpr int kTotal = ROWS * L::kUnits, kEach = (kTotal + THREADS - 1) / THREADS;
+    static constexpr int kRowsApart = THREADS / L::kUnits;  // rows between a thread's units
+    static_assert(THREADS % L::kUnits == 0, "a thread's units lie in one column");
+    u32x4 x[kEach];
+
+    // p: the tile's first row and channel.  The rows before `pad` are zeros and not read, as are channels from `channels` on.
+    // st: from row to row, backwards in time negative.
+    __device__ __forceinline__ void load(const T *p, int st, int channels, int vectors, int pad) {
+        const int row0 = threadIdx.x / L::kUnits, c = threadIdx.x % L::kUnits * L::kPerUnit;
+        const int offset = row0 * st + c;
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+            const int row = row0 + u * kRowsApart;
+            x[u] = u32x4{0, 0, 0, 0};
+            if ((kTotal % THREADS && row >= ROWS) || row < pad || c >= channels) continue;
+            const T *const q = p + (int64_t)u * kRowsApart * st + offset;
+            if (vectors) {
+                x[u] = *(const u32x4 *)q;
+            } else {
+                Pack<T, L::kPerUnit> one = {};
+#pragma unroll
+                for (int e = 0; e < L::kPerUnit; ++e)
+                    if (c + e < channels) one.v[e] = q[e];
+                x[u] = __builtin_bit_cast(u32x4, one);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(char *lds) const {
+        const int row0 = threadIdx.x / L::kUnits, unit = threadIdx.x % L::kUnits;
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+            const int row = row0 + u * kRowsApart;
+            if (kTotal % THREADS && row >= ROWS) continue;
+            L::store(lds, row, unit, x[u]);
+        }
+    }
+};
+
+// l^(C-1-j) v_j in terms of the type of the products: all bits of it (three of bf16)
+template <typename T>
+struct Terms;
+template <>
+struct Terms<float> {
+    static constexpr int kCount = 1;
+    static __device__ __forceinline__ void split(f32x8 x, f32x8 (&out)[1]) { out[0] = x; }
+};
+template <>
+struct Terms<bf16> {
+    static constexpr int kCount = 3;
+    static __device__ __forceinline__ void split(f32x8 x, bf16x8 (&out)[3]) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            out[i] = rounded<bf16>(x);
+            x -= widened(out[i]);
+        }
+    }
+};
+
+// Bytes that a thread fetches of a chunk of 32 tiles tokens.
+constexpr int fetched(int element, int tiles, int DKT, int NW) { return 32 * tiles * (2 * 32 * DKT + 32 * NW) * element / (64 * NW); }
+
+// 64 tokens in bf16, half as many where a thread would fetch more than 320 bytes of a chunk, and in fp32, where it is twice as
+// many bytes
+template <typename T>
+constexpr int chunk_tiles(int DKT, int NW) {
+    return sizeof(T) == 2 && fetched(2, 2, DKT, NW) <= 320 ? 2 : 1;
+}
+
+template <typename T, typename O, int DKT, int NW, bool FOLD>
+__global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_kernel(const Sweep a, int slices) {
+    constexpr int DK = 32 * DKT, DV = 32 * NW, CT = chunk_tiles<T>(DKT, NW), C = 32 * CT, THREADS = 64 * NW;
+    // fetched a chunk ahead, where registers allow it
+    constexpr bool kAhead = fetched(sizeof(T), CT, DKT, NW) <= 320;
+    using KTile = Tile<T, DK>;
+    using VTile = Tile<T, DV>;
+    constexpr int kKBytes = C * KTile::kRow, kVBytes = C * VTile::kRow;
+    __shared__ __align__(16) char lds[kKBytes * (FOLD ? 1 : 2) + kVBytes];
+    __shared__ __align__(16) f32x4 table_later[4][2], table_diagonal[FOLD ? 1 : 4][64];
+    char *const lds_k = lds, *const lds_v = lds + kKBytes, *const lds_q = lds_v + kVBytes;
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, ln = lane & 31;
+    const int slice = blockIdx.x % slices, h = blockIdx.x / slices, piece = blockIdx.y;
+    const int64_t b = blockIdx.z;
+    const int dv0 = slice * DV, dv = dv0 + 32 * wave + ln;  // this lane's column of the state
+    const int64_t n = length_of(a.lengths, b, a.L);
+    const int64_t begin = piece * a.piece, end = min(begin + a.piece, n);
+    const float g2 = decay_of(a.log_decay, h) * kLog2e;
+    const int64_t plane = (int64_t)a.Dk * a.Dv, head = (b * a.H + h) * plane;
+
+    if (!FOLD) {
+        // tokens behind the end of the sequence
+        const int64_t z0 = max(n, begin), z1 = min(begin + a.piece, a.L);
+        const int width = min(DV, a.Dv - dv0);
+        for (int64_t t = z0 + wave; t < z1; t += NW)
+            for (int c = lane; c < width; c += 64) ((O *)a.out)[((b * a.L + t) * a.H + h) * a.Dv + dv0 + c] = from_float<O>(0.f);
+    }
+    const bool owns_end = !FOLD && a.last.p && (end == n && (begin < n || piece == 0));
+    if (begin >= end && !owns_end && !FOLD) return;
+
+    f32x16 S[DKT];
+    {
+        const float *from = nullptr;
+        int64_t row = 0, column = 0;
+        if (!FOLD && a.pieces > 1) {
+            from = a.starts.p + (int64_t)piece * a.B * a.H * plane + head;
+            row = a.starts.row;
+            column = a.starts.column;
+        } else if (!FOLD && a.first.p) {
+            from = a.first.p + head;
+            row = a.first.row;
+            column = a.first.column;
+        }
+#pragma unroll
+        for (int t = 0; t < DKT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int dk = 32 * t + acc_row(r, half);
+                S[t][r] = from && dk < a.Dk && dv < a.Dv ? from[dk * row + dv * column] : 0.f;
+            }
+    }
+
+    // factors of a lane's registers: l^(31 - j), and l^(i - j) in a tile on the diagonal (j after i is masked where it is used).  In
+    // LDS: 32 registers that are read once a chunk
+    if (threadIdx.x < 64) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int j = acc_row(r, half);
+            if (ln == 0) table_later[r / 4][half][r % 4] = exp2f(g2 * (float)(31 - j));
+            if constexpr (!FOLD) table_diagonal[r / 4][lane][r % 4] = a.in_scale * exp2f(g2 * (float)max(ln - j, 0));
+        }
+    }
+    const float since = a.in_scale * exp2f(g2 * (float)(ln + 1));
+
+    const T *const kp = (const T *)a.k.p + b * a.k.sb + (h / a.k.group) * a.k.sh;
+    const T *const vp = (const T *)a.v.p + b * a.v.sb + (h / a.v.group) * a.v.sh + dv0;
+    const T *const qp = FOLD ? nullptr : (const T *)a.q.p + b * a.q.sb + (h / a.q.group) * a.q.sh;
+    const int sign = a.reverse ? -1 : 1;
+    Fetch<T, DK, C, THREADS> fk, fq;
+    Fetch<T, DV, C, THREADS> fv;
+    const int chunks = (int)((max(end - begin, (int64_t)0) + C - 1) / C);
+    int64_t r0 = end - (int64_t)chunks * C;  // of the chunk being worked on; before `begin` where the first is not full
+    auto fetch = [&](int64_t at, int pad) {
+        const int64_t t = a.reverse ? n - 1 - at : at;
+        fk.load(kp + t * a.k.st, sign * (int)a.k.st, a.Dk, a.k.vectors, pad);
+        if (!kAhead) fk.store(lds_k);
+        fv.load(vp + t * a.v.st, sign * (int)a.v.st, a.Dv - dv0, a.v.vectors, pad);
+        if (!kAhead) fv.store(lds_v);
+        if (!FOLD) fq.load(qp + t * a.q.st, sign * (int)a.q.st, a.Dk, a.q.vectors, pad);
+        if (!kAhead && !FOLD) fq.store(lds_q);
+    };
+    if (kAhead && chunks > 0) fetch(r0, (int)(begin - r0));
+    const int row_base_of_lane = KTile::row_base(ln, half);
+    int k_bases_of_lane[KTile::kColumnBases], v_bases_of_lane[VTile::kColumnBases];
+    KTile::column_bases(k_bases_of_lane, lane);
+    VTile::column_bases(v_bases_of_lane, lane);
+    for (int c = 0; c < chunks; ++c, r0 += C) {
+        const int pad = (int)max(begin - r0, (int64_t)0);
+        __syncthreads();  // the tiles of the chunk before are read
+        if (kAhead) {
+            fk.store(lds_k);
+            fv.store(lds_v);
+            if (!FOLD) fq.store(lds_q);
+        } else {
+            fetch(r0, pad);
+        }
+        __syncthreads();
+        if (kAhead && c + 1 < chunks) fetch(r0 + C, 0);
+
+        // (addresses are worked out from these in every chunk: held for all reads, they would fill the registers)
+        int row_base = row_base_of_lane, k_bases[KTile::kColumnBases], v_bases[VTile::kColumnBases];
+        asm volatile("" : "+v"(row_base));
+#pragma unroll
+        for (int g = 0; g < KTile::kColumnBases; ++g) {
+            k_bases[g] = k_bases_of_lane[g];
+            v_bases[g] = v_bases_of_lane[g] ^ (wave * 32 * (int)sizeof(T));
+            asm volatile("" : "+v"(k_bases[g]), "+v"(v_bases[g]));
+        }
+
+        if constexpr (!FOLD) {
+#pragma unroll
+            for (int i = 0; i < CT; ++i) {
+                f32x16 P[CT], out = f32x16{};
+#pragma unroll
+                for (int j = 0; j <= i; ++j) P[j] = f32x16{};
+#pragma unroll
+                for (int kk = 0; kk < DK / 16; ++kk) {
+                    const Frag<T> q = KTile::row(lds_q, row_base, i, kk);
+                    const Frag<T> st = rounded<T>(kk % 2 ? half_of<1>(S[kk / 2]) : half_of<0>(S[kk / 2]));
+                    out = mma(st, q, out);
+#pragma unroll
+                    for (int j = 0; j <= i; ++j) P[j] = mma(KTile::row(lds_k, row_base, j, kk), q, P[j]);
+                    if (kk % 2) __builtin_amdgcn_sched_barrier(0);  // operands of a few steps ahead fill the registers
+                }
+                // (rows of padding have answers that no one reads; their exponent is kept from turning around)
+                out *= exp2f(g2 * (float)max(32 * i + ln + 1 - a.reverse - pad, 0));
+#pragma unroll
+                for (int j = 0; j <= i; ++j) {
+#pragma unroll
+                    for (int r4 = 0; r4 < 4; ++r4) {
+                        const f32x4 f = j == i ? table_diagonal[r4][lane] : table_later[r4][half] * since;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int r = 4 * r4 + e;
+                            P[j][r] *= f[e];
+                            // (selected, not multiplied by zero: a score of a later token may be infinite)
+                            if (j == i && acc_row(r, half) > ln) P[j][r] = 0.f;
+                        }
+                    }
+                    out = mma(VTile::column(lds_v, v_bases, 0, 2 * j), rounded<T>(half_of<0>(P[j])), out);
+                    out = mma(VTile::column(lds_v, v_bases, 0, 2 * j + 1), rounded<T>(half_of<1>(P[j])), out);
+                }
+                const int row = 32 * i + ln;
+                if (row >= pad) {
+                    const int64_t t = a.reverse ? n - 1 - (r0 + row) : r0 + row;
+                    O *const to = (O *)a.out + ((b * a.L + t) * a.H + h) * a.Dv;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int d = dv0 + 32 * wave + 8 * g + 4 * half;
+                        if (a.Dv % 4 == 0) {
+                            if (d < a.Dv) {
+                                Pack<O, 4> four;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) four.v[e] = from_float<O>(out[4 * g + e] * a.out_scale);
+                                *(Pack<O, 4> *)(to + d) = four;
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (d + e < a.Dv) to[d + e] = from_float<O>(out[4 * g + e] * a.out_scale);
+                        }
+                    }
+                }
+            }
+        }
+
+        // the state after the chunk
+        const float whole = exp2f(g2 * (float)(C - pad));
+#pragma unroll
+        for (int t = 0; t < DKT; ++t) S[t] *= whole;
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+            const float rest = a.in_scale * exp2f(g2 * (float)(32 * (CT - 1 - j) + a.reverse));
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                f32x8 x = widened(VTile::column(lds_v, v_bases, 0, 2 * j + s));
+#pragma unroll
+                for (int r4 = 0; r4 < 2; ++r4) {
+                    const f32x4 f = table_later[2 * s + r4][half] * rest;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[4 * r4 + e] *= f[e];
+                }
+                Frag<T> terms[Terms<T>::kCount];
+                Terms<T>::split(x, terms);
+#pragma unroll
+                for (int t = 0; t < DKT; ++t) {
+                    const Frag<T> kt = KTile::column(lds_k, k_bases, t, 2 * j + s);
+#pragma unroll
+                    for (int i = 0; i < Terms<T>::kCount; ++i) S[t] = mma(kt, terms[i], S[t]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+
+    float *to = nullptr;
+    int64_t row = 0, column = 0;
+    if (FOLD) {
+        to = a.starts.p + (int64_t)(piece + 1) * a.B * a.H * plane + head;
+        row = a.starts.row;
+        column = a.starts.column;
+    } else if (owns_end) {
+        to = a.last.p + head;
+        row = a.last.row;
+        column = a.last.column;
+    }
+    if (!to) return;
+#pragma unroll
+    for (int t = 0; t < DKT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int dk = 32 * t + acc_row(r, half);
+            if (dk < a.Dk && dv < a.Dv) to[dk * row + dv * column] = S[t][r];
+        }
+}
+
+template <typename T, int DKT, int NW>
+void launch_width(const Sweep &a, bool fold, hipStream_t stream) {
+    const int slices = (int)ceil_div(a.Dv, 32 * NW);
+    const dim3 grid((unsigned)(slices * a.H), (unsigned)(fold ? a.pieces - 1 : a.pieces), (unsigned)a.B), block(64 * NW);
+    if (fold)
+        chunk_kernel<T, T, DKT, NW, true><<<grid, block, 0, stream>>>(a, slices);
+    else if (a.out_float && sizeof(T) == 2)
+        chunk_kernel<T, float, DKT, NW, false><<<grid, block, 0, stream>>>(a, slices);
+    else
+        chunk_kernel<T, T, DKT, NW, false><<<grid, block, 0, stream>>>(a, slices);
+}
+
+}  // namespace
+
+template <typename T, int DKT>
+void launch_chunks(const Sweep &a, bool fold, hipStream_t stream) {
+    if (a.Dv <= 32) return launch_width<T, DKT, 1>(a, fold, stream);
+    if (a.Dv <= 64) return launch_width<T, DKT, 2>(a, fold, stream);
+    launch_width<T, DKT, 4>(a, fold, stream);
+}
+
+template void launch_chunks<float, PSIG_KEY_TILES>(const Sweep &, bool, hipStream_t);
+template void launch_chunks<bf16, PSIG_KEY_TILES>(const Sweep &, bool, hipStream_t);
+
+}  // namespace seq
+}  // namespace psig

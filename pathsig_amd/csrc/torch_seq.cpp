@@ -28,8 +28,11 @@ void check_like(const Tensor &t, const char *what, const Tensor &like, const cha
     TORCH_CHECK(t.device() == like.device(), what, " must be on the device of ", like_name);
 }
 
-// the channels of a head side by side
-Tensor side_by_side(const Tensor &t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+// the channels of a head side by side, and tokens no further apart than the kernels' offsets reach
+Tensor side_by_side(const Tensor &t) {
+    const bool near = t.dim() < 4 || t.stride(1) <= PATHSIG_MAX_TOKEN_STRIDE;
+    return near && (t.size(-1) == 1 || t.stride(-1) == 1) ? t : t.contiguous();
+}
 
 // ---- linear attention ---------------------------------------------------------------------------------------------
 struct AttentionCall {
