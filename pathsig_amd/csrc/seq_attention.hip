@@ -4,7 +4,7 @@
 // Recurrence of a head, state S [Dk, Dv]:  S_t = e^g S_(t-1) + k_t v_t^T,  o_t = scale S_t^T q_t.
 // Gradients, with R_t = dL/dS_t through the outputs from t on:  R_t = e^g R_(t+1) + scale q_t do_t^T,
 //   dq_t = scale S_t do_t,   dk_t = R_t v_t,   dv_t = R_t^T k_t,   dS_(-1) = e^g R_0,
-//   dg = sum over t of scale do_t^T T_t^T q_t with T_t = dS_t/dg = e^g (T_(t-1) + S_(t-1)), and <dS_end, T_end>.
+//   dg = sum over t of e^g <S_(t-1), R_t>, worked out inside chunks and pieces as seq_chunks.hip says.
 // So all three gradients are the forward's recurrence with other tensors in the places of q, k and v: dq with (do, v, k),
 // dv backwards in time with (k, q, do), dk backwards in time with (v, do, q).
 //
@@ -33,51 +33,12 @@ __global__ __launch_bounds__(256) void join_kernel(const Sweep a) {
     float *const p = a.starts.p + head + i;
     float x = a.first.p ? a.first.p[head + at] : 0.f;
     p[0] = x;
-    const float full = exp2f(g2 * (float)a.piece);
 #pragma unroll 8
     for (int s = 1; s < a.pieces; ++s) {
-        const int64_t left = n - (s - 1) * a.piece;  // tokens from the piece before on
-        x = x * (left >= a.piece ? full : left > 0 ? exp2f(g2 * (float)left) : 1.f) + p[s * stride];
+        const Range before = range_of(a, n, s - 1);
+        x = x * exp2f(g2 * (float)(before.end - before.begin)) + p[s * stride];
         p[s * stride] = x;
     }
-}
-
-// dL/dg: the state and its derivative side by side.
-template <typename T>
-__global__ __launch_bounds__(32) void decay_scan_kernel(const Sweep a, const T *grad_out, const float *grad_final, float *partial) {
-    __shared__ float S[PATHSIG_MAX_HEAD_DIM][32], D[PATHSIG_MAX_HEAD_DIM][32];
-    const int lane = threadIdx.x, h = blockIdx.y;
-    const int64_t b = blockIdx.z;
-    const int c = blockIdx.x * 32 + lane;
-    const bool mine = c < a.Dv;
-    const int64_t n = length_of(a.lengths, b, a.L);
-    const float decay = expf(decay_of(a.log_decay, h));
-    const int64_t head = (b * a.H + h) * a.Dk * a.Dv;
-    for (int r = 0; r < a.Dk; ++r) {
-        S[r][lane] = mine && a.first.p ? a.first.p[head + (int64_t)r * a.Dv + c] : 0.f;
-        D[r][lane] = 0.f;
-    }
-    const T *q = (const T *)a.q.p + b * a.q.sb + (h / a.q.group) * a.q.sh;
-    const T *k = (const T *)a.k.p + b * a.k.sb + (h / a.k.group) * a.k.sh;
-    const T *v = (const T *)a.v.p + b * a.v.sb + (h / a.v.group) * a.v.sh;
-    double total = 0;
-    for (int64_t t = 0; t < n; ++t) {
-        const float vc = mine ? to_float(v[t * a.v.st + c]) : 0.f;
-        const float go = mine ? to_float(grad_out[((b * a.L + t) * a.H + h) * a.Dv + c]) * a.out_scale : 0.f;
-        float o = 0.f;
-        for (int r = 0; r < a.Dk; ++r) {
-            const float s = S[r][lane], d = decay * (D[r][lane] + s);
-            D[r][lane] = d;
-            S[r][lane] = s * decay + to_float(k[t * a.k.st + r]) * vc;
-            o += to_float(q[t * a.q.st + r]) * d;
-        }
-        total += o * go;
-    }
-    if (grad_final && mine)
-        for (int r = 0; r < a.Dk; ++r) total += D[r][lane] * grad_final[head + (int64_t)r * a.Dv + c];
-    float sum = (float)total;
-    for (int m = 1; m < 32; m <<= 1) sum += __shfl_xor(sum, m);
-    if (lane == 0) partial[((int64_t)blockIdx.x * gridDim.z + b) * a.H + h] = sum;
 }
 
 __global__ void decay_sum_kernel(const float *partial, int64_t rows, int H, float *out) {
@@ -209,6 +170,23 @@ View dense(const void *p, int64_t L, int64_t H, int64_t D, int element) {
     return view(p, stride, 1, element);
 }
 
+// Pieces of a call's sweeps, the same for all of them: as many as bring the blocks to two for each of the 256 compute units, of whole
+// chunks, and not below 256 tokens, where what a piece costs (its state written and read, 4 Dk Dv bytes each) would be half of
+// what its tokens do.
+void cut(const pathsig_linattn *c, int64_t *piece, int *pieces) {
+    const int64_t blocks = c->B * c->H;
+    const int64_t want = std::max<int64_t>(1, std::min(512 / std::max<int64_t>(blocks, 1), c->L / 256));
+    *piece = std::max<int64_t>(ceil_div(ceil_div(c->L, want), 64) * 64, 64);
+    *pieces = (int)std::max<int64_t>(ceil_div(c->L, *piece), 1);
+}
+
+size_t starts_bytes(const pathsig_linattn *c) {
+    int64_t piece;
+    int pieces;
+    cut(c, &piece, &pieces);
+    return pieces > 1 ? (size_t)pieces * c->B * c->H * c->Dk * c->Dv * sizeof(float) : 0;
+}
+
 Sweep sweep_of(const pathsig_linattn *c) {
     Sweep a = {};
     a.log_decay = c->log_decay;
@@ -220,24 +198,8 @@ Sweep sweep_of(const pathsig_linattn *c) {
     a.Dv = (int)c->Dv;
     a.in_scale = 1.f;
     a.out_scale = 1.f;
+    cut(c, &a.piece, &a.pieces);
     return a;
-}
-
-// Pieces of a sweep whose state has Dv columns: as many as bring the blocks to two for each of the 256 compute units, of whole
-// chunks, and not below 256 tokens, where what a piece costs (its state written and read, 4 Dk Dv bytes each) would be half of
-// what its tokens do.
-void cut(const pathsig_linattn *c, int64_t Dv, int64_t *piece, int *pieces) {
-    const int64_t blocks = c->B * c->H * ceil_div(Dv, 128);
-    const int64_t want = std::max<int64_t>(1, std::min(512 / std::max<int64_t>(blocks, 1), c->L / 256));
-    *piece = std::max<int64_t>(ceil_div(ceil_div(c->L, want), 64) * 64, 64);
-    *pieces = (int)std::max<int64_t>(ceil_div(c->L, *piece), 1);
-}
-
-size_t starts_bytes(const pathsig_linattn *c, int64_t Dv) {
-    int64_t piece;
-    int pieces;
-    cut(c, Dv, &piece, &pieces);
-    return pieces > 1 ? (size_t)pieces * c->B * c->H * c->Dk * c->Dv * sizeof(float) : 0;
 }
 
 template <typename T>
@@ -248,18 +210,21 @@ void chunks(const Sweep &a, bool fold, hipStream_t stream) {
     launch_chunks<T, 8>(a, fold, stream);
 }
 
-// joined: `starts` already holds the states in front of the pieces
+// the states in front of the pieces
 template <typename T>
-void run_sweep(Sweep &a, const pathsig_linattn *c, float *starts, bool joined, hipStream_t stream) {
-    if (!joined) {
-        cut(c, a.Dv, &a.piece, &a.pieces);
-        a.starts = {starts, a.Dv, 1};
-        if (a.pieces > 1) {
-            chunks<T>(a, true, stream);
-            join_kernel<<<dim3((unsigned)ceil_div((int64_t)a.Dk * a.Dv, 256), a.H, (unsigned)a.B), 256, 0, stream>>>(a);
-        }
-    }
-    chunks<T>(a, false, stream);
+void fold(Sweep &a, float *starts, hipStream_t stream) {
+    a.starts = {starts, a.Dv, 1};
+    if (a.pieces == 1) return;
+    chunks<T>(a, true, stream);
+    join_kernel<<<dim3((unsigned)ceil_div((int64_t)a.Dk * a.Dv, 256), a.H, (unsigned)a.B), 256, 0, stream>>>(a);
+}
+
+template <typename T>
+void decay(const Sweep &a, const View &grad_out, const StateRef &ends, float *partial, hipStream_t stream) {
+    if (a.Dk <= 32) return launch_decay<T, 1>(a, grad_out, ends, partial, stream);
+    if (a.Dk <= 64) return launch_decay<T, 2>(a, grad_out, ends, partial, stream);
+    if (a.Dk <= 128) return launch_decay<T, 4>(a, grad_out, ends, partial, stream);
+    launch_decay<T, 8>(a, grad_out, ends, partial, stream);
 }
 
 template <typename T>
@@ -274,12 +239,13 @@ int forward_t(const pathsig_linattn *c, const void *q, const void *k, const void
     a.last = {final_state, c->Dv, 1};
     a.out = out;
     a.out_scale = c->scale;
-    run_sweep<T>(a, c, starts, false, stream);
+    fold<T>(a, starts, stream);
+    chunks<T>(a, false, stream);
     return launch_status("linear attention");
 }
 
 struct BackwardLayout {
-    size_t starts, wide_k, wide_v, decay, total;  // byte offsets
+    size_t starts, ends, wide_k, wide_v, decay, total;  // byte offsets
 };
 
 size_t place(size_t &total, size_t bytes) {
@@ -288,15 +254,23 @@ size_t place(size_t &total, size_t bytes) {
     return at;
 }
 
+int64_t decay_partials(const pathsig_linattn *c) {
+    int64_t piece;
+    int pieces;
+    cut(c, &piece, &pieces);
+    return pieces * ceil_div(c->Dv, 128) * c->B;
+}
+
 BackwardLayout backward_layout(const pathsig_linattn *c, bool want_decay) {
     BackwardLayout l = {};
     const size_t tokens = (size_t)c->B * c->L * c->H;
-    l.starts = place(l.total, std::max(starts_bytes(c, c->Dk), starts_bytes(c, c->Dv)));
+    l.starts = place(l.total, starts_bytes(c));
+    l.ends = place(l.total, starts_bytes(c));
     if (c->H != c->Hkv) {
         l.wide_k = place(l.total, tokens * c->Dk * sizeof(float));
         l.wide_v = place(l.total, tokens * c->Dv * sizeof(float));
     }
-    if (want_decay) l.decay = place(l.total, (size_t)ceil_div(c->Dv, 32) * c->B * c->H * sizeof(float));
+    if (want_decay) l.decay = place(l.total, (size_t)decay_partials(c) * c->H * sizeof(float));
     return l;
 }
 
@@ -308,7 +282,7 @@ int backward_t(const pathsig_linattn *c, const void *q, const void *k, const voi
     const View vq = view(q, c->q_stride, 1, sizeof(T)), vk = view(k, c->k_stride, group, sizeof(T)),
                vv = view(v, c->v_stride, group, sizeof(T)), vdo = dense(grad_out, c->L, c->H, c->Dv, sizeof(T));
     const BackwardLayout l = backward_layout(c, grad_decay != nullptr);
-    float *const starts = (float *)(ws + l.starts);
+    float *const starts = (float *)(ws + l.starts), *const ends = (float *)(ws + l.ends);
     // dq: the forward with (do, v, k) and the transposed state
     Sweep a = sweep_of(c);
     std::swap(a.Dk, a.Dv);
@@ -318,7 +292,8 @@ int backward_t(const pathsig_linattn *c, const void *q, const void *k, const voi
     a.first = {const_cast<float *>(state), 1, c->Dv};
     a.out = grad_q;
     a.out_scale = c->scale;
-    run_sweep<T>(a, c, starts, false, stream);
+    fold<T>(a, starts, stream);
+    chunks<T>(a, false, stream);
     // dv: backwards in time with (k, q, do)
     a = sweep_of(c);
     a.q = vk;
@@ -330,29 +305,26 @@ int backward_t(const pathsig_linattn *c, const void *q, const void *k, const voi
     a.reverse = 1;
     a.out_float = group > 1;
     a.out = group > 1 ? (void *)(ws + l.wide_v) : grad_v;
-    run_sweep<T>(a, c, starts, false, stream);
-    // dk: backwards in time with (v, do, q) and the transposed gradient of the state
-    Sweep k_sweep = a;
-    std::swap(k_sweep.Dk, k_sweep.Dv);
-    k_sweep.q = vv;
-    k_sweep.k = vdo;
-    k_sweep.v = vq;
-    k_sweep.first = {const_cast<float *>(grad_final), 1, c->Dv};
-    k_sweep.last = {nullptr, 0, 0};
-    k_sweep.out = group > 1 ? (void *)(ws + l.wide_k) : grad_k;
-    // the states in front of the pieces are those of dv, transposed, as long as both are cut alike
-    int64_t piece;
-    int pieces;
-    cut(c, c->Dk, &piece, &pieces);
-    const bool joined = piece == a.piece;
-    if (joined) k_sweep.starts = {starts, 1, c->Dv};
-    run_sweep<T>(k_sweep, c, starts, joined, stream);
+    fold<T>(a, ends, stream);
+    chunks<T>(a, false, stream);
+    // dk: backwards in time with (v, do, q), from the same states, transposed
+    std::swap(a.Dk, a.Dv);
+    a.q = vv;
+    a.k = vdo;
+    a.v = vq;
+    a.first = {const_cast<float *>(grad_final), 1, c->Dv};
+    a.starts = {ends, 1, c->Dv};
+    a.last = {nullptr, 0, 0};
+    a.out = group > 1 ? (void *)(ws + l.wide_k) : grad_k;
+    chunks<T>(a, false, stream);
     if (group > 1) {
         const int64_t rows = c->B * c->L;
         const unsigned blocks_k = (unsigned)std::min<int64_t>(ceil_div(rows * c->Hkv * c->Dk, 256), 4096);
         const unsigned blocks_v = (unsigned)std::min<int64_t>(ceil_div(rows * c->Hkv * c->Dv, 256), 4096);
-        group_sum_kernel<T><<<blocks_k, 256, 0, stream>>>((const float *)(ws + l.wide_k), (T *)grad_k, rows, (int)c->Hkv, (int)group, (int)c->Dk);
-        group_sum_kernel<T><<<blocks_v, 256, 0, stream>>>((const float *)(ws + l.wide_v), (T *)grad_v, rows, (int)c->Hkv, (int)group, (int)c->Dv);
+        if (rows > 0) {
+            group_sum_kernel<T><<<blocks_k, 256, 0, stream>>>((const float *)(ws + l.wide_k), (T *)grad_k, rows, (int)c->Hkv, (int)group, (int)c->Dk);
+            group_sum_kernel<T><<<blocks_v, 256, 0, stream>>>((const float *)(ws + l.wide_v), (T *)grad_v, rows, (int)c->Hkv, (int)group, (int)c->Dv);
+        }
     }
     if (grad_decay) {
         a = sweep_of(c);
@@ -360,11 +332,11 @@ int backward_t(const pathsig_linattn *c, const void *q, const void *k, const voi
         a.k = vk;
         a.v = vv;
         a.first = {const_cast<float *>(state), c->Dv, 1};
+        a.starts = {starts, 1, c->Dk};
         a.out_scale = c->scale;
-        const int64_t slices = ceil_div(c->Dv, 32);
-        decay_scan_kernel<T><<<dim3((unsigned)slices, a.H, (unsigned)c->B), 32, 0, stream>>>(a, (const T *)grad_out, grad_final,
-                                                                                           (float *)(ws + l.decay));
-        decay_sum_kernel<<<a.H, 64, 0, stream>>>((const float *)(ws + l.decay), slices * c->B, a.H, grad_decay);
+        const StateRef behind = a.pieces > 1 ? StateRef{ends, c->Dv, 1} : StateRef{const_cast<float *>(grad_final), c->Dv, 1};
+        decay<T>(a, vdo, behind, (float *)(ws + l.decay), stream);
+        decay_sum_kernel<<<a.H, 64, 0, stream>>>((const float *)(ws + l.decay), decay_partials(c), a.H, grad_decay);
     }
     return launch_status("linear attention, backward");
 }
@@ -400,7 +372,7 @@ extern "C" {
 
 size_t pathsig_linattn_forward_workspace(const pathsig_linattn *call) {
     if (check_call(call) != PATHSIG_OK) return 0;
-    return starts_bytes(call, call->Dv);
+    return starts_bytes(call);
 }
 
 int pathsig_linattn_forward(const pathsig_linattn *call, const void *q, const void *k, const void *v, const float *state,

@@ -52,11 +52,28 @@ __device__ __forceinline__ float decay_of(const float *log_decay, int h) {
     return fmaxf(log_decay[h], -1e30f);
 }
 
+// Tokens [begin, end) of a piece in the order of the sweep.  Pieces are cut at the same tokens in both directions of time: the
+// s-th of a sweep backwards in time is the one s from the last, and empty where the sequence ends before it.
+struct Range {
+    int64_t begin, end;
+};
+__device__ __forceinline__ Range range_of(const Sweep &a, int64_t n, int s) {
+    const int64_t p = a.reverse ? a.pieces - 1 - s : s;
+    const int64_t t0 = min(p * a.piece, n), t1 = min((p + 1) * a.piece, n);
+    return a.reverse ? Range{n - t1, n - t0} : Range{t0, t1};
+}
+
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // seq_chunks.hip, for keys of up to 32 DKT channels.  fold: only the states that the pieces add, from zero, into starts[s + 1].
 template <typename T, int DKT>
 void launch_chunks(const Sweep &a, bool fold, hipStream_t stream);
+
+// The gradient of the decays: partial sums [pieces][slices][B][H], slices = ceil(Dv / 128), for the sweep forwards in time.
+// ends: the gradients of the states behind the pieces, the first piece's at the end (as a sweep backwards in time leaves them in
+// its `starts`), or with one piece that of the last state or NULL.
+template <typename T, int DKT>
+void launch_decay(const Sweep &a, const View &grad_out, const StateRef &ends, float *partial, hipStream_t stream);
 
 }  // namespace seq
 }  // namespace psig

@@ -245,18 +245,19 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
     const int64_t b = blockIdx.z;
     const int dv0 = slice * DV, dv = dv0 + 32 * wave + ln;  // this lane's column of the state
     const int64_t n = length_of(a.lengths, b, a.L);
-    const int64_t begin = piece * a.piece, end = min(begin + a.piece, n);
+    const auto [begin, end] = range_of(a, n, piece);
     const float g2 = decay_of(a.log_decay, h) * kLog2e;
     const int64_t plane = (int64_t)a.Dk * a.Dv, head = (b * a.H + h) * plane;
 
     if (!FOLD) {
         // tokens behind the end of the sequence
-        const int64_t z0 = max(n, begin), z1 = min(begin + a.piece, a.L);
+        const int64_t p = a.reverse ? a.pieces - 1 - piece : piece;
+        const int64_t z0 = max(n, p * a.piece), z1 = min((p + 1) * a.piece, a.L);
         const int width = min(DV, a.Dv - dv0);
         for (int64_t t = z0 + wave; t < z1; t += NW)
             for (int c = lane; c < width; c += 64) ((O *)a.out)[((b * a.L + t) * a.H + h) * a.Dv + dv0 + c] = from_float<O>(0.f);
     }
-    const bool owns_end = !FOLD && a.last.p && (end == n && (begin < n || piece == 0));
+    const bool owns_end = !FOLD && a.last.p && end == n && (begin < n || (n == 0 && piece == 0));
     if (begin >= end && !owns_end && !FOLD) return;
 
     f32x16 S[DKT];
@@ -445,6 +446,204 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
         }
 }
 
+// dL/dg of a piece.  With S the state of a head and D = dS/dg (zero in front of the piece, whose own S is given):
+//     dL/dg = sum over chunks of  sum over j <= i of (i - j) l^(i-j) (do_i . v_j) (q_i . k_j)
+//                                 + <D, G> + <S, G'>,   G = sum of l^(i+1) q_i do_i^T,  G' = sum of (i + 1) l^(i+1) q_i do_i^T,
+//             + <D behind the piece, dL/dS behind the piece>,
+//     D' = l^C (D + C S) + sum of (C - 1 - j) l^(C-1-j) k_j v_j^T.
+// Every term is a sum of like signs or of independent ones; sum over t of t (q_t . dq_t - k_t . dk_t), which needs no states,
+// cancels by the length of the sequence over the memory of the head.  Products of states stay in 32 bits (element by element on
+// accumulators); what enters them is split into two bf16 terms (relative 2^-18 a term).
+template <typename T, int COUNT>
+__device__ __forceinline__ void split_scaled(f32x8 x, const f32x8 &f, Frag<T> (&out)[COUNT]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= f[e];
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+        out[i] = rounded<T>(x);
+        x -= widened(out[i]);
+    }
+}
+
+__device__ __forceinline__ float sum16(f32x16 x) {
+    float s = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s += x[r];
+    return s;
+}
+
+template <typename T, int DKT, int NW>
+__global__ __launch_bounds__(64 * NW, 1) void decay_kernel(const Sweep a, const View grad, const StateRef ends, float *partial,
+                                                         int slices) {
+    constexpr int DK = 32 * DKT, DV = 32 * NW, THREADS = 64 * NW, TERMS = sizeof(T) == 2 ? 2 : 1;
+    constexpr int CT = chunk_tiles<T>(DKT, NW), C = 32 * CT;
+    using KTile = Tile<T, DK>;
+    using VTile = Tile<T, DV>;
+    constexpr int kKBytes = C * KTile::kRow, kVBytes = C * VTile::kRow;
+    __shared__ __align__(16) char lds[2 * kKBytes + 2 * kVBytes];
+    __shared__ float meet[NW];
+    char *const lds_k = lds, *const lds_q = lds + kKBytes, *const lds_v = lds_q + kKBytes, *const lds_o = lds_v + kVBytes;
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, ln = lane & 31;
+    const int slice = blockIdx.x % slices, h = blockIdx.x / slices, piece = blockIdx.y;
+    const int64_t b = blockIdx.z;
+    const int dv0 = slice * DV, dv = dv0 + 32 * wave + ln;
+    const int64_t n = length_of(a.lengths, b, a.L);
+    const auto [begin, end] = range_of(a, n, piece);
+    const float g2 = decay_of(a.log_decay, h) * kLog2e;
+    const int64_t plane = (int64_t)a.Dk * a.Dv, head = (b * a.H + h) * plane, between = a.B * a.H * plane;
+
+    f32x16 S[DKT], D[DKT];
+    {
+        const StateRef from = a.pieces > 1 ? StateRef{a.starts.p + piece * between, a.starts.row, a.starts.column} : a.first;
+#pragma unroll
+        for (int t = 0; t < DKT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int dk = 32 * t + acc_row(r, half);
+                S[t][r] = from.p && dk < a.Dk && dv < a.Dv ? from.p[head + dk * from.row + dv * from.column] : 0.f;
+                D[t][r] = 0.f;
+            }
+    }
+    const T *const kp = (const T *)a.k.p + b * a.k.sb + (h / a.k.group) * a.k.sh;
+    const T *const vp = (const T *)a.v.p + b * a.v.sb + (h / a.v.group) * a.v.sh + dv0;
+    const T *const qp = (const T *)a.q.p + b * a.q.sb + (h / a.q.group) * a.q.sh;
+    const T *const op = (const T *)grad.p + b * grad.sb + (h / grad.group) * grad.sh + dv0;
+    const int chunks = (int)((end - begin + C - 1) / C);
+    int64_t r0 = end - (int64_t)chunks * C;
+    const int row_base_of_lane = KTile::row_base(ln, half), v_row_base_of_lane = VTile::row_base(ln, half);
+    int k_bases_of_lane[KTile::kColumnBases], v_bases_of_lane[VTile::kColumnBases];
+    KTile::column_bases(k_bases_of_lane, lane);
+    VTile::column_bases(v_bases_of_lane, lane);
+    float total = 0.f;
+    for (int c = 0; c < chunks; ++c, r0 += C) {
+        const int pad = (int)max(begin - r0, (int64_t)0);
+        __syncthreads();
+        {
+            Fetch<T, DK, C, THREADS> x;
+            x.load(kp + r0 * a.k.st, (int)a.k.st, a.Dk, a.k.vectors, pad);
+            x.store(lds_k);
+            x.load(qp + r0 * a.q.st, (int)a.q.st, a.Dk, a.q.vectors, pad);
+            x.store(lds_q);
+            Fetch<T, DV, C, THREADS> y;
+            y.load(vp + r0 * a.v.st, (int)a.v.st, a.Dv - dv0, a.v.vectors, pad);
+            y.store(lds_v);
+            y.load(op + r0 * grad.st, (int)grad.st, a.Dv - dv0, grad.vectors, pad);
+            y.store(lds_o);
+        }
+        __syncthreads();
+        int row_base = row_base_of_lane, v_row_base = v_row_base_of_lane, k_bases[KTile::kColumnBases],
+            v_bases[VTile::kColumnBases];
+        asm volatile("" : "+v"(row_base), "+v"(v_row_base));
+#pragma unroll
+        for (int g = 0; g < KTile::kColumnBases; ++g) {
+            k_bases[g] = k_bases_of_lane[g];
+            v_bases[g] = v_bases_of_lane[g] ^ (wave * 32 * (int)sizeof(T));
+            asm volatile("" : "+v"(k_bases[g]), "+v"(v_bases[g]));
+        }
+        v_row_base ^= wave * 32 * (int)sizeof(T);
+
+        // inside the chunk; this wave's channels of do . v
+#pragma unroll
+        for (int i = 0; i < CT; ++i)
+#pragma unroll
+            for (int j = 0; j <= i; ++j) {
+                f32x16 scores = {}, pulls = {};
+#pragma unroll
+                for (int kk = 0; kk < DK / 16; ++kk) {
+                    scores = mma(KTile::row(lds_k, row_base, j, kk), KTile::row(lds_q, row_base, i, kk), scores);
+                    if (kk % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk)
+                    pulls = mma(VTile::row(lds_v, v_row_base, j, kk), VTile::row(lds_o, v_row_base, i, kk), pulls);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int gap = 32 * (i - j) + ln - acc_row(r, half);
+                    const float f = (float)gap * exp2f(g2 * (float)max(gap, 0));
+                    if (gap > 0) total += f * (scores[r] * pulls[r]);
+                }
+            }
+
+        // through the states
+#pragma unroll
+        for (int t = 0; t < DKT; ++t) {
+            f32x16 G = {}, G1 = {};
+#pragma unroll
+            for (int kk = 0; kk < 2 * CT; ++kk) {
+                f32x8 f, f1;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float since = (float)max(16 * kk + acc_row(e, half) + 1 - pad, 0);
+                    f[e] = exp2f(g2 * since);
+                    f1[e] = since * f[e];
+                }
+                const f32x8 o = widened(VTile::column(lds_o, v_bases, 0, kk));
+                Frag<T> x[TERMS], x1[TERMS];
+                split_scaled<T>(o, f, x);
+                split_scaled<T>(o, f1, x1);
+                const Frag<T> q = KTile::column(lds_q, k_bases, t, kk);
+#pragma unroll
+                for (int i = 0; i < TERMS; ++i) {
+                    G = mma(q, x[i], G);
+                    G1 = mma(q, x1[i], G1);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            total += sum16(D[t] * G + S[t] * G1);
+        }
+
+        const float count = (float)(C - pad), whole = exp2f(g2 * count);
+#pragma unroll
+        for (int t = 0; t < DKT; ++t) {
+            D[t] = whole * (D[t] + count * S[t]);
+            S[t] *= whole;
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2 * CT; ++kk) {
+            f32x8 f, f1;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float left = (float)(C - 1 - 16 * kk - acc_row(e, half));
+                f[e] = exp2f(g2 * left);
+                f1[e] = left * f[e];
+            }
+            const f32x8 v = widened(VTile::column(lds_v, v_bases, 0, kk));
+            Frag<T> x[TERMS], x1[TERMS];
+            split_scaled<T>(v, f, x);
+            split_scaled<T>(v, f1, x1);
+#pragma unroll
+            for (int t = 0; t < DKT; ++t) {
+                const Frag<T> k = KTile::column(lds_k, k_bases, t, kk);
+#pragma unroll
+                for (int i = 0; i < TERMS; ++i) {
+                    S[t] = mma(k, x[i], S[t]);
+                    D[t] = mma(k, x1[i], D[t]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    total *= a.out_scale;
+    if (ends.p) {
+        const float *const from = ends.p + (a.pieces > 1 ? (a.pieces - 1 - piece) * between : 0) + head;
+#pragma unroll
+        for (int t = 0; t < DKT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int dk = 32 * t + acc_row(r, half);
+                if (dk < a.Dk && dv < a.Dv) total += D[t][r] * from[dk * ends.row + dv * ends.column];
+            }
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) total += __shfl_xor(total, m);
+    if (lane == 0) meet[wave] = total;
+    __syncthreads();
+    if (threadIdx.x > 0) return;
+    for (int w = 1; w < NW; ++w) total += meet[w];
+    partial[(((int64_t)piece * slices + slice) * a.B + b) * a.H + h] = total;
+}
+
 template <typename T, int DKT, int NW>
 void launch_width(const Sweep &a, bool fold, hipStream_t stream) {
     const int slices = (int)ceil_div(a.Dv, 32 * NW);
@@ -466,8 +665,22 @@ void launch_chunks(const Sweep &a, bool fold, hipStream_t stream) {
     launch_width<T, DKT, 4>(a, fold, stream);
 }
 
+template <typename T, int DKT>
+void launch_decay(const Sweep &a, const View &grad_out, const StateRef &ends, float *partial, hipStream_t stream) {
+    const int slices = (int)ceil_div(a.Dv, 128);
+    const dim3 grid((unsigned)(slices * a.H), (unsigned)a.pieces, (unsigned)a.B);
+    if (a.Dv <= 32)
+        decay_kernel<T, DKT, 1><<<grid, 64, 0, stream>>>(a, grad_out, ends, partial, slices);
+    else if (a.Dv <= 64)
+        decay_kernel<T, DKT, 2><<<grid, 128, 0, stream>>>(a, grad_out, ends, partial, slices);
+    else
+        decay_kernel<T, DKT, 4><<<grid, 256, 0, stream>>>(a, grad_out, ends, partial, slices);
+}
+
 template void launch_chunks<float, PSIG_KEY_TILES>(const Sweep &, bool, hipStream_t);
 template void launch_chunks<bf16, PSIG_KEY_TILES>(const Sweep &, bool, hipStream_t);
+template void launch_decay<float, PSIG_KEY_TILES>(const Sweep &, const View &, const StateRef &, float *, hipStream_t);
+template void launch_decay<bf16, PSIG_KEY_TILES>(const Sweep &, const View &, const StateRef &, float *, hipStream_t);
 
 }  // namespace seq
 }  // namespace psig
