@@ -263,6 +263,7 @@ typedef struct pathsig_linattn {
     int64_t B, L, H, Hkv, Dk, Dv;
     int64_t q_stride[3], k_stride[3], v_stride[3]; /* of a sequence, a token, a head */
     float scale;
+    int learned_decay; /* the backward will want grad_log_decay */
     const float *log_decay;
     const int32_t *lengths;
 } pathsig_linattn;
@@ -273,15 +274,17 @@ int pathsig_linattn_forward(const pathsig_linattn *call, const void *q, const vo
                             void *out, float *final_state, void *workspace, size_t workspace_bytes, void *stream);
 
 /*
- * Its backward.  grad_out is a dense [B, L, H, Dv], grad_final_state [B, H, Dk, Dv] float32 or NULL (zero).
+ * Its backward.  kept: the forward's workspace as the forward of the same call left it (pathsig_linattn_forward_workspace bytes:
+ * the states between pieces of long sequences), or NULL, and the backward works them out again.
+ *   grad_out is a dense [B, L, H, Dv], grad_final_state [B, H, Dk, Dv] float32 or NULL (zero).
  *   grad_q [B, L, H, Dk], grad_k [B, L, Hkv, Dk], grad_v [B, L, Hkv, Dv] dense, in the type of q (sums over the heads that share
  *   a key); grad_log_decay [H] and grad_state [B, H, Dk, Dv] float32, each NULL where it is not wanted.
  */
 size_t pathsig_linattn_backward_workspace(const pathsig_linattn *call, int want_log_decay);
 int pathsig_linattn_backward(const pathsig_linattn *call, const void *q, const void *k, const void *v, const float *state,
-                             const void *grad_out, const float *grad_final_state, void *grad_q, void *grad_k, void *grad_v,
-                             float *grad_log_decay, float *grad_state, void *workspace, size_t workspace_bytes,
-                             void *stream);
+                             const void *kept, size_t kept_bytes, const void *grad_out, const float *grad_final_state, void *grad_q,
+                             void *grad_k, void *grad_v, float *grad_log_decay, float *grad_state, void *workspace,
+                             size_t workspace_bytes, void *stream);
 
 /* One token of every sequence: L = 1, no lengths; `state` is updated in place.  The token strides are not read. */
 int pathsig_linattn_step(const pathsig_linattn *call, const void *q, const void *k, const void *v, float *state, void *out,

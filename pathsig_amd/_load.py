@@ -29,7 +29,7 @@ class LinearAttentionCall(ctypes.Structure):
     """`pathsig_linattn` of include/pathsig_hip.h."""
     _fields_ = [("dtype", _INT), ("B", _I64), ("L", _I64), ("H", _I64), ("Hkv", _I64), ("Dk", _I64), ("Dv", _I64),
                 ("q_stride", _I64 * 3), ("k_stride", _I64 * 3), ("v_stride", _I64 * 3), ("scale", ctypes.c_float),
-                ("log_decay", _PTR), ("lengths", _PTR)]
+                ("learned_decay", _INT), ("log_decay", _PTR), ("lengths", _PTR)]
 
 
 class NormCall(ctypes.Structure):
@@ -54,7 +54,7 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.pathsig_linattn_backward_workspace.restype = _SIZE
     lib.pathsig_linattn_backward_workspace.argtypes = [_CALL, _INT]
     lib.pathsig_linattn_backward.restype = _INT
-    lib.pathsig_linattn_backward.argtypes = [_CALL] + [_PTR] * 12 + [_SIZE, _PTR]
+    lib.pathsig_linattn_backward.argtypes = [_CALL] + [_PTR] * 5 + [_SIZE] + [_PTR] * 8 + [_SIZE, _PTR]
     lib.pathsig_linattn_step.restype = _INT
     lib.pathsig_linattn_step.argtypes = [_CALL] + [_PTR] * 6
     _NORM = ctypes.POINTER(NormCall)

@@ -19,25 +19,33 @@ namespace psig {
 namespace seq {
 namespace {
 
-// starts[s] holds what piece s - 1 adds; in place becomes the state in front of piece s.
+// starts[s] holds what piece s - 1 adds; in place becomes the state in front of piece s.  Vectors of four elements along a row of
+// `starts` (V = 1 where the rows have no whole vectors), each with a thread of its own: bound by reading and writing `starts`.
+template <int V>
 __global__ __launch_bounds__(256) void join_kernel(const Sweep a) {
+    using P = Pack<float, V>;
     const int64_t plane = (int64_t)a.Dk * a.Dv;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
     if (i >= plane) return;
     const int h = blockIdx.y;
     const int64_t b = blockIdx.z, head = (b * a.H + h) * plane, stride = a.B * a.H * plane;
     const int64_t n = length_of(a.lengths, b, a.L);
     const float g2 = decay_of(a.log_decay, h) * kLog2e;
-    // (element i of `first` where its rows are the columns of `starts`)
-    const int64_t at = a.first.row == a.starts.row ? i : (i % a.Dv) * a.Dk + i / a.Dv;
     float *const p = a.starts.p + head + i;
-    float x = a.first.p ? a.first.p[head + at] : 0.f;
-    p[0] = x;
+    P x = {};
+    if (a.first.p) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) x.v[e] = a.first.p[head + (i + e) / a.Dv * a.first.row + (i + e) % a.Dv * a.first.column];
+    }
+    *(P *)p = x;
 #pragma unroll 8
     for (int s = 1; s < a.pieces; ++s) {
         const Range before = range_of(a, n, s - 1);
-        x = x * exp2f(g2 * (float)(before.end - before.begin)) + p[s * stride];
-        p[s * stride] = x;
+        const float f = exp2f(g2 * (float)(before.end - before.begin));
+        P add = *(const P *)(p + s * stride);
+#pragma unroll
+        for (int e = 0; e < V; ++e) x.v[e] = x.v[e] * f + add.v[e];
+        *(P *)(p + s * stride) = x;
     }
 }
 
@@ -216,15 +224,20 @@ void fold(Sweep &a, float *starts, hipStream_t stream) {
     a.starts = {starts, a.Dv, 1};
     if (a.pieces == 1) return;
     chunks<T>(a, true, stream);
-    join_kernel<<<dim3((unsigned)ceil_div((int64_t)a.Dk * a.Dv, 256), a.H, (unsigned)a.B), 256, 0, stream>>>(a);
+    if (a.pieces <= kJoinInside) return;
+    const int64_t plane = (int64_t)a.Dk * a.Dv;
+    if (plane % 4 == 0)
+        join_kernel<4><<<dim3((unsigned)ceil_div(plane, 1024), a.H, (unsigned)a.B), 256, 0, stream>>>(a);
+    else
+        join_kernel<1><<<dim3((unsigned)ceil_div(plane, 256), a.H, (unsigned)a.B), 256, 0, stream>>>(a);
 }
 
 template <typename T>
-void decay(const Sweep &a, const View &grad_out, const StateRef &ends, float *partial, hipStream_t stream) {
-    if (a.Dk <= 32) return launch_decay<T, 1>(a, grad_out, ends, partial, stream);
-    if (a.Dk <= 64) return launch_decay<T, 2>(a, grad_out, ends, partial, stream);
-    if (a.Dk <= 128) return launch_decay<T, 4>(a, grad_out, ends, partial, stream);
-    launch_decay<T, 8>(a, grad_out, ends, partial, stream);
+void decay(const Sweep &a, const Sweep &back, const View &grad_out, float *partial, hipStream_t stream) {
+    if (a.Dk <= 32) return launch_decay<T, 1>(a, back, grad_out, partial, stream);
+    if (a.Dk <= 64) return launch_decay<T, 2>(a, back, grad_out, partial, stream);
+    if (a.Dk <= 128) return launch_decay<T, 4>(a, back, grad_out, partial, stream);
+    launch_decay<T, 8>(a, back, grad_out, partial, stream);
 }
 
 template <typename T>
@@ -239,6 +252,7 @@ int forward_t(const pathsig_linattn *c, const void *q, const void *k, const void
     a.last = {final_state, c->Dv, 1};
     a.out = out;
     a.out_scale = c->scale;
+    a.exact_state = final_state || c->learned_decay;
     fold<T>(a, starts, stream);
     chunks<T>(a, false, stream);
     return launch_status("linear attention");
@@ -275,47 +289,62 @@ BackwardLayout backward_layout(const pathsig_linattn *c, bool want_decay) {
 }
 
 template <typename T>
-int backward_t(const pathsig_linattn *c, const void *q, const void *k, const void *v, const float *state, const void *grad_out,
-               const float *grad_final, void *grad_q, void *grad_k, void *grad_v, float *grad_decay, float *grad_state, char *ws,
-               hipStream_t stream) {
+int backward_t(const pathsig_linattn *c, const void *q, const void *k, const void *v, const float *state, const float *kept,
+               const void *grad_out, const float *grad_final, void *grad_q, void *grad_k, void *grad_v, float *grad_decay,
+               float *grad_state, char *ws, hipStream_t stream) {
     const int64_t group = c->H / c->Hkv;
     const View vq = view(q, c->q_stride, 1, sizeof(T)), vk = view(k, c->k_stride, group, sizeof(T)),
                vv = view(v, c->v_stride, group, sizeof(T)), vdo = dense(grad_out, c->L, c->H, c->Dv, sizeof(T));
     const BackwardLayout l = backward_layout(c, grad_decay != nullptr);
-    float *const starts = (float *)(ws + l.starts), *const ends = (float *)(ws + l.ends);
-    // dq: the forward with (do, v, k) and the transposed state
-    Sweep a = sweep_of(c);
+    // the forward's states in front of the pieces
+    Sweep forward = sweep_of(c);
+    forward.q = vq;
+    forward.k = vk;
+    forward.v = vv;
+    forward.first = {const_cast<float *>(state), c->Dv, 1};
+    forward.out_scale = c->scale;
+    forward.exact_state = grad_decay != nullptr;
+    if (kept)
+        forward.starts = {const_cast<float *>(kept), c->Dv, 1};
+    else
+        fold<T>(forward, (float *)(ws + l.starts), stream);
+    // dq: the forward with (do, v, k) and the transposed states
+    Sweep a = forward;
     std::swap(a.Dk, a.Dv);
     a.q = vdo;
     a.k = vv;
     a.v = vk;
-    a.first = {const_cast<float *>(state), 1, c->Dv};
+    a.first = {forward.first.p, 1, c->Dv};
+    a.starts = {forward.starts.p, 1, c->Dv};
     a.out = grad_q;
-    a.out_scale = c->scale;
-    fold<T>(a, starts, stream);
+    a.exact_state = 0;
     chunks<T>(a, false, stream);
     // dv: backwards in time with (k, q, do)
-    a = sweep_of(c);
-    a.q = vk;
-    a.k = vq;
-    a.v = vdo;
-    a.first = {const_cast<float *>(grad_final), c->Dv, 1};
-    a.last = {grad_state, c->Dv, 1};
-    a.in_scale = c->scale;
-    a.reverse = 1;
-    a.out_float = group > 1;
-    a.out = group > 1 ? (void *)(ws + l.wide_v) : grad_v;
-    fold<T>(a, ends, stream);
-    chunks<T>(a, false, stream);
+    Sweep back = sweep_of(c);
+    back.q = vk;
+    back.k = vq;
+    back.v = vdo;
+    back.first = {const_cast<float *>(grad_final), c->Dv, 1};
+    back.last = {grad_state, c->Dv, 1};
+    back.in_scale = c->scale;
+    back.reverse = 1;
+    back.out_float = group > 1;
+    back.out = group > 1 ? (void *)(ws + l.wide_v) : grad_v;
+    back.exact_state = grad_state || grad_decay;
+    fold<T>(back, (float *)(ws + l.ends), stream);
+    back.exact_state = grad_state != nullptr;
+    chunks<T>(back, false, stream);
     // dk: backwards in time with (v, do, q), from the same states, transposed
+    a = back;
     std::swap(a.Dk, a.Dv);
     a.q = vv;
     a.k = vdo;
     a.v = vq;
-    a.first = {const_cast<float *>(grad_final), 1, c->Dv};
-    a.starts = {ends, 1, c->Dv};
+    a.first = {back.first.p, 1, c->Dv};
+    a.starts = {back.starts.p, 1, c->Dv};
     a.last = {nullptr, 0, 0};
     a.out = group > 1 ? (void *)(ws + l.wide_k) : grad_k;
+    a.exact_state = 0;
     chunks<T>(a, false, stream);
     if (group > 1) {
         const int64_t rows = c->B * c->L;
@@ -327,16 +356,8 @@ int backward_t(const pathsig_linattn *c, const void *q, const void *k, const voi
         }
     }
     if (grad_decay) {
-        a = sweep_of(c);
-        a.q = vq;
-        a.k = vk;
-        a.v = vv;
-        a.first = {const_cast<float *>(state), c->Dv, 1};
-        a.starts = {starts, 1, c->Dk};
-        a.out_scale = c->scale;
-        const StateRef behind = a.pieces > 1 ? StateRef{ends, c->Dv, 1} : StateRef{const_cast<float *>(grad_final), c->Dv, 1};
-        decay<T>(a, vdo, behind, (float *)(ws + l.decay), stream);
-        decay_sum_kernel<<<a.H, 64, 0, stream>>>((const float *)(ws + l.decay), decay_partials(c), a.H, grad_decay);
+        decay<T>(forward, back, vdo, (float *)(ws + l.decay), stream);
+        decay_sum_kernel<<<(unsigned)c->H, 64, 0, stream>>>((const float *)(ws + l.decay), decay_partials(c), (int)c->H, grad_decay);
     }
     return launch_status("linear attention, backward");
 }
@@ -398,12 +419,20 @@ size_t pathsig_linattn_backward_workspace(const pathsig_linattn *call, int want_
 }
 
 int pathsig_linattn_backward(const pathsig_linattn *call, const void *q, const void *k, const void *v, const float *state,
-                             const void *grad_out, const float *grad_final_state, void *grad_q, void *grad_k, void *grad_v,
-                             float *grad_log_decay, float *grad_state, void *workspace, size_t workspace_bytes,
-                             void *stream) {
+                             const void *kept, size_t kept_bytes, const void *grad_out, const float *grad_final_state, void *grad_q,
+                             void *grad_k, void *grad_v, float *grad_log_decay, float *grad_state, void *workspace,
+                             size_t workspace_bytes, void *stream) {
     if (const int rc = check_call(call)) return rc;
     if (call->B > 0 && call->L > 0 && (!q || !k || !v || !grad_out || !grad_q || !grad_k || !grad_v)) {
         set_error("q, k, v, grad_out, grad_q, grad_k and grad_v must not be NULL");
+        return PATHSIG_ERR_ARGUMENT;
+    }
+    if (grad_log_decay && !call->learned_decay) {
+        set_error("grad_log_decay is asked for, but learned_decay is not set");
+        return PATHSIG_ERR_ARGUMENT;
+    }
+    if (kept && kept_bytes != starts_bytes(call)) {
+        set_error("kept: the forward's workspace has %zu bytes, got %zu", starts_bytes(call), kept_bytes);
         return PATHSIG_ERR_ARGUMENT;
     }
     const size_t need = backward_layout(call, grad_log_decay != nullptr).total;
@@ -417,10 +446,10 @@ int pathsig_linattn_backward(const pathsig_linattn *call, const void *q, const v
         return launch_status("linear attention, backward");
     }
     if (call->dtype == PATHSIG_F32)
-        return backward_t<float>(call, q, k, v, state, grad_out, grad_final_state, grad_q, grad_k, grad_v, grad_log_decay,
-                                 grad_state, (char *)workspace, (hipStream_t)stream);
-    return backward_t<bf16>(call, q, k, v, state, grad_out, grad_final_state, grad_q, grad_k, grad_v, grad_log_decay,
-                            grad_state, (char *)workspace, (hipStream_t)stream);
+        return backward_t<float>(call, q, k, v, state, (const float *)kept, grad_out, grad_final_state, grad_q, grad_k, grad_v,
+                                 grad_log_decay, grad_state, (char *)workspace, (hipStream_t)stream);
+    return backward_t<bf16>(call, q, k, v, state, (const float *)kept, grad_out, grad_final_state, grad_q, grad_k, grad_v,
+                            grad_log_decay, grad_state, (char *)workspace, (hipStream_t)stream);
 }
 
 int pathsig_linattn_step(const pathsig_linattn *call, const void *q, const void *k, const void *v, float *state, void *out,

@@ -20,6 +20,8 @@ struct StateRef {
     int64_t row, column;
 };
 
+constexpr float kLog2e = 1.44269504088896340736f;
+
 // One pass of the recurrence over all tokens, S <- decay S + in_scale k v^T, out = out_scale S^T q, or backwards in time, where
 // the decay comes after the token: S <- S + in_scale k v^T, out = out_scale S^T q, S <- decay S.  Dk and Dv are the rows and
 // columns of this pass' state, whichever tensors are in the places of k and v.
@@ -34,12 +36,17 @@ struct Sweep {
     int H, Dk, Dv;
     float in_scale, out_scale;
     int reverse;
-    // the sequence in pieces of `piece` tokens: states in front of each, [pieces][B][H][Dk * Dv], in first's order of rows
-    // and columns of `starts`
+    int exact_state;       // the state is wanted in 32 bits, not only the answers
+    // the sequence in pieces of `piece` tokens: starts [pieces][B][H][Dk * Dv], whose s-th entry is the state in front of piece s
+    // or, with few pieces (kJoinInside), what piece s - 1 adds to a state of zero
     int64_t piece;
     int pieces;
     StateRef starts;
 };
+
+// Up to so many pieces, every block adds up the pieces before its own by itself: at most 1.5 states read for each block instead of
+// a launch that reads all of them and writes them back (measured with two pieces of 256 heads, 128 x 128: 25 us).
+constexpr int kJoinInside = 4;
 
 __device__ __forceinline__ int64_t length_of(const int32_t *lengths, int64_t b, int64_t L) {
     if (!lengths) return L;
@@ -63,17 +70,14 @@ __device__ __forceinline__ Range range_of(const Sweep &a, int64_t n, int s) {
     return a.reverse ? Range{n - t1, n - t0} : Range{t0, t1};
 }
 
-constexpr float kLog2e = 1.44269504088896340736f;
-
 // seq_chunks.hip, for keys of up to 32 DKT channels.  fold: only the states that the pieces add, from zero, into starts[s + 1].
 template <typename T, int DKT>
 void launch_chunks(const Sweep &a, bool fold, hipStream_t stream);
 
-// The gradient of the decays: partial sums [pieces][slices][B][H], slices = ceil(Dv / 128), for the sweep forwards in time.
-// ends: the gradients of the states behind the pieces, the first piece's at the end (as a sweep backwards in time leaves them in
-// its `starts`), or with one piece that of the last state or NULL.
+// The gradient of the decays: partial sums [pieces][slices][B][H], slices = ceil(Dv / 128).  a: the sweep forwards in time; back: the
+// one backwards in time with the same rows and columns, whose states are the gradients of a's.
 template <typename T, int DKT>
-void launch_decay(const Sweep &a, const View &grad_out, const StateRef &ends, float *partial, hipStream_t stream);
+void launch_decay(const Sweep &a, const Sweep &back, const View &grad_out, float *partial, hipStream_t stream);
 
 }  // namespace seq
 }  // namespace psig

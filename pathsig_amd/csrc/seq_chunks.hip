@@ -166,17 +166,23 @@ struct Fetch {
     u32x4 x[kEach];
 
     // p: the tile's first row and channel.  The rows before `pad` are zeros and not read, as are channels from `channels` on.
-    // st: from row to row, backwards in time negative.
-    __device__ __forceinline__ void load(const T *p, int st, int channels, int vectors, int pad) {
+    // st: from row to row, backwards in time negative.  VECTORS: whole units at addresses of whole units.
+    template <bool VECTORS>
+    __device__ __forceinline__ void load(const T *p, int st, int channels, int pad) {
         const int row0 = threadIdx.x / L::kUnits, c = threadIdx.x % L::kUnits * L::kPerUnit;
         const int offset = row0 * st + c;
+        if (VECTORS && kTotal % THREADS == 0 && pad <= 0 && channels >= D) {
+#pragma unroll
+            for (int u = 0; u < kEach; ++u) x[u] = *(const u32x4 *)(p + (int64_t)u * kRowsApart * st + offset);
+            return;
+        }
 #pragma unroll
         for (int u = 0; u < kEach; ++u) {
             const int row = row0 + u * kRowsApart;
             x[u] = u32x4{0, 0, 0, 0};
             if ((kTotal % THREADS && row >= ROWS) || row < pad || c >= channels) continue;
             const T *const q = p + (int64_t)u * kRowsApart * st + offset;
-            if (vectors) {
+            if constexpr (VECTORS) {
                 x[u] = *(const u32x4 *)q;
             } else {
                 Pack<T, L::kPerUnit> one = {};
@@ -198,25 +204,17 @@ struct Fetch {
     }
 };
 
-// l^(C-1-j) v_j in terms of the type of the products: all bits of it (three of bf16)
-template <typename T>
-struct Terms;
-template <>
-struct Terms<float> {
-    static constexpr int kCount = 1;
-    static __device__ __forceinline__ void split(f32x8 x, f32x8 (&out)[1]) { out[0] = x; }
-};
-template <>
-struct Terms<bf16> {
-    static constexpr int kCount = 3;
-    static __device__ __forceinline__ void split(f32x8 x, bf16x8 (&out)[3]) {
+// f x in COUNT terms of the type of the products; three of bf16 hold all 24 bits
+template <typename T, int COUNT>
+__device__ __forceinline__ void split_scaled(f32x8 x, const f32x8 &f, Frag<T> (&out)[COUNT]) {
 #pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            out[i] = rounded<bf16>(x);
-            x -= widened(out[i]);
-        }
+    for (int e = 0; e < 8; ++e) x[e] *= f[e];
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+        out[i] = rounded<T>(x);
+        if (i + 1 < COUNT) x -= widened(out[i]);
     }
-};
+}
 
 // Bytes that a thread fetches of a chunk of 32 tiles tokens.
 constexpr int fetched(int element, int tiles, int DKT, int NW) { return 32 * tiles * (2 * 32 * DKT + 32 * NW) * element / (64 * NW); }
@@ -228,19 +226,49 @@ constexpr int chunk_tiles(int DKT, int NW) {
     return sizeof(T) == 2 && fetched(2, 2, DKT, NW) <= 320 ? 2 : 1;
 }
 
-template <typename T, typename O, int DKT, int NW, bool FOLD>
+// The state in front of a piece (FOLD: zero): this lane's column dv, rows in accumulator order.
+template <int DKT, bool FOLD>
+__device__ __forceinline__ void load_state(f32x16 (&S)[DKT], const Sweep &a, int64_t b, int h, int64_t n, int piece, float g2, int dv,
+                                           int half) {
+    const int64_t plane = (int64_t)a.Dk * a.Dv, head = (b * a.H + h) * plane, between = a.B * a.H * plane;
+#pragma unroll
+    for (int t = 0; t < DKT; ++t) S[t] = f32x16{};
+    if (FOLD) return;
+    auto add = [&](const float *p, int64_t row, int64_t column, float f) {
+        p += dv * column + 4 * half * row;
+#pragma unroll
+        for (int t = 0; t < DKT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                S[t][r] = S[t][r] * f + (32 * t + acc_row(r, half) < a.Dk && dv < a.Dv ? p[(32 * t + acc_row(r, 0)) * row] : 0.f);
+    };
+    if (a.pieces > kJoinInside) return add(a.starts.p + piece * between + head, a.starts.row, a.starts.column, 0.f);
+    if (a.first.p) add(a.first.p + head, a.first.row, a.first.column, 0.f);
+    for (int s = 0; s < piece; ++s) {
+        const Range r = range_of(a, n, s);
+        add(a.starts.p + (s + 1) * between + head, a.starts.row, a.starts.column, exp2f(g2 * (float)(r.end - r.begin)));
+    }
+}
+
+// TERMS: of l^(C-1-j) v_j in the state's update.
+template <typename T, typename O, int DKT, int NW, int TERMS, bool FOLD, bool VECTORS>
 __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_kernel(const Sweep a, int slices) {
     constexpr int DK = 32 * DKT, DV = 32 * NW, CT = chunk_tiles<T>(DKT, NW), C = 32 * CT, THREADS = 64 * NW;
     // fetched a chunk ahead, where registers allow it
     constexpr bool kAhead = fetched(sizeof(T), CT, DKT, NW) <= 320;
+    // Scores: tiles (j, i) = (0, 0), (0, 1), (1, 1) are dealt to the waves; a single tile is split along the channels instead
+    constexpr int kTiles = CT * (CT + 1) / 2, kParts = CT == 1 ? (NW < 2 * DKT ? NW : 2 * DKT) : 1, kSteps = DK / 16 / kParts;
     using KTile = Tile<T, DK>;
     using VTile = Tile<T, DV>;
     constexpr int kKBytes = C * KTile::kRow, kVBytes = C * VTile::kRow;
     __shared__ __align__(16) char lds[kKBytes * (FOLD ? 1 : 2) + kVBytes];
-    __shared__ __align__(16) f32x4 table_later[4][2], table_diagonal[FOLD ? 1 : 4][64];
+    __shared__ __align__(16) f32x4 table_left[CT][4][2], table_later[4][2], table_diagonal[FOLD ? 1 : 4][64];
+    // rounded scores as operands, or the parts of a tile's sums
+    __shared__ __align__(16) Frag<T> scores[FOLD || kParts > 1 ? 1 : kTiles][2][64];
+    __shared__ __align__(16) f32x4 sums[!FOLD && kParts > 1 ? kParts : 1][4][64];
     char *const lds_k = lds, *const lds_v = lds + kKBytes, *const lds_q = lds_v + kVBytes;
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, ln = lane & 31;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, ln = lane & 31;
     const int slice = blockIdx.x % slices, h = blockIdx.x / slices, piece = blockIdx.y;
     const int64_t b = blockIdx.z;
     const int dv0 = slice * DV, dv = dv0 + 32 * wave + ln;  // this lane's column of the state
@@ -261,38 +289,26 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
     if (begin >= end && !owns_end && !FOLD) return;
 
     f32x16 S[DKT];
-    {
-        const float *from = nullptr;
-        int64_t row = 0, column = 0;
-        if (!FOLD && a.pieces > 1) {
-            from = a.starts.p + (int64_t)piece * a.B * a.H * plane + head;
-            row = a.starts.row;
-            column = a.starts.column;
-        } else if (!FOLD && a.first.p) {
-            from = a.first.p + head;
-            row = a.first.row;
-            column = a.first.column;
-        }
-#pragma unroll
-        for (int t = 0; t < DKT; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int dk = 32 * t + acc_row(r, half);
-                S[t][r] = from && dk < a.Dk && dv < a.Dv ? from[dk * row + dv * column] : 0.f;
-            }
-    }
+    load_state<DKT, FOLD>(S, a, b, h, n, piece, g2, dv, half);
 
-    // factors of a lane's registers: l^(31 - j), and l^(i - j) in a tile on the diagonal (j after i is masked where it is used).  In
-    // LDS: 32 registers that are read once a chunk
+    // Factors of a lane's registers, in LDS (they would fill the registers, and are read once a chunk): l^(C - 1 - j) for the state's
+    // update; for scores l^(31 - j), which l^(i + 1) completes in the tile off the diagonal, and l^(i - j) in those on it (j after i
+    // is masked where it is used)
+    const float both = a.in_scale * a.out_scale;
     if (threadIdx.x < 64) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int j = acc_row(r, half);
-            if (ln == 0) table_later[r / 4][half][r % 4] = exp2f(g2 * (float)(31 - j));
-            if constexpr (!FOLD) table_diagonal[r / 4][lane][r % 4] = a.in_scale * exp2f(g2 * (float)max(ln - j, 0));
+            if (ln == 0) {
+                table_later[r / 4][half][r % 4] = exp2f(g2 * (float)(31 - j));
+#pragma unroll
+                for (int t = 0; t < CT; ++t)
+                    table_left[t][r / 4][half][r % 4] = a.in_scale * exp2f(g2 * (float)(C - 1 - 32 * t - j + a.reverse));
+            }
+            if constexpr (!FOLD) table_diagonal[r / 4][lane][r % 4] = both * exp2f(g2 * (float)max(ln - j, 0));
         }
     }
-    const float since = a.in_scale * exp2f(g2 * (float)(ln + 1));
+    const float since = both * exp2f(g2 * (float)(ln + 1));
 
     const T *const kp = (const T *)a.k.p + b * a.k.sb + (h / a.k.group) * a.k.sh;
     const T *const vp = (const T *)a.v.p + b * a.v.sb + (h / a.v.group) * a.v.sh + dv0;
@@ -302,32 +318,35 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
     Fetch<T, DV, C, THREADS> fv;
     const int chunks = (int)((max(end - begin, (int64_t)0) + C - 1) / C);
     int64_t r0 = end - (int64_t)chunks * C;  // of the chunk being worked on; before `begin` where the first is not full
+    // (where registers do not hold a whole chunk, the tensors pass through them one after the other)
     auto fetch = [&](int64_t at, int pad) {
         const int64_t t = a.reverse ? n - 1 - at : at;
-        fk.load(kp + t * a.k.st, sign * (int)a.k.st, a.Dk, a.k.vectors, pad);
+        fk.template load<VECTORS>(kp + t * a.k.st, sign * (int)a.k.st, a.Dk, pad);
         if (!kAhead) fk.store(lds_k);
-        fv.load(vp + t * a.v.st, sign * (int)a.v.st, a.Dv - dv0, a.v.vectors, pad);
+        fv.template load<VECTORS>(vp + t * a.v.st, sign * (int)a.v.st, a.Dv - dv0, pad);
         if (!kAhead) fv.store(lds_v);
-        if (!FOLD) fq.load(qp + t * a.q.st, sign * (int)a.q.st, a.Dk, a.q.vectors, pad);
+        if (!FOLD) fq.template load<VECTORS>(qp + t * a.q.st, sign * (int)a.q.st, a.Dk, pad);
         if (!kAhead && !FOLD) fq.store(lds_q);
     };
-    if (kAhead && chunks > 0) fetch(r0, (int)(begin - r0));
+    auto store = [&]() {
+        fk.store(lds_k);
+        fv.store(lds_v);
+        if (!FOLD) fq.store(lds_q);
+    };
+    if (chunks > 0) {
+        fetch(r0, (int)(begin - r0));
+        if (kAhead) {
+            store();
+            if (chunks > 1) fetch(r0 + C, 0);
+        }
+    }
     const int row_base_of_lane = KTile::row_base(ln, half);
     int k_bases_of_lane[KTile::kColumnBases], v_bases_of_lane[VTile::kColumnBases];
     KTile::column_bases(k_bases_of_lane, lane);
     VTile::column_bases(v_bases_of_lane, lane);
     for (int c = 0; c < chunks; ++c, r0 += C) {
         const int pad = (int)max(begin - r0, (int64_t)0);
-        __syncthreads();  // the tiles of the chunk before are read
-        if (kAhead) {
-            fk.store(lds_k);
-            fv.store(lds_v);
-            if (!FOLD) fq.store(lds_q);
-        } else {
-            fetch(r0, pad);
-        }
-        __syncthreads();
-        if (kAhead && c + 1 < chunks) fetch(r0 + C, 0);
+        __syncthreads();  // this chunk's tiles are in LDS, the scores of the chunk before are read
 
         // (addresses are worked out from these in every chunk: held for all reads, they would fill the registers)
         int row_base = row_base_of_lane, k_bases[KTile::kColumnBases], v_bases[VTile::kColumnBases];
@@ -339,38 +358,105 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
             asm volatile("" : "+v"(k_bases[g]), "+v"(v_bases[g]));
         }
 
+        // scores
+        f32x16 out[FOLD ? 1 : CT];
+        if constexpr (!FOLD) {
+            if constexpr (kParts > 1) {
+                if (wave < kParts) {
+                    f32x16 P = {};
+                    const int base = row_base ^ (wave * kSteps * 16 * (int)sizeof(T));
+#pragma unroll
+                    for (int kk = 0; kk < kSteps; ++kk) P = mma(KTile::row(lds_k, base, 0, kk), KTile::row(lds_q, base, 0, kk), P);
+#pragma unroll
+                    for (int r4 = 0; r4 < 4; ++r4) sums[wave][r4][lane] = f32x4{P[4 * r4], P[4 * r4 + 1], P[4 * r4 + 2], P[4 * r4 + 3]};
+                }
+            } else {
+                for (int tile = wave; tile < kTiles; tile += NW) {
+                    const int i = tile > 0, j = tile > 1;
+                    f32x16 P = {};
+                    const char *const kt = lds_k + j * 32 * KTile::kRow, *const qt = lds_q + i * 32 * KTile::kRow;
+#pragma unroll
+                    for (int kk = 0; kk < DK / 16; ++kk) P = mma(KTile::row(kt, row_base, 0, kk), KTile::row(qt, row_base, 0, kk), P);
+                    if (i == j) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            // (selected, not multiplied by zero: a score of a later token may be infinite)
+                            P[r] = acc_row(r, half) <= ln ? P[r] * table_diagonal[r / 4][lane][r % 4] : 0.f;
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) P[r] *= table_later[r / 4][half][r % 4] * since;
+                    }
+                    scores[tile][0][lane] = rounded<T>(half_of<0>(P));
+                    scores[tile][1][lane] = rounded<T>(half_of<1>(P));
+                }
+            }
+            // answers from the state
+#pragma unroll
+            for (int i = 0; i < CT; ++i) out[i] = f32x16{};
+#pragma unroll
+            for (int kk = 0; kk < DK / 16; ++kk) {
+                const Frag<T> st = rounded<T>(kk % 2 ? half_of<1>(S[kk / 2]) : half_of<0>(S[kk / 2]));
+#pragma unroll
+                for (int i = 0; i < CT; ++i) out[i] = mma(st, KTile::row(lds_q, row_base, i, kk), out[i]);
+            }
+        }
+
+        // the state after the chunk
+        Frag<T> vt[CT][2];
+        const float whole = exp2f(g2 * (float)(C - pad));
+#pragma unroll
+        for (int t = 0; t < DKT; ++t) S[t] *= whole;
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                vt[j][s] = VTile::column(lds_v, v_bases, 0, 2 * j + s);
+                f32x8 f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = table_left[j][2 * s + e / 4][half][e % 4];
+                Frag<T> terms[TERMS];
+                split_scaled<T>(widened(vt[j][s]), f, terms);
+#pragma unroll
+                for (int t = 0; t < DKT; ++t) {
+                    const Frag<T> kt = KTile::column(lds_k, k_bases, t, 2 * j + s);
+#pragma unroll
+                    for (int i = 0; i < TERMS; ++i) S[t] = mma(kt, terms[i], S[t]);
+                }
+            }
+        }
+
+        __syncthreads();  // the tiles are read, the scores are in LDS
+        if (c + 1 < chunks) {
+            if (kAhead) {
+                store();
+                if (c + 2 < chunks) fetch(r0 + 2 * C, 0);
+            } else {
+                fetch(r0 + C, 0);
+            }
+        }
         if constexpr (!FOLD) {
 #pragma unroll
             for (int i = 0; i < CT; ++i) {
-                f32x16 P[CT], out = f32x16{};
-#pragma unroll
-                for (int j = 0; j <= i; ++j) P[j] = f32x16{};
-#pragma unroll
-                for (int kk = 0; kk < DK / 16; ++kk) {
-                    const Frag<T> q = KTile::row(lds_q, row_base, i, kk);
-                    const Frag<T> st = rounded<T>(kk % 2 ? half_of<1>(S[kk / 2]) : half_of<0>(S[kk / 2]));
-                    out = mma(st, q, out);
-#pragma unroll
-                    for (int j = 0; j <= i; ++j) P[j] = mma(KTile::row(lds_k, row_base, j, kk), q, P[j]);
-                    if (kk % 2) __builtin_amdgcn_sched_barrier(0);  // operands of a few steps ahead fill the registers
-                }
                 // (rows of padding have answers that no one reads; their exponent is kept from turning around)
-                out *= exp2f(g2 * (float)max(32 * i + ln + 1 - a.reverse - pad, 0));
-#pragma unroll
-                for (int j = 0; j <= i; ++j) {
+                out[i] *= a.out_scale * exp2f(g2 * (float)max(32 * i + ln + 1 - a.reverse - pad, 0));
+                if constexpr (kParts > 1) {
+                    f32x8 P[2];
 #pragma unroll
                     for (int r4 = 0; r4 < 4; ++r4) {
-                        const f32x4 f = j == i ? table_diagonal[r4][lane] : table_later[r4][half] * since;
+                        f32x4 x = sums[0][r4][lane];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int r = 4 * r4 + e;
-                            P[j][r] *= f[e];
-                            // (selected, not multiplied by zero: a score of a later token may be infinite)
-                            if (j == i && acc_row(r, half) > ln) P[j][r] = 0.f;
-                        }
+                        for (int w = 1; w < kParts; ++w) x += sums[w][r4][lane];
+                        x *= table_diagonal[r4][lane];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) P[r4 / 2][r4 % 2 * 4 + e] = acc_row(4 * r4 + e, half) <= ln ? x[e] : 0.f;
                     }
-                    out = mma(VTile::column(lds_v, v_bases, 0, 2 * j), rounded<T>(half_of<0>(P[j])), out);
-                    out = mma(VTile::column(lds_v, v_bases, 0, 2 * j + 1), rounded<T>(half_of<1>(P[j])), out);
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) out[i] = mma(vt[0][s], rounded<T>(P[s]), out[i]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j <= i; ++j)
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) out[i] = mma(vt[j][s], scores[i + j][s][lane], out[i]);
                 }
                 const int row = 32 * i + ln;
                 if (row >= pad) {
@@ -379,48 +465,20 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
                         const int d = dv0 + 32 * wave + 8 * g + 4 * half;
-                        if (a.Dv % 4 == 0) {
+                        if constexpr (VECTORS) {
                             if (d < a.Dv) {
                                 Pack<O, 4> four;
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) four.v[e] = from_float<O>(out[4 * g + e] * a.out_scale);
+                                for (int e = 0; e < 4; ++e) four.v[e] = from_float<O>(out[i][4 * g + e]);
                                 *(Pack<O, 4> *)(to + d) = four;
                             }
                         } else {
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
-                                if (d + e < a.Dv) to[d + e] = from_float<O>(out[4 * g + e] * a.out_scale);
+                                if (d + e < a.Dv) to[d + e] = from_float<O>(out[i][4 * g + e]);
                         }
                     }
                 }
-            }
-        }
-
-        // the state after the chunk
-        const float whole = exp2f(g2 * (float)(C - pad));
-#pragma unroll
-        for (int t = 0; t < DKT; ++t) S[t] *= whole;
-#pragma unroll
-        for (int j = 0; j < CT; ++j) {
-            const float rest = a.in_scale * exp2f(g2 * (float)(32 * (CT - 1 - j) + a.reverse));
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                f32x8 x = widened(VTile::column(lds_v, v_bases, 0, 2 * j + s));
-#pragma unroll
-                for (int r4 = 0; r4 < 2; ++r4) {
-                    const f32x4 f = table_later[2 * s + r4][half] * rest;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[4 * r4 + e] *= f[e];
-                }
-                Frag<T> terms[Terms<T>::kCount];
-                Terms<T>::split(x, terms);
-#pragma unroll
-                for (int t = 0; t < DKT; ++t) {
-                    const Frag<T> kt = KTile::column(lds_k, k_bases, t, 2 * j + s);
-#pragma unroll
-                    for (int i = 0; i < Terms<T>::kCount; ++i) S[t] = mma(kt, terms[i], S[t]);
-                }
-                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
@@ -454,17 +512,6 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
 // Every term is a sum of like signs or of independent ones; sum over t of t (q_t . dq_t - k_t . dk_t), which needs no states,
 // cancels by the length of the sequence over the memory of the head.  Products of states stay in 32 bits (element by element on
 // accumulators); what enters them is split into two bf16 terms (relative 2^-18 a term).
-template <typename T, int COUNT>
-__device__ __forceinline__ void split_scaled(f32x8 x, const f32x8 &f, Frag<T> (&out)[COUNT]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= f[e];
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i) {
-        out[i] = rounded<T>(x);
-        x -= widened(out[i]);
-    }
-}
-
 __device__ __forceinline__ float sum16(f32x16 x) {
     float s = 0.f;
 #pragma unroll
@@ -472,8 +519,8 @@ __device__ __forceinline__ float sum16(f32x16 x) {
     return s;
 }
 
-template <typename T, int DKT, int NW>
-__global__ __launch_bounds__(64 * NW, 1) void decay_kernel(const Sweep a, const View grad, const StateRef ends, float *partial,
+template <typename T, int DKT, int NW, bool VECTORS>
+__global__ __launch_bounds__(64 * NW, 1) void decay_kernel(const Sweep a, const Sweep back, const View grad, float *partial,
                                                          int slices) {
     constexpr int DK = 32 * DKT, DV = 32 * NW, THREADS = 64 * NW, TERMS = sizeof(T) == 2 ? 2 : 1;
     constexpr int CT = chunk_tiles<T>(DKT, NW), C = 32 * CT;
@@ -491,20 +538,11 @@ __global__ __launch_bounds__(64 * NW, 1) void decay_kernel(const Sweep a, const 
     const int64_t n = length_of(a.lengths, b, a.L);
     const auto [begin, end] = range_of(a, n, piece);
     const float g2 = decay_of(a.log_decay, h) * kLog2e;
-    const int64_t plane = (int64_t)a.Dk * a.Dv, head = (b * a.H + h) * plane, between = a.B * a.H * plane;
 
     f32x16 S[DKT], D[DKT];
-    {
-        const StateRef from = a.pieces > 1 ? StateRef{a.starts.p + piece * between, a.starts.row, a.starts.column} : a.first;
+    load_state<DKT, false>(S, a, b, h, n, piece, g2, dv, half);
 #pragma unroll
-        for (int t = 0; t < DKT; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int dk = 32 * t + acc_row(r, half);
-                S[t][r] = from.p && dk < a.Dk && dv < a.Dv ? from.p[head + dk * from.row + dv * from.column] : 0.f;
-                D[t][r] = 0.f;
-            }
-    }
+    for (int t = 0; t < DKT; ++t) D[t] = f32x16{};
     const T *const kp = (const T *)a.k.p + b * a.k.sb + (h / a.k.group) * a.k.sh;
     const T *const vp = (const T *)a.v.p + b * a.v.sb + (h / a.v.group) * a.v.sh + dv0;
     const T *const qp = (const T *)a.q.p + b * a.q.sb + (h / a.q.group) * a.q.sh;
@@ -521,14 +559,14 @@ __global__ __launch_bounds__(64 * NW, 1) void decay_kernel(const Sweep a, const 
         __syncthreads();
         {
             Fetch<T, DK, C, THREADS> x;
-            x.load(kp + r0 * a.k.st, (int)a.k.st, a.Dk, a.k.vectors, pad);
+            x.template load<VECTORS>(kp + r0 * a.k.st, (int)a.k.st, a.Dk, pad);
             x.store(lds_k);
-            x.load(qp + r0 * a.q.st, (int)a.q.st, a.Dk, a.q.vectors, pad);
+            x.template load<VECTORS>(qp + r0 * a.q.st, (int)a.q.st, a.Dk, pad);
             x.store(lds_q);
             Fetch<T, DV, C, THREADS> y;
-            y.load(vp + r0 * a.v.st, (int)a.v.st, a.Dv - dv0, a.v.vectors, pad);
+            y.template load<VECTORS>(vp + r0 * a.v.st, (int)a.v.st, a.Dv - dv0, pad);
             y.store(lds_v);
-            y.load(op + r0 * grad.st, (int)grad.st, a.Dv - dv0, grad.vectors, pad);
+            y.template load<VECTORS>(op + r0 * grad.st, (int)grad.st, a.Dv - dv0, pad);
             y.store(lds_o);
         }
         __syncthreads();
@@ -625,16 +663,10 @@ __global__ __launch_bounds__(64 * NW, 1) void decay_kernel(const Sweep a, const 
         }
     }
     total *= a.out_scale;
-    if (ends.p) {
-        const float *const from = ends.p + (a.pieces > 1 ? (a.pieces - 1 - piece) * between : 0) + head;
+    // the gradient of the state behind the piece
+    load_state<DKT, false>(S, back, b, h, n, a.pieces - 1 - piece, g2, dv, half);
 #pragma unroll
-        for (int t = 0; t < DKT; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int dk = 32 * t + acc_row(r, half);
-                if (dk < a.Dk && dv < a.Dv) total += D[t][r] * from[dk * ends.row + dv * ends.column];
-            }
-    }
+    for (int t = 0; t < DKT; ++t) total += sum16(D[t] * S[t]);
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) total += __shfl_xor(total, m);
     if (lane == 0) meet[wave] = total;
@@ -644,43 +676,70 @@ __global__ __launch_bounds__(64 * NW, 1) void decay_kernel(const Sweep a, const 
     partial[(((int64_t)piece * slices + slice) * a.B + b) * a.H + h] = total;
 }
 
-template <typename T, int DKT, int NW>
+// Whole units of 16 bytes everywhere: all rows start at addresses of units, and heads have whole units of channels (a head that
+// ends inside a unit would read its neighbour's channels, or a view's hidden ones).
+bool whole_units(const Sweep &a, int element, bool more = true) {
+    const int E = 16 / element;
+    return more && (a.q.vectors || !a.q.p) && a.k.vectors && a.v.vectors && a.Dk % E == 0 && a.Dv % E == 0 && aligned16(a.out);
+}
+
+template <typename T, int DKT, int NW, int TERMS, bool VECTORS>
 void launch_width(const Sweep &a, bool fold, hipStream_t stream) {
     const int slices = (int)ceil_div(a.Dv, 32 * NW);
     const dim3 grid((unsigned)(slices * a.H), (unsigned)(fold ? a.pieces - 1 : a.pieces), (unsigned)a.B), block(64 * NW);
     if (fold)
-        chunk_kernel<T, T, DKT, NW, true><<<grid, block, 0, stream>>>(a, slices);
+        chunk_kernel<T, T, DKT, NW, TERMS, true, VECTORS><<<grid, block, 0, stream>>>(a, slices);
     else if (a.out_float && sizeof(T) == 2)
-        chunk_kernel<T, float, DKT, NW, false><<<grid, block, 0, stream>>>(a, slices);
+        chunk_kernel<T, float, DKT, NW, TERMS, false, VECTORS><<<grid, block, 0, stream>>>(a, slices);
     else
-        chunk_kernel<T, T, DKT, NW, false><<<grid, block, 0, stream>>>(a, slices);
+        chunk_kernel<T, T, DKT, NW, TERMS, false, VECTORS><<<grid, block, 0, stream>>>(a, slices);
+}
+
+// A state that is handed out in 32 bits is summed from all bits of its terms.  One that only answers, through a copy in the type
+// of the products, is summed from terms of that type: each is off by as much as the copy is.
+template <typename T, int DKT, int NW, bool VECTORS>
+void launch_terms(const Sweep &a, bool fold, hipStream_t stream) {
+    if constexpr (sizeof(T) == 2)
+        if (a.exact_state) return launch_width<T, DKT, NW, 3, VECTORS>(a, fold, stream);
+    launch_width<T, DKT, NW, 1, VECTORS>(a, fold, stream);
+}
+
+template <typename T, int DKT, int NW>
+void launch_aligned(const Sweep &a, bool fold, hipStream_t stream) {
+    if (whole_units(a, sizeof(T))) return launch_terms<T, DKT, NW, true>(a, fold, stream);
+    launch_terms<T, DKT, NW, false>(a, fold, stream);
+}
+
+template <typename T, int DKT, int NW>
+void launch_decay_width(const Sweep &a, const Sweep &back, const View &grad, float *partial, hipStream_t stream) {
+    const int slices = (int)ceil_div(a.Dv, 32 * NW);
+    const dim3 grid((unsigned)(slices * a.H), (unsigned)a.pieces, (unsigned)a.B), block(64 * NW);
+    if (whole_units(a, sizeof(T), grad.vectors))
+        decay_kernel<T, DKT, NW, true><<<grid, block, 0, stream>>>(a, back, grad, partial, slices);
+    else
+        decay_kernel<T, DKT, NW, false><<<grid, block, 0, stream>>>(a, back, grad, partial, slices);
 }
 
 }  // namespace
 
 template <typename T, int DKT>
 void launch_chunks(const Sweep &a, bool fold, hipStream_t stream) {
-    if (a.Dv <= 32) return launch_width<T, DKT, 1>(a, fold, stream);
-    if (a.Dv <= 64) return launch_width<T, DKT, 2>(a, fold, stream);
-    launch_width<T, DKT, 4>(a, fold, stream);
+    if (a.Dv <= 32) return launch_aligned<T, DKT, 1>(a, fold, stream);
+    if (a.Dv <= 64) return launch_aligned<T, DKT, 2>(a, fold, stream);
+    launch_aligned<T, DKT, 4>(a, fold, stream);
 }
 
 template <typename T, int DKT>
-void launch_decay(const Sweep &a, const View &grad_out, const StateRef &ends, float *partial, hipStream_t stream) {
-    const int slices = (int)ceil_div(a.Dv, 128);
-    const dim3 grid((unsigned)(slices * a.H), (unsigned)a.pieces, (unsigned)a.B);
-    if (a.Dv <= 32)
-        decay_kernel<T, DKT, 1><<<grid, 64, 0, stream>>>(a, grad_out, ends, partial, slices);
-    else if (a.Dv <= 64)
-        decay_kernel<T, DKT, 2><<<grid, 128, 0, stream>>>(a, grad_out, ends, partial, slices);
-    else
-        decay_kernel<T, DKT, 4><<<grid, 256, 0, stream>>>(a, grad_out, ends, partial, slices);
+void launch_decay(const Sweep &a, const Sweep &back, const View &grad_out, float *partial, hipStream_t stream) {
+    if (a.Dv <= 32) return launch_decay_width<T, DKT, 1>(a, back, grad_out, partial, stream);
+    if (a.Dv <= 64) return launch_decay_width<T, DKT, 2>(a, back, grad_out, partial, stream);
+    launch_decay_width<T, DKT, 4>(a, back, grad_out, partial, stream);
 }
 
 template void launch_chunks<float, PSIG_KEY_TILES>(const Sweep &, bool, hipStream_t);
 template void launch_chunks<bf16, PSIG_KEY_TILES>(const Sweep &, bool, hipStream_t);
-template void launch_decay<float, PSIG_KEY_TILES>(const Sweep &, const View &, const StateRef &, float *, hipStream_t);
-template void launch_decay<bf16, PSIG_KEY_TILES>(const Sweep &, const View &, const StateRef &, float *, hipStream_t);
+template void launch_decay<float, PSIG_KEY_TILES>(const Sweep &, const Sweep &, const View &, float *, hipStream_t);
+template void launch_decay<bf16, PSIG_KEY_TILES>(const Sweep &, const Sweep &, const View &, float *, hipStream_t);
 
 }  // namespace seq
 }  // namespace psig

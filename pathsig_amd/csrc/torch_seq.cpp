@@ -102,10 +102,13 @@ AttentionCall attention_call(const Tensor &q, const Tensor &k, const Tensor &v, 
     return a;
 }
 
-std::tuple<Tensor, Tensor> attention_forward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay,
-                                             const Tensor &state, const Tensor &lengths, double scale, bool return_state) {
+// (out, last state or an empty tensor, the workspace: what the backward of the same call can use again, or undefined)
+std::tuple<Tensor, Tensor, Tensor> attention_forward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay,
+                                                     const Tensor &state, const Tensor &lengths, double scale, bool return_state,
+                                                     bool learned_decay) {
     c10::DeviceGuard guard(q.device());
-    const AttentionCall a = attention_call(q, k, v, log_decay, state, lengths, scale, true);
+    AttentionCall a = attention_call(q, k, v, log_decay, state, lengths, scale, true);
+    a.c.learned_decay = learned_decay;
     Tensor out = at::empty({a.c.B, a.c.L, a.c.H, a.c.Dv}, a.q.options());
     Tensor last = return_state ? at::empty({a.c.B, a.c.H, a.c.Dk, a.c.Dv}, a.log_decay.options())
                                : at::empty({0}, a.log_decay.options());
@@ -113,17 +116,18 @@ std::tuple<Tensor, Tensor> attention_forward(const Tensor &q, const Tensor &k, c
     Tensor ws = scratch(ws_bytes, a.q);
     check_rc(pathsig_linattn_forward(&a.c, ptr(a.q), ptr(a.k), ptr(a.v), (const float *)ptr(a.state), ptr(out),
                                      (float *)ptr(last), ptr(ws), ws_bytes, stream_of(a.q)));
-    return {out, last};
+    return {out, last, ws};
 }
 
 using Gradients = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
 
 // the gradients of log_decay and state are empty tensors where they are not wanted
 Gradients attention_backward(const Tensor &grad_out_in, const Tensor &grad_last_in, const Tensor &q, const Tensor &k,
-                             const Tensor &v, const Tensor &log_decay, const Tensor &state, const Tensor &lengths, double scale,
-                             bool want_decay, bool want_state) {
+                             const Tensor &v, const Tensor &log_decay, const Tensor &state, const Tensor &lengths,
+                             const Tensor &kept, double scale, bool want_decay, bool want_state) {
     c10::DeviceGuard guard(q.device());
-    const AttentionCall a = attention_call(q, k, v, log_decay, state, lengths, scale, true);
+    AttentionCall a = attention_call(q, k, v, log_decay, state, lengths, scale, true);
+    a.c.learned_decay = want_decay;
     check_like(grad_out_in, "grad_out", q, "q");
     TORCH_CHECK(grad_out_in.scalar_type() == q.scalar_type(), "grad_out must have same dtype as q");
     TORCH_CHECK(grad_out_in.sizes() == at::IntArrayRef({a.c.B, a.c.L, a.c.H, a.c.Dv}), "grad_out must be [B, L, H, Dv]");
@@ -142,8 +146,8 @@ Gradients attention_backward(const Tensor &grad_out_in, const Tensor &grad_last_
                                : at::empty({0}, a.log_decay.options());
     const size_t ws_bytes = pathsig_linattn_backward_workspace(&a.c, want_decay);
     Tensor ws = scratch(ws_bytes, a.q);
-    check_rc(pathsig_linattn_backward(&a.c, ptr(a.q), ptr(a.k), ptr(a.v), (const float *)ptr(a.state), ptr(grad_out),
-                                      (const float *)ptr(grad_last), ptr(dq), ptr(dk), ptr(dv), (float *)ptr(ddecay),
+    check_rc(pathsig_linattn_backward(&a.c, ptr(a.q), ptr(a.k), ptr(a.v), (const float *)ptr(a.state), ptr(kept),
+                                      kept.defined() ? (size_t)kept.numel() : 0, ptr(grad_out), (const float *)ptr(grad_last), ptr(dq), ptr(dk), ptr(dv), (float *)ptr(ddecay),
                                       (float *)ptr(dstate), ptr(ws), ws_bytes, stream_of(a.q)));
     return {dq, dk, dv, ddecay, dstate};
 }
@@ -162,14 +166,16 @@ Tensor attention_step(const Tensor &q, const Tensor &k, const Tensor &v, const T
 std::tuple<Tensor, Tensor> linear_attention_hip(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay,
                                                 const MaybeTensor &state, const MaybeTensor &lengths, double scale,
                                                 bool return_state) {
-    return attention_forward(q, k, v, log_decay, or_undefined(state), or_undefined(lengths), scale, return_state);
+    auto [out, last, kept] =
+        attention_forward(q, k, v, log_decay, or_undefined(state), or_undefined(lengths), scale, return_state, false);
+    return {out, last};
 }
 
 Gradients linear_attention_backward_hip(const Tensor &grad_out, const MaybeTensor &grad_state, const Tensor &q, const Tensor &k,
                                         const Tensor &v, const Tensor &log_decay, const MaybeTensor &state,
                                         const MaybeTensor &lengths, double scale, bool want_log_decay, bool want_state) {
     return attention_backward(grad_out, or_undefined(grad_state), q, k, v, log_decay, or_undefined(state), or_undefined(lengths),
-                              scale, want_log_decay, want_state);
+                              Tensor(), scale, want_log_decay, want_state);
 }
 
 bool any_grad(std::initializer_list<const Tensor *> all) {
@@ -199,14 +205,15 @@ struct AttentionFunction : public torch::autograd::Function<AttentionFunction<DI
                                  bool return_state) {
         at::AutoDispatchBelowADInplaceOrView below;
         const Tensor state = or_undefined(maybe_state), lengths = or_undefined(maybe_lengths);
-        Tensor out, last;
+        Tensor out, last, kept;
         if constexpr (DIRECT) {
-            std::tie(out, last) = attention_forward(q, k, v, log_decay, state, lengths, scale, return_state);
+            std::tie(out, last, kept) =
+                attention_forward(q, k, v, log_decay, state, lengths, scale, return_state, log_decay.requires_grad());
         } else {
             static auto op = typed_op<AttentionOp>("pathsig::linear_attention");
             std::tie(out, last) = op.call(q, k, v, log_decay, maybe_state, maybe_lengths, scale, return_state);
         }
-        ctx->save_for_backward({q, k, v, log_decay, state, lengths});
+        ctx->save_for_backward({q, k, v, log_decay, state, lengths, kept});
         ctx->saved_data["scale"] = scale;
         ctx->set_materialize_grads(false);
         if (!return_state) ctx->mark_non_differentiable({last});
@@ -216,17 +223,18 @@ struct AttentionFunction : public torch::autograd::Function<AttentionFunction<DI
         variable_list out(8);
         if (!grads[0].defined() && !grads[1].defined()) return out;
         const auto saved = ctx->get_saved_variables();
-        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &log_decay = saved[3], &state = saved[4], &lengths = saved[5];
+        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &log_decay = saved[3], &state = saved[4], &lengths = saved[5],
+                     &kept = saved[6];
         const double scale = ctx->saved_data["scale"].toDouble();
         Tensor grad_out = grads[0];
         if (!grad_out.defined()) grad_out = at::zeros({q.size(0), q.size(1), q.size(2), v.size(3)}, q.options());
         const bool want_decay = ctx->needs_input_grad(3), want_state = state.defined() && ctx->needs_input_grad(4);
         bool direct = DIRECT && !at::GradMode::is_enabled();
         for (const Tensor *t : {(const Tensor *)&grad_out, &q, &k, &v, &log_decay}) direct = direct && plain(*t);
-        for (const Tensor *t : {&state, &lengths, (const Tensor *)&grads[1]}) direct = direct && (!t->defined() || plain(*t));
+        for (const Tensor *t : {&state, &lengths, &kept, (const Tensor *)&grads[1]}) direct = direct && (!t->defined() || plain(*t));
         Gradients g;
         if (direct) {
-            g = attention_backward(grad_out, grads[1], q, k, v, log_decay, state, lengths, scale, want_decay, want_state);
+            g = attention_backward(grad_out, grads[1], q, k, v, log_decay, state, lengths, kept, scale, want_decay, want_state);
         } else {
             static auto op = typed_op<AttentionBackwardOp>("pathsig::linear_attention_backward");
             g = op.call(grad_out, or_none(grads[1]), q, k, v, log_decay, or_none(state), or_none(lengths), scale, want_decay,
@@ -490,7 +498,8 @@ PyObject *py_linear_attention(PyObject *, PyObject *const *args, Py_ssize_t narg
             last = both[1];
         } else {
             at::AutoDispatchBelowADInplaceOrView below;
-            std::tie(out, last) = attention_forward(t[0], t[1], t[2], t[3], t[4], t[5], scale, return_state);
+            Tensor kept;
+            std::tie(out, last, kept) = attention_forward(t[0], t[1], t[2], t[3], t[4], t[5], scale, return_state, false);
         }
     }
     if (!return_state) return THPVariable_Wrap(std::move(out));
