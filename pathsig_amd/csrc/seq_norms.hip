@@ -38,31 +38,49 @@ struct Deal {
     static __device__ __forceinline__ int column(int v, int t) { return (v * TPR + t) * E; }
 };
 
+// a thread's share of a row as it lies in memory
+template <typename T, int TPR, int EPT, int E>
+struct RawRow {
+    using D = Deal<TPR, EPT, E>;
+    Pack<T, E> p[D::kVectors];
+    __device__ __forceinline__ void load(const T *row, int t, int C) {
+#pragma unroll
+        for (int v = 0; v < D::kVectors; ++v) {
+            const int c = D::column(v, t);
+            p[v] = {};
+            if (c < C) p[v] = *(const Pack<T, E> *)(row + c);  // (C is a multiple of E)
+        }
+    }
+    __device__ __forceinline__ float at(int e) const { return to_float(p[e / E].v[e % E]); }
+    __device__ __forceinline__ void get(float (&out)[EPT]) const {
+#pragma unroll
+        for (int v = 0; v < D::kVectors; ++v)
+#pragma unroll
+            for (int e = 0; e < E; ++e) out[v * E + e] = to_float(p[v].v[e]);
+    }
+};
+
 template <typename T, int TPR, int EPT, int E>
 __device__ __forceinline__ void load_row(float (&out)[EPT], const T *row, int t, int C) {
-    using D = Deal<TPR, EPT, E>;
+    RawRow<T, TPR, EPT, E> raw;
+    raw.load(row, t, C);
+    raw.get(out);
+}
+
+template <typename T, int TPR, int E>
+__device__ __forceinline__ void store_vector(T *row, const float *x, int v, int t, int C) {
+    const int c = (v * TPR + t) * E;
+    if (c >= C) return;
+    Pack<T, E> p;
 #pragma unroll
-    for (int v = 0; v < D::kVectors; ++v) {
-        const int c = D::column(v, t);
-        Pack<T, E> p = {};
-        if (c < C) p = *(const Pack<T, E> *)(row + c);  // (C is a multiple of E)
-#pragma unroll
-        for (int e = 0; e < E; ++e) out[v * E + e] = to_float(p.v[e]);
-    }
+    for (int e = 0; e < E; ++e) p.v[e] = from_float<T>(x[e]);
+    *(Pack<T, E> *)(row + c) = p;
 }
 
 template <typename T, int TPR, int EPT, int E>
 __device__ __forceinline__ void store_row(T *row, const float (&x)[EPT], int t, int C) {
-    using D = Deal<TPR, EPT, E>;
 #pragma unroll
-    for (int v = 0; v < D::kVectors; ++v) {
-        const int c = D::column(v, t);
-        if (c >= C) continue;
-        Pack<T, E> p;
-#pragma unroll
-        for (int e = 0; e < E; ++e) p.v[e] = from_float<T>(x[v * E + e]);
-        *(Pack<T, E> *)(row + c) = p;
-    }
+    for (int v = 0; v < EPT / E; ++v) store_vector<T, TPR, E>(row, x + v * E, v, t, C);
 }
 
 // a parameter of the columns (NULL: `fill`), float32 or in the type of the rows
@@ -78,8 +96,8 @@ __device__ __forceinline__ void load_param(float (&out)[EPT], const void *p, int
     }
 }
 
-// sum over the TPR threads of a row; `slot` of LDS is only used when a row spans waves, and may be used again by the next call
-// after another one with the other `slot`
+// Sum over the TPR threads of a row.  Where a row spans waves, through `slot` of LDS, which may be written again after a barrier;
+// then every thread of the block has to come here.
 template <int TPR>
 __device__ __forceinline__ float row_sum(float x, float *slot) {
 #pragma unroll
@@ -95,7 +113,8 @@ __device__ __forceinline__ float row_sum(float x, float *slot) {
     return x;
 }
 
-__device__ __forceinline__ float logistic(float g) { return 1.f / (1.f + __expf(-g)); }
+// (the hardware's reciprocal, off by one unit in the last place at most; a division would take ten instructions)
+__device__ __forceinline__ float logistic(float g) { return __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
 
 __device__ __forceinline__ float gate_value(float g, int activation) {
     if (activation == PATHSIG_GATE_LINEAR) return g;
@@ -120,14 +139,17 @@ __device__ __forceinline__ void gate_both(float g, int activation, float &u, flo
     }
 }
 
+// rows of up to a wave's threads share a block of four waves, wider ones have one to themselves
+constexpr int threads_of(int threads_per_row) { return threads_per_row <= 64 ? 256 : threads_per_row; }
+
 template <typename T, int TPR, int EPT, int E>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_forward_kernel(const NormArgs a) {
-    constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
-    __shared__ float slots[2][8];
+__global__ __launch_bounds__(threads_of(TPR)) void norm_forward_kernel(const NormArgs a) {
+    constexpr int kRows = threads_of(TPR) / TPR;
+    __shared__ float slots[2][16];
     const int t = threadIdx.x % TPR;
-    const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
-    // (rows of several waves are whole blocks, so the threads that leave here leave no one waiting)
-    if (row >= a.rows) return;
+    const int64_t row_or_behind = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
+    const bool live = row_or_behind < a.rows;  // (all threads of a block meet at barriers)
+    const int64_t row = live ? row_or_behind : a.rows - 1;
     const int C = a.C;
     float x[EPT], w[EPT];
     load_row<T, TPR, EPT, E>(x, (const T *)a.x + row * a.x_stride, t, C);
@@ -153,8 +175,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_forward_kernel(con
 #pragma unroll
         for (int e = 0; e < EPT; ++e) x[e] += w[e];
     }
-    store_row<T, TPR, EPT, E>((T *)a.out + row * C, x, t, C);
-    if (a.stats && t == 0) a.stats[row] = r;
+    if (live) store_row<T, TPR, EPT, E>((T *)a.out + row * C, x, t, C);
+    if (live && a.stats && t == 0) a.stats[row] = r;
     if (!a.next) return;
     // (columns behind the last hold zeros: they were loaded as zeros, and gates and scales only multiply)
     sum = 0.f;
@@ -164,102 +186,117 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_forward_kernel(con
     load_param<T, TPR, EPT, E>(w, a.next_weight, a.float_params, t, C, 1.f);
 #pragma unroll
     for (int e = 0; e < EPT; ++e) x[e] = x[e] * r2 * w[e];
+    if (!live) return;
     store_row<T, TPR, EPT, E>((T *)a.next + row * C, x, t, C);
     if (a.stats && t == 0) a.stats[a.rows + row] = r2;
+}
+
+// Waves to a SIMD that the backward is compiled for and launched with: what its registers allow without spilling.  Rows that have a
+// block to themselves have their addresses in scalar registers.
+constexpr int backward_waves(int element, int threads_per_row) {
+    if (threads_per_row > 256) return 4;
+    return element == 4 && threads_per_row <= 64 ? 2 : 3;
 }
 
 // Blocks take rows in turn and hold the sums over their rows of the parameters' gradients in registers; norm_columns_kernel
 // adds the blocks in a fixed order.
 template <typename T, int TPR, int EPT, int E>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_kernel(const NormArgs a) {
-    constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
+__global__ __launch_bounds__(TPR > 256 ? 1024 : threads_of(TPR), backward_waves(sizeof(T), TPR)) void norm_backward_kernel(const NormArgs a) {
+    constexpr int kRows = threads_of(TPR) / TPR;
     using D = Deal<TPR, EPT, E>;
-    __shared__ float slots[2][8];
-    const int t = threadIdx.x % TPR;
+    __shared__ float slots[2][16];
+    const int t = kRows > 1 ? threadIdx.x % TPR : threadIdx.x;
     const int C = a.C;
     float sum_w[EPT] = {}, sum_s[EPT] = {}, sum_n[EPT] = {};
-    // the same number of turns for every thread: rows of several waves meet at barriers
-    for (int64_t first = (int64_t)blockIdx.x * kRows; first < a.rows; first += (int64_t)gridDim.x * kRows) {
-        const int64_t row = first + threadIdx.x / TPR;
-        if (row >= a.rows) break;
-        float unit[EPT], w[EPT], u[EPT], p[EPT], d[EPT];
-        load_row<T, TPR, EPT, E>(unit, (const T *)a.x + row * a.x_stride, t, C);
-        const float r = a.stats[row];
-        if (a.grad_out) {
-            load_row<T, TPR, EPT, E>(d, (const T *)a.grad_out + row * C, t, C);
-        } else {
-#pragma unroll
-            for (int e = 0; e < EPT; ++e) d[e] = 0.f;
+    // The tensors of a row are loaded while the row before is worked on.
+    RawRow<T, TPR, EPT, E> raw_x, raw_d, raw_u, raw_out, raw_n;
+    float raw_r = 0.f, raw_r2 = 0.f;
+    // (a row behind the last is one of zeros, which adds nothing)
+    auto fetch = [&](int64_t row) {
+        const bool live = row < a.rows;
+        const int have = live ? C : 0;
+        raw_x.load((const T *)a.x + row * a.x_stride, t, have);
+        raw_r = live ? a.stats[row] : 0.f;
+        if (a.grad_out) raw_d.load((const T *)a.grad_out + row * C, t, have);
+        if (a.gate) raw_u.load((const T *)a.gate + row * a.gate_stride, t, have);
+        if (a.grad_next) {
+            if (a.residual) raw_out.load((const T *)a.residual + row * a.residual_stride, t, have);
+            raw_n.load((const T *)a.grad_next + row * C, t, have);
+            raw_r2 = live ? a.stats[a.rows + row] : 0.f;
         }
-        load_param<T, TPR, EPT, E>(w, a.weight, a.float_params, t, C, 1.f);
-        load_param<T, TPR, EPT, E>(p, a.scale, a.float_params, t, C, 1.f);
-        if (a.gate) {
-            load_row<T, TPR, EPT, E>(u, (const T *)a.gate + row * a.gate_stride, t, C);
-        } else {
+    };
+    const int64_t step = (int64_t)gridDim.x * kRows;
+    const int own = kRows > 1 ? threadIdx.x / TPR : 0;
+    fetch((int64_t)blockIdx.x * kRows + own);
+    // as many turns for every thread of a block: they meet at barriers
+    for (int64_t first = (int64_t)blockIdx.x * kRows; first < a.rows; first += step) {
+        const int64_t row = first + own;
+        const bool live = row < a.rows;
+        RawRow<T, TPR, EPT, E> x = raw_x, d = raw_d, u = raw_u, residual = raw_out, n = raw_n;
+        const float r = raw_r, r2 = raw_r2;
+        if (first + step < a.rows) fetch(row + step);
+        // (read again for every row, from the cache: held, the parameters would take 24 registers)
+        const void *weight = a.weight, *scale = a.scale, *next_weight = a.next_weight;
+        asm volatile("" : "+s"(weight), "+s"(scale), "+s"(next_weight));
+        float unit[EPT], w[EPT], p[EPT], up[EPT];
+        load_param<T, TPR, EPT, E>(w, weight, a.float_params, t, C, 1.f);
+        load_param<T, TPR, EPT, E>(p, scale, a.float_params, t, C, 1.f);
 #pragma unroll
-            for (int e = 0; e < EPT; ++e) u[e] = 1.f;
+        for (int e = 0; e < EPT; ++e) {
+            unit[e] = x.at(e) * r;
+            up[e] = a.grad_out ? d.at(e) : 0.f;
         }
-#pragma unroll
-        for (int e = 0; e < EPT; ++e) unit[e] *= r;
         if (a.grad_next) {
             // out as the forward had it before rounding, from the same inputs
-            float out[EPT], n[EPT], nw[EPT];
-            if (a.residual) {
-                load_row<T, TPR, EPT, E>(out, (const T *)a.residual + row * a.residual_stride, t, C);
-            } else {
-#pragma unroll
-                for (int e = 0; e < EPT; ++e) out[e] = 0.f;
-            }
-            load_row<T, TPR, EPT, E>(n, (const T *)a.grad_next + row * C, t, C);
-            load_param<T, TPR, EPT, E>(nw, a.next_weight, a.float_params, t, C, 1.f);
-            const float r2 = a.stats[a.rows + row];
+            float unit2[EPT], dn[EPT], nw[EPT];
+            load_param<T, TPR, EPT, E>(nw, next_weight, a.float_params, t, C, 1.f);
             float dot = 0.f;
 #pragma unroll
             for (int e = 0; e < EPT; ++e) {
-                const float g = a.gate ? gate_value(u[e], a.activation) : 1.f;
-                out[e] = (out[e] + unit[e] * w[e] * g * p[e]) * r2;
-                sum_n[e] += n[e] * out[e];
-                n[e] *= nw[e];
-                dot += n[e] * out[e];
+                const float g = a.gate ? gate_value(u.at(e), a.activation) : 1.f;
+                unit2[e] = ((a.residual ? residual.at(e) : 0.f) + unit[e] * w[e] * g * p[e]) * r2;
+                dn[e] = n.at(e);
+                sum_n[e] += dn[e] * unit2[e];
+                dn[e] *= nw[e];
+                dot += dn[e] * unit2[e];
             }
             dot = row_sum<TPR>(dot, slots[0]) / (float)C;
 #pragma unroll
-            for (int e = 0; e < EPT; ++e) d[e] += r2 * (n[e] - out[e] * dot);
+            for (int e = 0; e < EPT; ++e) up[e] += r2 * (dn[e] - unit2[e] * dot);
         }
-        if (a.grad_residual) store_row<T, TPR, EPT, E>((T *)a.grad_residual + row * C, d, t, C);
+        if (live && a.grad_residual) store_row<T, TPR, EPT, E>((T *)a.grad_residual + row * C, up, t, C);
         if (a.gate) {
-            float dg[EPT];
+            float to_gate[EPT];
 #pragma unroll
             for (int e = 0; e < EPT; ++e) {
-                float g, du;
-                gate_both(u[e], a.activation, g, du);
+                float g, dg;
+                gate_both(u.at(e), a.activation, g, dg);
                 const float normed = unit[e] * w[e];
-                sum_s[e] += d[e] * normed * g;
-                d[e] *= p[e];
-                dg[e] = d[e] * normed * du;
-                d[e] *= g;
+                sum_s[e] += up[e] * normed * g;
+                up[e] *= p[e];
+                to_gate[e] = up[e] * normed * dg;
+                up[e] *= g;
             }
-            if (a.grad_gate) store_row<T, TPR, EPT, E>((T *)a.grad_gate + row * C, dg, t, C);
+            if (live && a.grad_gate) store_row<T, TPR, EPT, E>((T *)a.grad_gate + row * C, to_gate, t, C);
         } else {
 #pragma unroll
             for (int e = 0; e < EPT; ++e) {
-                sum_s[e] += d[e] * unit[e] * w[e];
-                d[e] *= p[e];
+                sum_s[e] += up[e] * unit[e] * w[e];
+                up[e] *= p[e];
             }
         }
         float dot = 0.f;
 #pragma unroll
         for (int e = 0; e < EPT; ++e) {
-            sum_w[e] += d[e] * unit[e];
-            d[e] *= w[e];
-            dot += d[e] * unit[e];
+            sum_w[e] += up[e] * unit[e];
+            up[e] *= w[e];
+            dot += up[e] * unit[e];
         }
-        // (the other slot than above: a wave that is ahead may write it while others still read the first; and between two
-        // writes of one slot lies a barrier of the other, or without a second norm this one's own)
+        // (the other slot than above: a wave that is ahead may write it while others still read the first)
         dot = row_sum<TPR>(dot, slots[1]) / (float)C;
 #pragma unroll
-        for (int e = 0; e < EPT; ++e) d[e] = r * (d[e] - unit[e] * dot);
-        if (a.grad_x) store_row<T, TPR, EPT, E>((T *)a.grad_x + row * C, d, t, C);
+        for (int e = 0; e < EPT; ++e) up[e] = r * (up[e] - unit[e] * dot);
+        if (live && a.grad_x) store_row<T, TPR, EPT, E>((T *)a.grad_x + row * C, up, t, C);
         if (TPR > 64) __syncthreads();  // before slots are written again
     }
     if (!a.partial) return;
@@ -327,26 +364,28 @@ struct RowShape {
     int threads_per_row, elements;
 };
 
-// The fewest threads that hold a row with eight elements each; sixteen only where the next larger group would be another wave
-// or more.
+// The fewest threads that hold a row with eight elements each, sixteen only for the widest rows.
 RowShape row_shape(int64_t C) {
-    static constexpr RowShape kShapes[] = {{8, 8}, {16, 8}, {64, 8}, {64, 16}, {256, 8}, {256, 16}, {512, 16}};
+    static constexpr RowShape kShapes[] = {{8, 8}, {16, 8}, {32, 8}, {64, 8}, {128, 8}, {256, 8}, {512, 8}, {1024, 8}};
     for (const RowShape &s : kShapes)
         if (C <= (int64_t)s.threads_per_row * s.elements) return s;
     return {0, 0};
 }
 
-int rows_per_block(const RowShape &s) { return s.threads_per_row < 256 ? 256 / s.threads_per_row : 1; }
+int rows_per_block(const RowShape &s) { return threads_of(s.threads_per_row) / s.threads_per_row; }
 
-int64_t backward_blocks(int64_t rows, int64_t C) {
+// Blocks of the backward: as many as the device holds at once.
+int64_t backward_blocks(int dtype, int64_t rows, int64_t C) {
     const RowShape s = row_shape(C);
+    const int threads = threads_of(s.threads_per_row);
     const int64_t groups = ceil_div(rows, rows_per_block(s));
-    return std::max<int64_t>(1, std::min<int64_t>(groups, 512));
+    const int waves = backward_waves(dtype == PATHSIG_F32 ? 4 : 2, s.threads_per_row);
+    return std::max<int64_t>(1, std::min<int64_t>(groups, 256 * (256 * waves / threads)));
 }
 
 template <typename T, int TPR, int EPT, int E>
 void launch(const NormArgs &a, bool backward, int64_t blocks, hipStream_t stream) {
-    constexpr int kThreads = TPR < 256 ? 256 : TPR;
+    constexpr int kThreads = threads_of(TPR);
     if (backward)
         norm_backward_kernel<T, TPR, EPT, E><<<dim3((unsigned)blocks), dim3(kThreads), 0, stream>>>(a);
     else
@@ -359,11 +398,12 @@ void dispatch(const NormArgs &a, bool backward, int64_t blocks, hipStream_t stre
     switch (s.threads_per_row * 100 + s.elements) {
         case 808: return launch<T, 8, 8, E>(a, backward, blocks, stream);
         case 1608: return launch<T, 16, 8, E>(a, backward, blocks, stream);
+        case 3208: return launch<T, 32, 8, E>(a, backward, blocks, stream);
         case 6408: return launch<T, 64, 8, E>(a, backward, blocks, stream);
-        case 6416: return launch<T, 64, 16, E>(a, backward, blocks, stream);
+        case 12808: return launch<T, 128, 8, E>(a, backward, blocks, stream);
         case 25608: return launch<T, 256, 8, E>(a, backward, blocks, stream);
-        case 25616: return launch<T, 256, 16, E>(a, backward, blocks, stream);
-        default: return launch<T, 512, 16, E>(a, backward, blocks, stream);
+        case 51208: return launch<T, 512, 8, E>(a, backward, blocks, stream);
+        default: return launch<T, 1024, 8, E>(a, backward, blocks, stream);
     }
 }
 
@@ -472,7 +512,7 @@ int pathsig_norm_forward(const pathsig_norm *call, void *out, void *next, float 
 
 size_t pathsig_norm_backward_workspace(const pathsig_norm *call) {
     if (check_norm(call) != PATHSIG_OK || call->rows == 0) return 0;
-    return (size_t)3 * backward_blocks(call->rows, call->C) * call->C * sizeof(float);
+    return (size_t)3 * backward_blocks(call->dtype, call->rows, call->C) * call->C * sizeof(float);
 }
 
 int pathsig_norm_backward(const pathsig_norm *call, const float *statistics, const void *grad_out, const void *grad_next,
@@ -494,7 +534,7 @@ int pathsig_norm_backward(const pathsig_norm *call, const float *statistics, con
         return PATHSIG_ERR_WORKSPACE;
     }
     NormArgs a = norm_args(call);
-    const int64_t blocks = call->rows > 0 ? backward_blocks(a.rows, a.C) : 0;
+    const int64_t blocks = call->rows > 0 ? backward_blocks(call->dtype, a.rows, a.C) : 0;
     if (call->rows > 0) {
         a.stats = const_cast<float *>(statistics);
         a.grad_out = grad_out;
