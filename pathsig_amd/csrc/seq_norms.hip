@@ -374,13 +374,14 @@ RowShape row_shape(int64_t C) {
 
 int rows_per_block(const RowShape &s) { return threads_of(s.threads_per_row) / s.threads_per_row; }
 
-// Blocks of the backward: as many as the device holds at once.
+// Blocks of the backward: as many as the device holds at once, and the rows dealt evenly to them.
 int64_t backward_blocks(int dtype, int64_t rows, int64_t C) {
     const RowShape s = row_shape(C);
     const int threads = threads_of(s.threads_per_row);
     const int64_t groups = ceil_div(rows, rows_per_block(s));
     const int waves = backward_waves(dtype == PATHSIG_F32 ? 4 : 2, s.threads_per_row);
-    return std::max<int64_t>(1, std::min<int64_t>(groups, 256 * (256 * waves / threads)));
+    const int64_t most = (int64_t)256 * (256 * waves / threads);
+    return ceil_div(groups, ceil_div(groups, most));
 }
 
 template <typename T, int TPR, int EPT, int E>
