@@ -19,8 +19,8 @@ namespace psig {
 namespace seq {
 namespace {
 
-// starts[s] holds what piece s - 1 adds; in place becomes the state in front of piece s.  Vectors of four elements along a row of
-// `starts` (V = 1 where the rows have no whole vectors), each with a thread of its own: bound by reading and writing `starts`.
+// starts[s] holds what piece s - 1 adds; in place becomes the state in front of piece s.  Vectors of V elements with a thread each:
+// bound by reading and writing `starts`.
 template <int V>
 __global__ __launch_bounds__(256) void join_kernel(const Sweep a) {
     using P = Pack<float, V>;
@@ -31,11 +31,11 @@ __global__ __launch_bounds__(256) void join_kernel(const Sweep a) {
     const int64_t b = blockIdx.z, head = (b * a.H + h) * plane, stride = a.B * a.H * plane;
     const int64_t n = length_of(a.lengths, b, a.L);
     const float g2 = decay_of(a.log_decay, h) * kLog2e;
-    float *const p = a.starts.p + head + i;
+    float *const p = a.starts + head + i;
     P x = {};
-    if (a.first.p) {
+    if (a.first) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) x.v[e] = a.first.p[head + (i + e) / a.Dv * a.first.row + (i + e) % a.Dv * a.first.column];
+        for (int e = 0; e < V; ++e) x.v[e] = a.first[head + i + e];
     }
     *(P *)p = x;
 #pragma unroll 8
@@ -178,20 +178,22 @@ View dense(const void *p, int64_t L, int64_t H, int64_t D, int element) {
     return view(p, stride, 1, element);
 }
 
-// Pieces of a call's sweeps, the same for all of them: as many as bring the blocks to two for each of the 256 compute units, of whole
-// chunks, and not below 256 tokens, where what a piece costs (its state written and read, 4 Dk Dv bytes each) would be half of
-// what its tokens do.
-void cut(const pathsig_linattn *c, int64_t *piece, int *pieces) {
-    const int64_t blocks = c->B * c->H;
-    const int64_t want = std::max<int64_t>(1, std::min(512 / std::max<int64_t>(blocks, 1), c->L / 256));
-    *piece = std::max<int64_t>(ceil_div(ceil_div(c->L, want), 64) * 64, 64);
-    *pieces = (int)std::max<int64_t>(ceil_div(c->L, *piece), 1);
+// Pieces of a call's sweeps, the same for all of them: as many as bring the blocks to two for each of the 256 compute units, of
+// whole chunks, and not below 256 tokens, where what a piece costs (its state written and read, 4 Dk Dv bytes each) would be half of
+// what its tokens do.  Two pieces are folded in halves, or every second unit would have no block to fold with.
+void cut(const pathsig_linattn *c, int64_t *piece, int *pieces, int *run) {
+    const int64_t blocks = std::max<int64_t>(c->B * c->H, 1);
+    const int64_t want = std::max<int64_t>(1, std::min(512 / blocks, c->L / 256));
+    *run = want == 2 && c->L >= 1024 ? 2 : 1;
+    const int64_t count = want * *run;
+    *piece = std::max<int64_t>(ceil_div(ceil_div(c->L, count), 64) * 64, 64);
+    *pieces = (int)(*run * std::max<int64_t>(ceil_div(c->L, *piece * *run), 1));
 }
 
 size_t starts_bytes(const pathsig_linattn *c) {
     int64_t piece;
-    int pieces;
-    cut(c, &piece, &pieces);
+    int pieces, run;
+    cut(c, &piece, &pieces, &run);
     return pieces > 1 ? (size_t)pieces * c->B * c->H * c->Dk * c->Dv * sizeof(float) : 0;
 }
 
@@ -206,7 +208,9 @@ Sweep sweep_of(const pathsig_linattn *c) {
     a.Dv = (int)c->Dv;
     a.in_scale = 1.f;
     a.out_scale = 1.f;
-    cut(c, &a.piece, &a.pieces);
+    a.row = c->Dv;
+    a.column = 1;
+    cut(c, &a.piece, &a.pieces, &a.run);
     return a;
 }
 
@@ -221,7 +225,7 @@ void chunks(const Sweep &a, bool fold, hipStream_t stream) {
 // the states in front of the pieces
 template <typename T>
 void fold(Sweep &a, float *starts, hipStream_t stream) {
-    a.starts = {starts, a.Dv, 1};
+    a.starts = starts;
     if (a.pieces == 1) return;
     chunks<T>(a, true, stream);
     if (a.pieces <= kJoinInside) return;
@@ -248,8 +252,8 @@ int forward_t(const pathsig_linattn *c, const void *q, const void *k, const void
     a.q = view(q, c->q_stride, 1, sizeof(T));
     a.k = view(k, c->k_stride, group, sizeof(T));
     a.v = view(v, c->v_stride, group, sizeof(T));
-    a.first = {const_cast<float *>(state), c->Dv, 1};
-    a.last = {final_state, c->Dv, 1};
+    a.first = state;
+    a.last = final_state;
     a.out = out;
     a.out_scale = c->scale;
     a.exact_state = final_state || c->learned_decay;
@@ -270,9 +274,9 @@ size_t place(size_t &total, size_t bytes) {
 
 int64_t decay_partials(const pathsig_linattn *c) {
     int64_t piece;
-    int pieces;
-    cut(c, &piece, &pieces);
-    return pieces * ceil_div(c->Dv, 128) * c->B;
+    int pieces, run;
+    cut(c, &piece, &pieces, &run);
+    return pieces / run * ceil_div(c->Dv, 128) * c->B;
 }
 
 BackwardLayout backward_layout(const pathsig_linattn *c, bool want_decay) {
@@ -301,11 +305,11 @@ int backward_t(const pathsig_linattn *c, const void *q, const void *k, const voi
     forward.q = vq;
     forward.k = vk;
     forward.v = vv;
-    forward.first = {const_cast<float *>(state), c->Dv, 1};
+    forward.first = state;
     forward.out_scale = c->scale;
     forward.exact_state = grad_decay != nullptr;
     if (kept)
-        forward.starts = {const_cast<float *>(kept), c->Dv, 1};
+        forward.starts = const_cast<float *>(kept);
     else
         fold<T>(forward, (float *)(ws + l.starts), stream);
     // dq: the forward with (do, v, k) and the transposed states
@@ -314,8 +318,7 @@ int backward_t(const pathsig_linattn *c, const void *q, const void *k, const voi
     a.q = vdo;
     a.k = vv;
     a.v = vk;
-    a.first = {forward.first.p, 1, c->Dv};
-    a.starts = {forward.starts.p, 1, c->Dv};
+    std::swap(a.row, a.column);
     a.out = grad_q;
     a.exact_state = 0;
     chunks<T>(a, false, stream);
@@ -324,8 +327,8 @@ int backward_t(const pathsig_linattn *c, const void *q, const void *k, const voi
     back.q = vk;
     back.k = vq;
     back.v = vdo;
-    back.first = {const_cast<float *>(grad_final), c->Dv, 1};
-    back.last = {grad_state, c->Dv, 1};
+    back.first = grad_final;
+    back.last = grad_state;
     back.in_scale = c->scale;
     back.reverse = 1;
     back.out_float = group > 1;
@@ -340,9 +343,8 @@ int backward_t(const pathsig_linattn *c, const void *q, const void *k, const voi
     a.q = vv;
     a.k = vdo;
     a.v = vq;
-    a.first = {back.first.p, 1, c->Dv};
-    a.starts = {back.starts.p, 1, c->Dv};
-    a.last = {nullptr, 0, 0};
+    std::swap(a.row, a.column);
+    a.last = nullptr;
     a.out = group > 1 ? (void *)(ws + l.wide_k) : grad_k;
     a.exact_state = 0;
     chunks<T>(a, false, stream);

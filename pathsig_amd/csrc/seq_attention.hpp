@@ -15,11 +15,6 @@ struct View {
     int vectors;  // rows start at multiples of 16 bytes
 };
 
-struct StateRef {
-    float *p;  // [B, H, Dk * Dv]; element (a, c) of a head at a * row + c * column
-    int64_t row, column;
-};
-
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // One pass of the recurrence over all tokens, S <- decay S + in_scale k v^T, out = out_scale S^T q, or backwards in time, where
@@ -27,7 +22,11 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // columns of this pass' state, whichever tensors are in the places of k and v.
 struct Sweep {
     View q, k, v;
-    StateRef first, last;  // p may be NULL
+    // [B, H, Dk * Dv], each may be NULL: the state in front of the first token, whose element (a, c) lies at a * row + c * column
+    // of a head's (as in `starts`), and the one behind the last, row by row
+    const float *first;
+    float *last;
+    int64_t row, column;
     void *out;             // [B, L, H, Dv] dense
     int out_float;         // float32 instead of the type of q
     const float *log_decay;
@@ -38,10 +37,11 @@ struct Sweep {
     int reverse;
     int exact_state;       // the state is wanted in 32 bits, not only the answers
     // the sequence in pieces of `piece` tokens: starts [pieces][B][H][Dk * Dv], whose s-th entry is the state in front of piece s
-    // or, with few pieces (kJoinInside), what piece s - 1 adds to a state of zero
+    // or, with few pieces (kJoinInside), what piece s - 1 adds to a state of zero.  A block of the sweep takes `run` of them, one
+    // after the other.
     int64_t piece;
-    int pieces;
-    StateRef starts;
+    int pieces, run;
+    float *starts;
 };
 
 // Up to so many pieces, every block adds up the pieces before its own by itself: at most 1.5 states read for each block instead of
@@ -59,14 +59,15 @@ __device__ __forceinline__ float decay_of(const float *log_decay, int h) {
     return fmaxf(log_decay[h], -1e30f);
 }
 
-// Tokens [begin, end) of a piece in the order of the sweep.  Pieces are cut at the same tokens in both directions of time: the
-// s-th of a sweep backwards in time is the one s from the last, and empty where the sequence ends before it.
+// Tokens [begin, end) of `count` pieces from the s-th on, in the order of the sweep.  Pieces are cut at the same tokens in both
+// directions of time: the s-th of a sweep backwards in time is the one s from the last, and empty where the sequence ends
+// before it.
 struct Range {
     int64_t begin, end;
 };
-__device__ __forceinline__ Range range_of(const Sweep &a, int64_t n, int s) {
-    const int64_t p = a.reverse ? a.pieces - 1 - s : s;
-    const int64_t t0 = min(p * a.piece, n), t1 = min((p + 1) * a.piece, n);
+__device__ __forceinline__ Range range_of(const Sweep &a, int64_t n, int s, int count = 1) {
+    const int64_t p = a.reverse ? a.pieces - s - count : s;
+    const int64_t t0 = min(p * a.piece, n), t1 = min((p + count) * a.piece, n);
     return a.reverse ? Range{n - t1, n - t0} : Range{t0, t1};
 }
 

@@ -227,26 +227,53 @@ constexpr int chunk_tiles(int DKT, int NW) {
 }
 
 // The state in front of a piece (FOLD: zero): this lane's column dv, rows in accumulator order.
-template <int DKT, bool FOLD>
-__device__ __forceinline__ void load_state(f32x16 (&S)[DKT], const Sweep &a, int64_t b, int h, int64_t n, int piece, float g2, int dv,
-                                           int half) {
+template <int DKT, int NW, bool FOLD>
+__device__ __forceinline__ void load_state(f32x16 (&S)[DKT], const Sweep &a, int64_t b, int h, int64_t n, int piece, float g2, int dv0,
+                                           int dv, int half) {
     const int64_t plane = (int64_t)a.Dk * a.Dv, head = (b * a.H + h) * plane, between = a.B * a.H * plane;
 #pragma unroll
     for (int t = 0; t < DKT; ++t) S[t] = f32x16{};
     if (FOLD) return;
-    auto add = [&](const float *p, int64_t row, int64_t column, float f) {
-        p += dv * column + 4 * half * row;
+    const bool joined = a.pieces > kJoinInside, whole = a.Dk == 32 * DKT && dv0 + 32 * NW <= a.Dv;
+    const int row = (int)a.row, column = (int)a.column;
+    // one base for all lanes and 32-bit offsets; rows and columns behind the last are zeros, their addresses are kept inside
+    const uint32_t offset = whole ? dv * column + 4 * half * row : min(dv, a.Dv - 1) * column;
+    // the state in front of the first token (s = -1) and what the pieces up to this one add, or all of that at once
+    for (int s = joined ? piece - 1 : a.first ? -1 : 0; s < piece; ++s) {
+        const float *const p = (s < 0 && !joined ? a.first : a.starts + (s + 1) * between) + head;
+        float f = 0.f;
+        if (s >= 0 && !joined) {
+            const Range r = range_of(a, n, s);
+            f = exp2f(g2 * (float)(r.end - r.begin));
+        }
+        f32x16 x[DKT];  // (all loads are on their way before the first is waited for)
+        if (whole && row == 1) {
 #pragma unroll
-        for (int t = 0; t < DKT; ++t)
+            for (int t = 0; t < DKT; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                S[t][r] = S[t][r] * f + (32 * t + acc_row(r, half) < a.Dk && dv < a.Dv ? p[(32 * t + acc_row(r, 0)) * row] : 0.f);
-    };
-    if (a.pieces > kJoinInside) return add(a.starts.p + piece * between + head, a.starts.row, a.starts.column, 0.f);
-    if (a.first.p) add(a.first.p + head, a.first.row, a.first.column, 0.f);
-    for (int s = 0; s < piece; ++s) {
-        const Range r = range_of(a, n, s);
-        add(a.starts.p + (s + 1) * between + head, a.starts.row, a.starts.column, exp2f(g2 * (float)(r.end - r.begin)));
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    float four[4];
+                    __builtin_memcpy(four, p + 32 * t + 8 * r4 + offset, 16);  // (a state may start at any float)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[t][4 * r4 + e] = four[e];
+                }
+        } else if (whole) {
+#pragma unroll
+            for (int t = 0; t < DKT; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[t][r] = (p + (32 * t + acc_row(r, 0)) * row)[offset];
+        } else {
+#pragma unroll
+            for (int t = 0; t < DKT; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int dk = 32 * t + acc_row(r, half);
+                    const float y = p[offset + (uint32_t)(min(dk, a.Dk - 1) * row)];
+                    x[t][r] = dk < a.Dk && dv < a.Dv ? y : 0.f;
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < DKT; ++t) S[t] = S[t] * f + x[t];
     }
 }
 
@@ -269,27 +296,27 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
     char *const lds_k = lds, *const lds_v = lds + kKBytes, *const lds_q = lds_v + kVBytes;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, ln = lane & 31;
-    const int slice = blockIdx.x % slices, h = blockIdx.x / slices, piece = blockIdx.y;
+    const int slice = blockIdx.x % slices, h = blockIdx.x / slices, run = FOLD ? 1 : a.run, piece = blockIdx.y * run;
     const int64_t b = blockIdx.z;
     const int dv0 = slice * DV, dv = dv0 + 32 * wave + ln;  // this lane's column of the state
     const int64_t n = length_of(a.lengths, b, a.L);
-    const auto [begin, end] = range_of(a, n, piece);
+    const auto [begin, end] = range_of(a, n, piece, run);
     const float g2 = decay_of(a.log_decay, h) * kLog2e;
     const int64_t plane = (int64_t)a.Dk * a.Dv, head = (b * a.H + h) * plane;
 
     if (!FOLD) {
         // tokens behind the end of the sequence
-        const int64_t p = a.reverse ? a.pieces - 1 - piece : piece;
-        const int64_t z0 = max(n, p * a.piece), z1 = min((p + 1) * a.piece, a.L);
+        const int64_t p = a.reverse ? a.pieces - piece - run : piece;
+        const int64_t z0 = max(n, p * a.piece), z1 = min((p + run) * a.piece, a.L);
         const int width = min(DV, a.Dv - dv0);
         for (int64_t t = z0 + wave; t < z1; t += NW)
             for (int c = lane; c < width; c += 64) ((O *)a.out)[((b * a.L + t) * a.H + h) * a.Dv + dv0 + c] = from_float<O>(0.f);
     }
-    const bool owns_end = !FOLD && a.last.p && end == n && (begin < n || (n == 0 && piece == 0));
+    const bool owns_end = !FOLD && a.last && end == n && (begin < n || (n == 0 && piece == 0));
     if (begin >= end && !owns_end && !FOLD) return;
 
     f32x16 S[DKT];
-    load_state<DKT, FOLD>(S, a, b, h, n, piece, g2, dv, half);
+    load_state<DKT, NW, FOLD>(S, a, b, h, n, piece, g2, dv0, dv, half);
 
     // Factors of a lane's registers, in LDS (they would fill the registers, and are read once a chunk): l^(C - 1 - j) for the state's
     // update; for scores l^(31 - j), which l^(i + 1) completes in the tile off the diagonal, and l^(i - j) in those on it (j after i
@@ -483,25 +510,15 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
         }
     }
 
-    float *to = nullptr;
-    int64_t row = 0, column = 0;
-    if (FOLD) {
-        to = a.starts.p + (int64_t)(piece + 1) * a.B * a.H * plane + head;
-        row = a.starts.row;
-        column = a.starts.column;
-    } else if (owns_end) {
-        to = a.last.p + head;
-        row = a.last.row;
-        column = a.last.column;
-    }
+    float *to = FOLD ? a.starts + (int64_t)(piece + 1) * a.B * a.H * plane : owns_end ? a.last : nullptr;
     if (!to) return;
+    to += head;
+    const uint32_t offset = dv + 4 * half * a.Dv;
 #pragma unroll
     for (int t = 0; t < DKT; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int dk = 32 * t + acc_row(r, half);
-            if (dk < a.Dk && dv < a.Dv) to[dk * row + dv * column] = S[t][r];
-        }
+        for (int r = 0; r < 16; ++r)
+            if (32 * t + acc_row(r, half) < a.Dk && dv < a.Dv) (to + (32 * t + acc_row(r, 0)) * a.Dv)[offset] = S[t][r];
 }
 
 // dL/dg of a piece.  With S the state of a head and D = dS/dg (zero in front of the piece, whose own S is given):
@@ -528,19 +545,19 @@ __global__ __launch_bounds__(64 * NW, 1) void decay_kernel(const Sweep a, const 
     using VTile = Tile<T, DV>;
     constexpr int kKBytes = C * KTile::kRow, kVBytes = C * VTile::kRow;
     __shared__ __align__(16) char lds[2 * kKBytes + 2 * kVBytes];
-    __shared__ float meet[NW];
+    __shared__ double meet[NW];
     char *const lds_k = lds, *const lds_q = lds + kKBytes, *const lds_v = lds_q + kKBytes, *const lds_o = lds_v + kVBytes;
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, ln = lane & 31;
-    const int slice = blockIdx.x % slices, h = blockIdx.x / slices, piece = blockIdx.y;
+    const int slice = blockIdx.x % slices, h = blockIdx.x / slices, piece = blockIdx.y * a.run;
     const int64_t b = blockIdx.z;
     const int dv0 = slice * DV, dv = dv0 + 32 * wave + ln;
     const int64_t n = length_of(a.lengths, b, a.L);
-    const auto [begin, end] = range_of(a, n, piece);
+    const auto [begin, end] = range_of(a, n, piece, a.run);
     const float g2 = decay_of(a.log_decay, h) * kLog2e;
 
     f32x16 S[DKT], D[DKT];
-    load_state<DKT, false>(S, a, b, h, n, piece, g2, dv, half);
+    load_state<DKT, NW, false>(S, a, b, h, n, piece, g2, dv0, dv, half);
 #pragma unroll
     for (int t = 0; t < DKT; ++t) D[t] = f32x16{};
     const T *const kp = (const T *)a.k.p + b * a.k.sb + (h / a.k.group) * a.k.sh;
@@ -553,7 +570,7 @@ __global__ __launch_bounds__(64 * NW, 1) void decay_kernel(const Sweep a, const 
     int k_bases_of_lane[KTile::kColumnBases], v_bases_of_lane[VTile::kColumnBases];
     KTile::column_bases(k_bases_of_lane, lane);
     VTile::column_bases(v_bases_of_lane, lane);
-    float total = 0.f;
+    double total = 0;  // of chunks; terms of a chunk are added in 32 bits
     for (int c = 0; c < chunks; ++c, r0 += C) {
         const int pad = (int)max(begin - r0, (int64_t)0);
         __syncthreads();
@@ -581,6 +598,7 @@ __global__ __launch_bounds__(64 * NW, 1) void decay_kernel(const Sweep a, const 
         }
         v_row_base ^= wave * 32 * (int)sizeof(T);
 
+        float chunk = 0.f;
         // inside the chunk; this wave's channels of do . v
 #pragma unroll
         for (int i = 0; i < CT; ++i)
@@ -599,7 +617,7 @@ __global__ __launch_bounds__(64 * NW, 1) void decay_kernel(const Sweep a, const 
                 for (int r = 0; r < 16; ++r) {
                     const int gap = 32 * (i - j) + ln - acc_row(r, half);
                     const float f = (float)gap * exp2f(g2 * (float)max(gap, 0));
-                    if (gap > 0) total += f * (scores[r] * pulls[r]);
+                    if (gap > 0) chunk += f * (scores[r] * pulls[r]);
                 }
             }
 
@@ -628,8 +646,9 @@ __global__ __launch_bounds__(64 * NW, 1) void decay_kernel(const Sweep a, const 
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            total += sum16(D[t] * G + S[t] * G1);
+            chunk += sum16(D[t] * G + S[t] * G1);
         }
+        total += chunk;
 
         const float count = (float)(C - pad), whole = exp2f(g2 * count);
 #pragma unroll
@@ -664,7 +683,7 @@ __global__ __launch_bounds__(64 * NW, 1) void decay_kernel(const Sweep a, const 
     }
     total *= a.out_scale;
     // the gradient of the state behind the piece
-    load_state<DKT, false>(S, back, b, h, n, a.pieces - 1 - piece, g2, dv, half);
+    load_state<DKT, NW, false>(S, back, b, h, n, a.pieces - piece - a.run, g2, dv0, dv, half);
 #pragma unroll
     for (int t = 0; t < DKT; ++t) total += sum16(D[t] * S[t]);
 #pragma unroll
@@ -673,7 +692,7 @@ __global__ __launch_bounds__(64 * NW, 1) void decay_kernel(const Sweep a, const 
     __syncthreads();
     if (threadIdx.x > 0) return;
     for (int w = 1; w < NW; ++w) total += meet[w];
-    partial[(((int64_t)piece * slices + slice) * a.B + b) * a.H + h] = total;
+    partial[(((int64_t)blockIdx.y * slices + slice) * a.B + b) * a.H + h] = (float)total;
 }
 
 // Whole units of 16 bytes everywhere: all rows start at addresses of units, and heads have whole units of channels (a head that
@@ -686,7 +705,7 @@ bool whole_units(const Sweep &a, int element, bool more = true) {
 template <typename T, int DKT, int NW, int TERMS, bool VECTORS>
 void launch_width(const Sweep &a, bool fold, hipStream_t stream) {
     const int slices = (int)ceil_div(a.Dv, 32 * NW);
-    const dim3 grid((unsigned)(slices * a.H), (unsigned)(fold ? a.pieces - 1 : a.pieces), (unsigned)a.B), block(64 * NW);
+    const dim3 grid((unsigned)(slices * a.H), (unsigned)(fold ? a.pieces - a.run : a.pieces / a.run), (unsigned)a.B), block(64 * NW);
     if (fold)
         chunk_kernel<T, T, DKT, NW, TERMS, true, VECTORS><<<grid, block, 0, stream>>>(a, slices);
     else if (a.out_float && sizeof(T) == 2)
@@ -713,7 +732,7 @@ void launch_aligned(const Sweep &a, bool fold, hipStream_t stream) {
 template <typename T, int DKT, int NW>
 void launch_decay_width(const Sweep &a, const Sweep &back, const View &grad, float *partial, hipStream_t stream) {
     const int slices = (int)ceil_div(a.Dv, 32 * NW);
-    const dim3 grid((unsigned)(slices * a.H), (unsigned)a.pieces, (unsigned)a.B), block(64 * NW);
+    const dim3 grid((unsigned)(slices * a.H), (unsigned)(a.pieces / a.run), (unsigned)a.B), block(64 * NW);
     if (whole_units(a, sizeof(T), grad.vectors))
         decay_kernel<T, DKT, NW, true><<<grid, block, 0, stream>>>(a, back, grad, partial, slices);
     else
