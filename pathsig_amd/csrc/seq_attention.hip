@@ -38,14 +38,21 @@ __global__ __launch_bounds__(256) void join_kernel(const Sweep a) {
         for (int e = 0; e < V; ++e) x.v[e] = a.first[head + i + e];
     }
     *(P *)p = x;
-#pragma unroll 8
-    for (int s = 1; s < a.pieces; ++s) {
-        const Range before = range_of(a, n, s - 1);
-        const float f = exp2f(g2 * (float)(before.end - before.begin));
-        P add = *(const P *)(p + s * stride);
+    constexpr int kBatch = 16;  // loads on their way at once (stores of one and loads of the next may meet, for all the compiler knows)
+    for (int s0 = 1; s0 < a.pieces; s0 += kBatch) {
+        P add[kBatch];
 #pragma unroll
-        for (int e = 0; e < V; ++e) x.v[e] = x.v[e] * f + add.v[e];
-        *(P *)(p + s * stride) = x;
+        for (int j = 0; j < kBatch; ++j)
+            if (s0 + j < a.pieces) add[j] = *(const P *)(p + (s0 + j) * stride);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            if (s0 + j >= a.pieces) break;
+            const Range before = range_of(a, n, s0 + j - 1);
+            const float f = exp2f(g2 * (float)(before.end - before.begin));
+#pragma unroll
+            for (int e = 0; e < V; ++e) x.v[e] = x.v[e] * f + add[j].v[e];
+            *(P *)(p + (s0 + j) * stride) = x;
+        }
     }
 }
 
@@ -178,13 +185,16 @@ View dense(const void *p, int64_t L, int64_t H, int64_t D, int element) {
     return view(p, stride, 1, element);
 }
 
-// Pieces of a call's sweeps, the same for all of them: as many as bring the blocks to two for each of the 256 compute units, of
-// whole chunks, and not below 256 tokens, where what a piece costs (its state written and read, 4 Dk Dv bytes each) would be half of
-// what its tokens do.  Two pieces are folded in halves, or every second unit would have no block to fold with.
+// Pieces of a call's sweeps, the same for all of them: as many as bring two waves to each of the 1024 SIMDs (a block has a wave for
+// 32 columns of the state, up to four), of whole chunks, and not so short that what a piece costs (its state written and read,
+// 8 Dk Dv bytes) is more than what its tokens do.  Two pieces of blocks of four waves are folded in halves, or every second compute
+// unit would have no block to fold with.
 void cut(const pathsig_linattn *c, int64_t *piece, int *pieces, int *run) {
-    const int64_t blocks = std::max<int64_t>(c->B * c->H, 1);
-    const int64_t want = std::max<int64_t>(1, std::min(512 / blocks, c->L / 256));
-    *run = want == 2 && c->L >= 1024 ? 2 : 1;
+    const int64_t wide = std::max(c->Dk, c->Dv), waves = wide <= 32 ? 1 : wide <= 64 ? 2 : 4;
+    const int64_t blocks = std::max<int64_t>(c->B * c->H, 1), element = c->dtype == PATHSIG_F32 ? 4 : 2;
+    const int64_t least = std::max<int64_t>(64, 8 * c->Dk * c->Dv / (element * (c->Dk + c->Dv)));
+    const int64_t want = std::max<int64_t>(1, std::min(2048 / waves / blocks, c->L / least));
+    *run = want == 2 && waves == 4 && c->L >= 4 * least ? 2 : 1;
     const int64_t count = want * *run;
     *piece = std::max<int64_t>(ceil_div(ceil_div(c->L, count), 64) * 64, 64);
     *pieces = (int)(*run * std::max<int64_t>(ceil_div(c->L, *piece * *run), 1));

@@ -528,7 +528,7 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
 //     D' = l^C (D + C S) + sum of (C - 1 - j) l^(C-1-j) k_j v_j^T.
 // Every term is a sum of like signs or of independent ones; sum over t of t (q_t . dq_t - k_t . dk_t), which needs no states,
 // cancels by the length of the sequence over the memory of the head.  Products of states stay in 32 bits (element by element on
-// accumulators); what enters them is split into two bf16 terms (relative 2^-18 a term).
+// accumulators); what enters them is split into three bf16 terms.
 __device__ __forceinline__ float sum16(f32x16 x) {
     float s = 0.f;
 #pragma unroll
@@ -537,15 +537,21 @@ __device__ __forceinline__ float sum16(f32x16 x) {
 }
 
 template <typename T, int DKT, int NW, bool VECTORS>
-__global__ __launch_bounds__(64 * NW, 1) void decay_kernel(const Sweep a, const Sweep back, const View grad, float *partial,
+__global__ __launch_bounds__(64 * NW, DKT == 1 ? 2 : 1) void decay_kernel(const Sweep a, const Sweep back, const View grad, float *partial,
                                                          int slices) {
-    constexpr int DK = 32 * DKT, DV = 32 * NW, THREADS = 64 * NW, TERMS = sizeof(T) == 2 ? 2 : 1;
+    constexpr int DK = 32 * DKT, DV = 32 * NW, THREADS = 64 * NW, TERMS = sizeof(T) == 2 ? 3 : 1;
     constexpr int CT = chunk_tiles<T>(DKT, NW), C = 32 * CT;
+    // fetched a chunk ahead in bf16 (4 x 8192 tokens, 8 heads of 64 x 128: 153 -> 141 us); in fp32, whose chunks are half as long, the
+    // registers it takes cost the second block on a compute unit (50 x 333, 6 heads of 40 x 56: 88 -> 115)
+    constexpr bool kAhead = sizeof(T) == 2 && fetched(2, CT, DKT, NW) + C * DV * 2 / THREADS <= 256;
     using KTile = Tile<T, DK>;
     using VTile = Tile<T, DV>;
     constexpr int kKBytes = C * KTile::kRow, kVBytes = C * VTile::kRow;
     __shared__ __align__(16) char lds[2 * kKBytes + 2 * kVBytes];
     __shared__ double meet[NW];
+    // Factors by token of a chunk: l^(i+1) and l^(C-1-j), and by lane and register gap l^gap in tiles on the diagonal and off it
+    // (accumulator order, zero where j is not before i)
+    __shared__ __align__(16) f32x4 table_since[C / 4], table_left[C / 4], table_gap[CT][4][64];
     char *const lds_k = lds, *const lds_q = lds + kKBytes, *const lds_v = lds_q + kKBytes, *const lds_o = lds_v + kVBytes;
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, ln = lane & 31;
@@ -570,23 +576,54 @@ __global__ __launch_bounds__(64 * NW, 1) void decay_kernel(const Sweep a, const 
     int k_bases_of_lane[KTile::kColumnBases], v_bases_of_lane[VTile::kColumnBases];
     KTile::column_bases(k_bases_of_lane, lane);
     VTile::column_bases(v_bases_of_lane, lane);
+    if (threadIdx.x < C) table_left[threadIdx.x / 4][threadIdx.x % 4] = exp2f(g2 * (float)(C - 1 - (int)threadIdx.x));
+    if (wave < CT) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int gap = 32 * wave + ln - acc_row(r, half);
+            table_gap[wave][r / 4][lane][r % 4] = gap > 0 ? (float)gap * exp2f(g2 * (float)gap) : 0.f;
+        }
+    }
+    if (NW == 1 && CT == 2) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int gap = 32 + ln - acc_row(r, half);
+            table_gap[CT - 1][r / 4][lane][r % 4] = (float)gap * exp2f(g2 * (float)gap);
+        }
+    }
+    Fetch<T, DK, C, THREADS> fk, fq;
+    Fetch<T, DV, C, THREADS> fv, fo;
+    // (where registers do not hold a whole chunk, the tensors pass through them one after the other)
+    auto fetch = [&](int64_t at, int pad) {
+        fk.template load<VECTORS>(kp + at * a.k.st, (int)a.k.st, a.Dk, pad);
+        if (!kAhead) fk.store(lds_k);
+        fq.template load<VECTORS>(qp + at * a.q.st, (int)a.q.st, a.Dk, pad);
+        if (!kAhead) fq.store(lds_q);
+        fv.template load<VECTORS>(vp + at * a.v.st, (int)a.v.st, a.Dv - dv0, pad);
+        if (!kAhead) fv.store(lds_v);
+        fo.template load<VECTORS>(op + at * grad.st, (int)grad.st, a.Dv - dv0, pad);
+        if (!kAhead) fo.store(lds_o);
+    };
+    auto store = [&]() {
+        fk.store(lds_k);
+        fq.store(lds_q);
+        fv.store(lds_v);
+        fo.store(lds_o);
+    };
+    if (kAhead && chunks > 0) fetch(r0, (int)(begin - r0));
     double total = 0;  // of chunks; terms of a chunk are added in 32 bits
     for (int c = 0; c < chunks; ++c, r0 += C) {
         const int pad = (int)max(begin - r0, (int64_t)0);
         __syncthreads();
-        {
-            Fetch<T, DK, C, THREADS> x;
-            x.template load<VECTORS>(kp + r0 * a.k.st, (int)a.k.st, a.Dk, pad);
-            x.store(lds_k);
-            x.template load<VECTORS>(qp + r0 * a.q.st, (int)a.q.st, a.Dk, pad);
-            x.store(lds_q);
-            Fetch<T, DV, C, THREADS> y;
-            y.template load<VECTORS>(vp + r0 * a.v.st, (int)a.v.st, a.Dv - dv0, pad);
-            y.store(lds_v);
-            y.template load<VECTORS>(op + r0 * grad.st, (int)grad.st, a.Dv - dv0, pad);
-            y.store(lds_o);
-        }
+        // (tokens of padding are rows of zeros: their factor is kept from turning around)
+        if (c < 2 && threadIdx.x < C)
+            table_since[threadIdx.x / 4][threadIdx.x % 4] = exp2f(g2 * (float)max((int)threadIdx.x + 1 - pad, 0));
+        if (kAhead)
+            store();
+        else
+            fetch(r0, pad);
         __syncthreads();
+        if (kAhead && c + 1 < chunks) fetch(r0 + C, 0);
         int row_base = row_base_of_lane, v_row_base = v_row_base_of_lane, k_bases[KTile::kColumnBases],
             v_bases[VTile::kColumnBases];
         asm volatile("" : "+v"(row_base), "+v"(v_row_base));
@@ -613,40 +650,52 @@ __global__ __launch_bounds__(64 * NW, 1) void decay_kernel(const Sweep a, const 
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk)
                     pulls = mma(VTile::row(lds_v, v_row_base, j, kk), VTile::row(lds_o, v_row_base, i, kk), pulls);
+                float sum = 0.f;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int gap = 32 * (i - j) + ln - acc_row(r, half);
-                    const float f = (float)gap * exp2f(g2 * (float)max(gap, 0));
-                    if (gap > 0) chunk += f * (scores[r] * pulls[r]);
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    const f32x4 f = table_gap[i - j][r4][lane];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = scores[4 * r4 + e] * pulls[4 * r4 + e];
+                        // (selected, not multiplied by zero: a later token may be infinite)
+                        sum += i > j || acc_row(4 * r4 + e, half) < ln ? f[e] * x : 0.f;
+                    }
                 }
+                chunk += sum;
             }
 
-        // through the states
+        // through the states, some tiles of rows at a time
+        constexpr int kBlock = DKT < 4 ? DKT : 2;
 #pragma unroll
-        for (int t = 0; t < DKT; ++t) {
-            f32x16 G = {}, G1 = {};
+        for (int t0 = 0; t0 < DKT; t0 += kBlock) {
+            f32x16 G[kBlock], G1[kBlock];
+#pragma unroll
+            for (int t = 0; t < kBlock; ++t) G[t] = G1[t] = f32x16{};
 #pragma unroll
             for (int kk = 0; kk < 2 * CT; ++kk) {
                 f32x8 f, f1;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float since = (float)max(16 * kk + acc_row(e, half) + 1 - pad, 0);
-                    f[e] = exp2f(g2 * since);
-                    f1[e] = since * f[e];
+                    f[e] = table_since[4 * kk + 2 * (e / 4) + half][e % 4];
+                    f1[e] = (float)(16 * kk + acc_row(e, half) + 1 - pad) * f[e];
                 }
                 const f32x8 o = widened(VTile::column(lds_o, v_bases, 0, kk));
                 Frag<T> x[TERMS], x1[TERMS];
                 split_scaled<T>(o, f, x);
                 split_scaled<T>(o, f1, x1);
-                const Frag<T> q = KTile::column(lds_q, k_bases, t, kk);
 #pragma unroll
-                for (int i = 0; i < TERMS; ++i) {
-                    G = mma(q, x[i], G);
-                    G1 = mma(q, x1[i], G1);
+                for (int t = 0; t < kBlock; ++t) {
+                    const Frag<T> q = KTile::column(lds_q, k_bases, t0 + t, kk);
+#pragma unroll
+                    for (int i = 0; i < TERMS; ++i) {
+                        G[t] = mma(q, x[i], G[t]);
+                        G1[t] = mma(q, x1[i], G1[t]);
+                    }
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            chunk += sum16(D[t] * G + S[t] * G1);
+#pragma unroll
+            for (int t = 0; t < kBlock; ++t) chunk += sum16(D[t0 + t] * G[t] + S[t0 + t] * G1[t]);
         }
         total += chunk;
 
@@ -661,9 +710,8 @@ __global__ __launch_bounds__(64 * NW, 1) void decay_kernel(const Sweep a, const 
             f32x8 f, f1;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float left = (float)(C - 1 - 16 * kk - acc_row(e, half));
-                f[e] = exp2f(g2 * left);
-                f1[e] = left * f[e];
+                f[e] = table_left[4 * kk + 2 * (e / 4) + half][e % 4];
+                f1[e] = (float)(C - 1 - 16 * kk - acc_row(e, half)) * f[e];
             }
             const f32x8 v = widened(VTile::column(lds_v, v_bases, 0, kk));
             Frag<T> x[TERMS], x1[TERMS];

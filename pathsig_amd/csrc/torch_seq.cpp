@@ -15,6 +15,8 @@ using torch::autograd::variable_list;
 using MaybeTensor = std::optional<Tensor>;
 
 Tensor or_undefined(const MaybeTensor &t) { return t.has_value() ? *t : Tensor(); }
+// (an operator returns tensors: an empty one for what was not asked for)
+Tensor or_empty(const Tensor &t, const Tensor &like) { return t.defined() ? t : at::empty({0}, like.options()); }
 MaybeTensor or_none(const Tensor &t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
 
 int sequence_dtype(const Tensor &t, const char *what) {
@@ -102,7 +104,7 @@ AttentionCall attention_call(const Tensor &q, const Tensor &k, const Tensor &v, 
     return a;
 }
 
-// (out, last state or an empty tensor, the workspace: what the backward of the same call can use again, or undefined)
+// (out, last state or undefined, the workspace: what the backward of the same call can use again, or undefined)
 std::tuple<Tensor, Tensor, Tensor> attention_forward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay,
                                                      const Tensor &state, const Tensor &lengths, double scale, bool return_state,
                                                      bool learned_decay) {
@@ -110,8 +112,7 @@ std::tuple<Tensor, Tensor, Tensor> attention_forward(const Tensor &q, const Tens
     AttentionCall a = attention_call(q, k, v, log_decay, state, lengths, scale, true);
     a.c.learned_decay = learned_decay;
     Tensor out = at::empty({a.c.B, a.c.L, a.c.H, a.c.Dv}, a.q.options());
-    Tensor last = return_state ? at::empty({a.c.B, a.c.H, a.c.Dk, a.c.Dv}, a.log_decay.options())
-                               : at::empty({0}, a.log_decay.options());
+    Tensor last = return_state ? at::empty({a.c.B, a.c.H, a.c.Dk, a.c.Dv}, a.log_decay.options()) : Tensor();
     const size_t ws_bytes = pathsig_linattn_forward_workspace(&a.c);
     Tensor ws = scratch(ws_bytes, a.q);
     check_rc(pathsig_linattn_forward(&a.c, ptr(a.q), ptr(a.k), ptr(a.v), (const float *)ptr(a.state), ptr(out),
@@ -168,7 +169,7 @@ std::tuple<Tensor, Tensor> linear_attention_hip(const Tensor &q, const Tensor &k
                                                 bool return_state) {
     auto [out, last, kept] =
         attention_forward(q, k, v, log_decay, or_undefined(state), or_undefined(lengths), scale, return_state, false);
-    return {out, last};
+    return {out, or_empty(last, log_decay)};
 }
 
 Gradients linear_attention_backward_hip(const Tensor &grad_out, const MaybeTensor &grad_state, const Tensor &q, const Tensor &k,
@@ -216,12 +217,14 @@ struct AttentionFunction : public torch::autograd::Function<AttentionFunction<DI
         ctx->save_for_backward({q, k, v, log_decay, state, lengths, kept});
         ctx->saved_data["scale"] = scale;
         ctx->set_materialize_grads(false);
+        if (DIRECT && !return_state) return {out};
         if (!return_state) ctx->mark_non_differentiable({last});
         return {out, last};
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         variable_list out(8);
-        if (!grads[0].defined() && !grads[1].defined()) return out;
+        const Tensor grad_last = grads.size() > 1 ? grads[1] : Tensor();
+        if (!grads[0].defined() && !grad_last.defined()) return out;
         const auto saved = ctx->get_saved_variables();
         const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &log_decay = saved[3], &state = saved[4], &lengths = saved[5],
                      &kept = saved[6];
@@ -231,13 +234,13 @@ struct AttentionFunction : public torch::autograd::Function<AttentionFunction<DI
         const bool want_decay = ctx->needs_input_grad(3), want_state = state.defined() && ctx->needs_input_grad(4);
         bool direct = DIRECT && !at::GradMode::is_enabled();
         for (const Tensor *t : {(const Tensor *)&grad_out, &q, &k, &v, &log_decay}) direct = direct && plain(*t);
-        for (const Tensor *t : {&state, &lengths, &kept, (const Tensor *)&grads[1]}) direct = direct && (!t->defined() || plain(*t));
+        for (const Tensor *t : {&state, &lengths, &kept, &grad_last}) direct = direct && (!t->defined() || plain(*t));
         Gradients g;
         if (direct) {
-            g = attention_backward(grad_out, grads[1], q, k, v, log_decay, state, lengths, kept, scale, want_decay, want_state);
+            g = attention_backward(grad_out, grad_last, q, k, v, log_decay, state, lengths, kept, scale, want_decay, want_state);
         } else {
             static auto op = typed_op<AttentionBackwardOp>("pathsig::linear_attention_backward");
-            g = op.call(grad_out, or_none(grads[1]), q, k, v, log_decay, or_none(state), or_none(lengths), scale, want_decay,
+            g = op.call(grad_out, or_none(grad_last), q, k, v, log_decay, or_none(state), or_none(lengths), scale, want_decay,
                         want_state);
         }
         if (ctx->needs_input_grad(0)) out[0] = std::get<0>(g);
@@ -329,15 +332,15 @@ NormCall norm_call(const Tensor &x, const Tensor &weight, const Tensor &gate, co
     return a;
 }
 
-// (out, next, statistics): next and statistics are empty where they are not wanted
+// (out, next, statistics): next and statistics are undefined where they are not wanted
 std::tuple<Tensor, Tensor, Tensor> norm_forward(const Tensor &x, const Tensor &weight, const Tensor &gate, const Tensor &residual,
                                                 const Tensor &scale, const Tensor &next_weight, double eps, int64_t activation,
                                                 bool keep) {
     c10::DeviceGuard guard(x.device());
     const NormCall a = norm_call(x, weight, gate, residual, scale, next_weight, eps, activation);
     Tensor out = at::empty(a.shape, x.options());
-    Tensor next = next_weight.defined() ? at::empty(a.shape, x.options()) : at::empty({0}, x.options());
-    Tensor stats = at::empty({keep ? 2 : 0, a.c.rows}, x.options().dtype(at::kFloat));
+    Tensor next = next_weight.defined() ? at::empty(a.shape, x.options()) : Tensor();
+    Tensor stats = keep ? at::empty({2, a.c.rows}, x.options().dtype(at::kFloat)) : Tensor();
     check_rc(pathsig_norm_forward(&a.c, ptr(out), ptr(next), (float *)ptr(stats), stream_of(x)));
     return {out, next, stats};
 }
@@ -380,8 +383,10 @@ NormGradients norm_backward(const Tensor &grad_out, const Tensor &grad_next, con
 std::tuple<Tensor, Tensor, Tensor> norm_join_hip(const Tensor &x, const MaybeTensor &weight, const MaybeTensor &gate,
                                                  const MaybeTensor &residual, const MaybeTensor &scale,
                                                  const MaybeTensor &next_weight, double eps, int64_t activation, bool keep) {
-    return norm_forward(x, or_undefined(weight), or_undefined(gate), or_undefined(residual), or_undefined(scale),
-                        or_undefined(next_weight), eps, activation, keep);
+    auto [out, next, stats] = norm_forward(x, or_undefined(weight), or_undefined(gate), or_undefined(residual), or_undefined(scale),
+                                           or_undefined(next_weight), eps, activation, keep);
+    if (!keep) stats = at::empty({0, x.numel() / x.size(-1)}, x.options().dtype(at::kFloat));
+    return {out, or_empty(next, x), stats};
 }
 
 NormGradients norm_join_backward_hip(const MaybeTensor &grad_out, const MaybeTensor &grad_next, const Tensor &x,
@@ -419,6 +424,10 @@ struct NormFunction : public torch::autograd::Function<NormFunction<DIRECT>> {
         ctx->saved_data["eps"] = eps;
         ctx->saved_data["activation"] = activation;
         ctx->set_materialize_grads(false);
+        if constexpr (DIRECT) {
+            if (next_weight.defined()) return {out, next};
+            return {out};
+        }
         if (next_weight.defined())
             ctx->mark_non_differentiable({stats});
         else
@@ -427,19 +436,20 @@ struct NormFunction : public torch::autograd::Function<NormFunction<DIRECT>> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         variable_list out(8);
-        if (!grads[0].defined() && !grads[1].defined()) return out;
+        const Tensor &grad_out = grads[0], grad_next = grads.size() > 1 ? grads[1] : Tensor();
+        if (!grad_out.defined() && !grad_next.defined()) return out;
         const auto s = ctx->get_saved_variables();
         const double eps = ctx->saved_data["eps"].toDouble();
         const int64_t activation = ctx->saved_data["activation"].toInt();
         bool direct = DIRECT && !at::GradMode::is_enabled();
         for (const Tensor &t : s) direct = direct && (!t.defined() || plain(t));
-        for (int i = 0; i < 2; ++i) direct = direct && (!grads[i].defined() || plain(grads[i]));
+        for (const Tensor *t : {&grad_out, &grad_next}) direct = direct && (!t->defined() || plain(*t));
         NormGradients g;
         if (direct) {
-            g = norm_backward(grads[0], grads[1], s[0], s[1], s[2], s[3], s[4], s[5], s[6], eps, activation);
+            g = norm_backward(grad_out, grad_next, s[0], s[1], s[2], s[3], s[4], s[5], s[6], eps, activation);
         } else {
             static auto op = typed_op<NormBackwardOp>("pathsig::norm_join_backward");
-            g = op.call(or_none(grads[0]), or_none(grads[1]), s[0], or_none(s[1]), or_none(s[2]), or_none(s[3]), or_none(s[4]),
+            g = op.call(or_none(grad_out), or_none(grad_next), s[0], or_none(s[1]), or_none(s[2]), or_none(s[3]), or_none(s[4]),
                         or_none(s[5]), s[6], eps, activation);
         }
         const Tensor all[] = {std::get<0>(g), std::get<1>(g), std::get<2>(g), std::get<3>(g), std::get<4>(g), std::get<5>(g)};
@@ -495,7 +505,7 @@ PyObject *py_linear_attention(PyObject *, PyObject *const *args, Py_ssize_t narg
         if (any_grad({&t[0], &t[1], &t[2], &t[3], &t[4]})) {
             auto both = AttentionFunction<true>::apply(t[0], t[1], t[2], t[3], or_none(t[4]), or_none(t[5]), scale, return_state);
             out = both[0];
-            last = both[1];
+            if (return_state) last = both[1];
         } else {
             at::AutoDispatchBelowADInplaceOrView below;
             Tensor kept;
@@ -540,7 +550,7 @@ PyObject *py_norm_join(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
             auto all = NormFunction<true>::apply(t[0], or_none(t[1]), or_none(t[2]), or_none(t[3]), or_none(t[4]), or_none(t[5]), eps,
                                                  activation);
             out = all[0];
-            next = all[1];
+            if (t[5].defined()) next = all[1];
         } else {
             at::AutoDispatchBelowADInplaceOrView below;
             Tensor stats;
