@@ -55,8 +55,9 @@ __device__ __forceinline__ int64_t length_of(const int32_t *lengths, int64_t b, 
 }
 
 __device__ __forceinline__ float decay_of(const float *log_decay, int h) {
-    // (minus infinity forgets everything at once; a finite stand-in keeps 0 * g at 0)
-    return fmaxf(log_decay[h], -1e30f);
+    // (minus infinity forgets everything at once; a finite stand-in keeps 0 * g at 0.  NaN stays)
+    const float g = log_decay[h];
+    return g < -1e30f ? -1e30f : g;
 }
 
 // Tokens [begin, end) of `count` pieces from the s-th on, in the order of the sweep.  Pieces are cut at the same tokens in both

@@ -7,20 +7,28 @@
 //
 // A block has a head of a sequence (or of a piece of it) and up to 128 columns of its state; wave w has the 32 columns from
 // 32 w on, its part of the state in accumulator registers from the first chunk to the last.  All products are 32 x 32 tiles
-// laid out so that nothing crosses lanes:
+// laid out so that little crosses lanes:
 //   * scores transposed, K Q^T: a lane has one token i and sixteen j.  Decays and the causal mask are then factors of a lane's
-//     registers, and the rounded scores are, as they stand, the right operand of V^T P;
+//     registers, and the rounded scores are, as they stand, the right operand of V^T P.  The tiles are dealt to the waves (a single
+//     tile: its channels) and exchanged through LDS; computed by every wave they took a quarter of the matrix instructions;
 //   * answers transposed, S^T Q^T + V^T P: the state's accumulators, rounded, are, as they stand, the left operand;
 //   * an accumulator holds rows 8 (r / 4) + 4 (lane / 32) + r % 4.  Operands are read in that order of the contracted index
 //     ("accumulator order"): Q and K rows from LDS, where the channels of 16 are stored so that a lane's eight lie side by side,
 //     V^T and K^T with transposing reads of four rows each.
-// The scores are computed by every wave (a quarter of its matrix instructions) instead of exchanged through LDS behind a
-// barrier.  Rounding in bf16: scores and the state's copy to bf16 for the products with V and Q (relative 2^-8 a term, like the
-// rounding of the answers), the state itself and what is added to it stay in 32 bits: l^(C-1-j) v_j is split into three bf16
-// terms, which hold all 24 bits.
+// A chunk takes two barriers: before the first its tiles are stored, from registers that were loaded while the chunk before was
+// worked on; between the two everything that reads tiles happens; after the second the next chunk's tiles are stored while the
+// answers are finished from registers and scores.
+//
+// Rounding in bf16: scores and the state's copy for the products with V and Q (half a step of bf16 a term, like the rounding of the
+// answers).  The state itself stays in 32 bits, and so does what is added to it: l^(C-1-j) v_j is split into terms of bf16, three of
+// which hold all 24 bits (launch_terms).
 //
 // A first chunk that is not full is filled from the front with tokens of zeros, so that the factors l^(C-1-j) hold for every
 // chunk and none of them is a quotient.
+//
+// Bound by memory first: 16 x 4096 tokens of 16 heads of 128 in bf16 are 1.07 GB to read and write, 210 us at the rate of a large
+// copy (5.1 TB/s); the sweep takes 290 in two pieces, two blocks to a compute unit with 48 KB each on their way (without loads and
+// stores 150: 46 to 78 matrix instructions and about 400 vector ones a chunk and wave).  In one piece, one block to a unit, 356.
 #include <algorithm>
 
 #include "seq_attention.hpp"
@@ -31,8 +39,6 @@ namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
@@ -762,12 +768,15 @@ void launch_width(const Sweep &a, bool fold, hipStream_t stream) {
         chunk_kernel<T, T, DKT, NW, TERMS, false, VECTORS><<<grid, block, 0, stream>>>(a, slices);
 }
 
-// A state that is handed out in 32 bits is summed from all bits of its terms.  One that only answers, through a copy in the type
-// of the products, is summed from terms of that type: each is off by as much as the copy is.
+// A state that is handed out in 32 bits is summed from all bits of its terms.  For one that only answers, through a copy in the type
+// of the products, two terms of bf16 are enough; one would be off by as much as the copy is (root mean square of the error of an
+// answer 2.7e-3 of its size with one, 2.3e-3 with two or three, 1.7e-3 of them its own rounding; 16 x 4096 tokens, 16 heads of 128).
 template <typename T, int DKT, int NW, bool VECTORS>
 void launch_terms(const Sweep &a, bool fold, hipStream_t stream) {
-    if constexpr (sizeof(T) == 2)
+    if constexpr (sizeof(T) == 2) {
         if (a.exact_state) return launch_width<T, DKT, NW, 3, VECTORS>(a, fold, stream);
+        return launch_width<T, DKT, NW, 2, VECTORS>(a, fold, stream);
+    }
     launch_width<T, DKT, NW, 1, VECTORS>(a, fold, stream);
 }
 

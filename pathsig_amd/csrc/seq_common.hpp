@@ -1,7 +1,6 @@
 // What the sequence operators (linear attention, norms) share: element types, vector access, reductions.
 #pragma once
 
-#include <hip/hip_bf16.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -32,7 +32,7 @@ void check_like(const Tensor &t, const char *what, const Tensor &like, const cha
 
 // the channels of a head side by side, and tokens no further apart than the kernels' offsets reach
 Tensor side_by_side(const Tensor &t) {
-    const bool near = t.dim() < 4 || t.stride(1) <= PATHSIG_MAX_TOKEN_STRIDE;
+    const bool near = t.dim() < 4 || t.size(1) <= 1 || t.stride(1) <= PATHSIG_MAX_TOKEN_STRIDE;
     return near && (t.size(-1) == 1 || t.stride(-1) == 1) ? t : t.contiguous();
 }
 
@@ -42,10 +42,13 @@ struct AttentionCall {
     pathsig_linattn c;
 };
 
+// (the stride of an axis of one is anything, and never used)
+int64_t stride_of(const Tensor &t, int64_t axis) { return t.size(axis) > 1 ? t.stride(axis) : 0; }
+
 void set_strides(int64_t (&out)[3], const Tensor &t, bool token) {
-    out[0] = t.stride(0);
-    out[1] = token ? t.stride(1) : 0;
-    out[2] = t.stride(token ? 2 : 1);
+    out[0] = stride_of(t, 0);
+    out[1] = token ? stride_of(t, 1) : 0;
+    out[2] = stride_of(t, token ? 2 : 1);
 }
 
 // token: q is [B, L, H, D] and so on; else [B, H, D], one token of every sequence
@@ -159,8 +162,8 @@ Tensor attention_step(const Tensor &q, const Tensor &k, const Tensor &v, const T
     TORCH_CHECK(state.defined() && state.is_contiguous(), "state is updated in place: it must be contiguous");
     const AttentionCall a = attention_call(q, k, v, log_decay, state, Tensor(), scale, false);
     Tensor out = at::empty({a.c.B, a.c.H, a.c.Dv}, a.q.options());
+    torch::autograd::impl::bump_version(state);  // (first: it refuses an inference tensor outside of inference mode)
     check_rc(pathsig_linattn_step(&a.c, ptr(a.q), ptr(a.k), ptr(a.v), (float *)ptr(a.state), ptr(out), stream_of(a.q)));
-    torch::autograd::impl::bump_version(state);
     return out;
 }
 

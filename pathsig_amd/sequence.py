@@ -38,7 +38,7 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, *, stat
 
     Returns out (B, L, H, Dv), with `return_state` also S after the last token of every sequence, (B, H, Dk, Dv) float32.
     """
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    scale = max(q.shape[-1], 1) ** -0.5 if scale is None else float(scale)
     if not _is_compiling():
         out = _direct.linear_attention(q, k, v, log_decay, state, lengths, scale, return_state)
         if out is not None:
@@ -51,7 +51,7 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
                           scale: float | None = None) -> Tensor:
     """One token of every sequence: q (B, H, Dk), k (B, Hkv, Dk), v (B, Hkv, Dv); `state`, contiguous (B, H, Dk, Dv) float32,
     is updated in place.  Returns (B, H, Dv).  No gradient."""
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    scale = max(q.shape[-1], 1) ** -0.5 if scale is None else float(scale)
     if not _is_compiling():
         out = _direct.linear_attention_step(q, k, v, log_decay, state, scale)
         if out is not None:

@@ -300,6 +300,29 @@ def test_refusals_on_the_device():
         torch.autograd.grad(grad.sum(), q)
 
 
+def test_axes_of_one_and_decays_that_are_no_number():
+    from pathsig_amd import sequence
+    a = _inputs(2, 1, 2, 1, 8, 16, F32, seed=115)
+    want = sequence.linear_attention(a["q"], a["k"], a["v"], a["g"])
+    far = {n: torch.as_strided(a[n], a[n].shape, (a[n].stride(0), 2 ** 26, *a[n].stride()[2:])) for n in ("q", "k", "v")}
+    assert torch.equal(sequence.linear_attention(far["q"], far["k"], far["v"], a["g"]), want)
+    a["g"][1] = math.nan
+    out, last = sequence.linear_attention(a["q"], a["k"], a["v"], a["g"], state=a["s0"], return_state=True)
+    assert out[:, :, 1].isnan().all() and last[:, 1].isnan().all() and torch.isfinite(out[:, :, 0]).all()
+    state = a["s0"].clone()
+    sequence.linear_attention_step(a["q"][:, 0], a["k"][:, 0], a["v"][:, 0], a["g"], state)
+    assert state[:, 1].isnan().all() and torch.isfinite(state[:, 0]).all()
+    with torch.inference_mode():
+        state = a["s0"].clone()
+        sequence.linear_attention_step(a["q"][:, 0], a["k"][:, 0], a["v"][:, 0], a["g"], state)
+    kept = state.clone()
+    with torch.no_grad(), pytest.raises(RuntimeError, match="[Ii]nference"):
+        sequence.linear_attention_step(a["q"][:, 0], a["k"][:, 0], a["v"][:, 0], a["g"], state)
+    assert torch.equal(state[:, 0], kept[:, 0])
+    with pytest.raises(RuntimeError):
+        sequence.linear_attention(a["q"][..., :0], a["k"][..., :0], a["v"], a["g"])
+
+
 def test_nothing_to_do():
     from pathsig_amd import sequence
     g = torch.tensor([-0.1, -0.2], device=DEV, requires_grad=True)
