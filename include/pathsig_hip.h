@@ -252,7 +252,8 @@ float pathsig_profile_sweep_ms(void);
  *   hold; out and the gradients get zeros there.  The final state is S after token n_b - 1 (the initial state if n_b = 0).
  *   out [B, L, H, Dv] in the type of q, state and final_state [B, H, Dk, Dv] float32, all dense.
  * Types: PATHSIG_F32 and PATHSIG_BF16 for q, k, v, out and their gradients.  Dk and Dv from 1 to PATHSIG_MAX_HEAD_DIM, tokens up
- * to PATHSIG_MAX_TOKEN_STRIDE elements apart.
+ * to PATHSIG_MAX_TOKEN_STRIDE elements apart.  Where Dk, Dv and all strides are multiples of 16 bytes, q, k, v (and grad_out of the
+ * backward) have to start at such; other tensors may start anywhere and are copied into the workspace first.
  */
 #define PATHSIG_BF16 2
 #define PATHSIG_MAX_HEAD_DIM 256
@@ -275,7 +276,7 @@ int pathsig_linattn_forward(const pathsig_linattn *call, const void *q, const vo
 
 /*
  * Its backward.  kept: the forward's workspace as the forward of the same call left it (pathsig_linattn_forward_workspace bytes:
- * the states between pieces of long sequences), or NULL, and the backward works them out again.
+ * states between pieces of long sequences, copies), or NULL, and the backward works it out again.
  *   grad_out is a dense [B, L, H, Dv], grad_final_state [B, H, Dk, Dv] float32 or NULL (zero).
  *   grad_q [B, L, H, Dk], grad_k [B, L, Hkv, Dk], grad_v [B, L, Hkv, Dv] dense, in the type of q (sums over the heads that share
  *   a key); grad_log_decay [H] and grad_state [B, H, Dk, Dv] float32, each NULL where it is not wanted.

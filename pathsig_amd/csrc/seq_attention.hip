@@ -175,23 +175,31 @@ int check_call(const pathsig_linattn *c) {
     return PATHSIG_OK;
 }
 
-View view(const void *p, const int64_t *stride, int64_t group, int element) {
-    const int64_t E = 16 / element;
-    return {p, stride[0], stride[1], stride[2], (int)group, aligned16(p) && stride[0] % E == 0 && stride[1] % E == 0 && stride[2] % E == 0};
+View view(const void *p, const int64_t *stride, int64_t group) { return {p, stride[0], stride[1], stride[2], (int)group}; }
+
+View dense(const void *p, int64_t L, int64_t heads, int64_t D, int64_t group) {
+    return {p, L * heads * D, heads * D, D, (int)group};
 }
 
-View dense(const void *p, int64_t L, int64_t H, int64_t D, int element) {
-    const int64_t stride[3] = {L * H * D, H * D, D};
-    return view(p, stride, 1, element);
+int64_t element_of(const pathsig_linattn *c) { return c->dtype == PATHSIG_F32 ? 4 : 2; }
+// channels in whole units of 16 bytes
+int64_t padded(const pathsig_linattn *c, int64_t D) { return ceil_div(D * element_of(c), 16) * 16 / element_of(c); }
+
+// q, k and v do not lie in whole units of 16 bytes
+bool copied(const pathsig_linattn *c) {
+    const int64_t E = 16 / element_of(c);
+    int64_t odd = c->Dk % E + c->Dv % E;
+    for (int i = 0; i < 3; ++i) odd += c->q_stride[i] % E + c->k_stride[i] % E + c->v_stride[i] % E;
+    return odd > 0;
 }
 
 // Pieces of a call's sweeps, the same for all of them: as many as bring two waves to each of the 1024 SIMDs (a block has a wave for
-// 32 columns of the state, up to four), of whole chunks, and not so short that what a piece costs (its state written and read,
+// 32 columns of the state, up to four; four waves in fp32: 50 x 333, 6 heads of 40 x 56, 353 -> 393 us a step), of whole chunks, and not so short that what a piece costs (its state written and read,
 // 8 Dk Dv bytes) is more than what its tokens do.  Two pieces of blocks of four waves are folded in halves, or every second compute
 // unit would have no block to fold with.
 void cut(const pathsig_linattn *c, int64_t *piece, int *pieces, int *run) {
     const int64_t wide = std::max(c->Dk, c->Dv), waves = wide <= 32 ? 1 : wide <= 64 ? 2 : 4;
-    const int64_t blocks = std::max<int64_t>(c->B * c->H, 1), element = c->dtype == PATHSIG_F32 ? 4 : 2;
+    const int64_t blocks = std::max<int64_t>(c->B * c->H, 1), element = element_of(c);
     const int64_t least = std::max<int64_t>(64, 8 * c->Dk * c->Dv / (element * (c->Dk + c->Dv)));
     const int64_t want = std::max<int64_t>(1, std::min(2048 / waves / blocks, c->L / least));
     *run = want == 2 && waves == 4 && c->L >= 4 * least ? 2 : 1;
@@ -216,6 +224,8 @@ Sweep sweep_of(const pathsig_linattn *c) {
     a.H = (int)c->H;
     a.Dk = (int)c->Dk;
     a.Dv = (int)c->Dv;
+    a.Kp = (int)padded(c, c->Dk);
+    a.Vp = (int)padded(c, c->Dv);
     a.in_scale = 1.f;
     a.out_scale = 1.f;
     a.row = c->Dv;
@@ -250,31 +260,8 @@ template <typename T>
 void decay(const Sweep &a, const Sweep &back, const View &grad_out, float *partial, hipStream_t stream) {
     if (a.Dk <= 32) return launch_decay<T, 1>(a, back, grad_out, partial, stream);
     if (a.Dk <= 64) return launch_decay<T, 2>(a, back, grad_out, partial, stream);
-    if (a.Dk <= 128) return launch_decay<T, 4>(a, back, grad_out, partial, stream);
-    launch_decay<T, 8>(a, back, grad_out, partial, stream);
+    launch_decay<T, 4>(a, back, grad_out, partial, stream);
 }
-
-template <typename T>
-int forward_t(const pathsig_linattn *c, const void *q, const void *k, const void *v, const float *state, void *out, float *final_state,
-              float *starts, hipStream_t stream) {
-    Sweep a = sweep_of(c);
-    const int64_t group = c->H / c->Hkv;
-    a.q = view(q, c->q_stride, 1, sizeof(T));
-    a.k = view(k, c->k_stride, group, sizeof(T));
-    a.v = view(v, c->v_stride, group, sizeof(T));
-    a.first = state;
-    a.last = final_state;
-    a.out = out;
-    a.out_scale = c->scale;
-    a.exact_state = final_state || c->learned_decay;
-    fold<T>(a, starts, stream);
-    chunks<T>(a, false, stream);
-    return launch_status("linear attention");
-}
-
-struct BackwardLayout {
-    size_t starts, ends, wide_k, wide_v, decay, total;  // byte offsets
-};
 
 size_t place(size_t &total, size_t bytes) {
     const size_t at = total;
@@ -282,18 +269,127 @@ size_t place(size_t &total, size_t bytes) {
     return at;
 }
 
+// what a forward's workspace holds: the states in front of the pieces, and q, k and v where they are copied
+struct ForwardLayout {
+    size_t starts, q, k, v, total;  // byte offsets
+};
+
+ForwardLayout forward_layout(const pathsig_linattn *c) {
+    ForwardLayout l = {};
+    l.starts = place(l.total, starts_bytes(c));
+    if (copied(c)) {
+        const size_t tokens = (size_t)c->B * c->L * element_of(c), K = padded(c, c->Dk), V = padded(c, c->Dv);
+        l.q = place(l.total, tokens * c->H * K);
+        l.k = place(l.total, tokens * c->Hkv * K);
+        l.v = place(l.total, tokens * c->Hkv * V);
+    }
+    return l;
+}
+
+struct Copy {
+    const void *from;
+    void *to;
+    int64_t sb, st, sh;
+    int heads, D, padded;
+};
+struct Copies {
+    Copy c[3];
+};
+
+// Rows of D channels to rows of whole units, the rest zeros; a thread has a unit.  Tokens behind the end of a sequence are left out.
+template <typename T>
+__global__ __launch_bounds__(256) void copy_kernel(const Copies copies, int64_t L, const int32_t *lengths) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const Copy &c = copies.c[blockIdx.z];
+    const int64_t b = blockIdx.y, n = length_of(lengths, b, L), per_token = (int64_t)c.heads * (c.padded / E);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n * per_token; i += (int64_t)gridDim.x * 256) {
+        const int64_t t = i / per_token, in_token = i % per_token;
+        const int h = (int)(in_token / (c.padded / E)), at = (int)(in_token % (c.padded / E)) * E;
+        const T *const from = (const T *)c.from + b * c.sb + t * c.st + h * c.sh + at;
+        Pack<T, E> unit = {};
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (at + e < c.D) unit.v[e] = from[e];
+        *(Pack<T, E> *)((T *)c.to + ((b * L + t) * c.heads + h) * c.padded + at) = unit;
+    }
+}
+
+template <typename T>
+void copy(const pathsig_linattn *c, const Copy *list, int count, hipStream_t stream) {
+    if (c->L == 0) return;
+    Copies all = {};
+    int64_t most = 0;
+    for (int i = 0; i < count; ++i) {
+        all.c[i] = list[i];
+        most = std::max(most, c->L * list[i].heads * list[i].padded * (int64_t)sizeof(T) / 16);
+    }
+    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(most, 256), std::max<int64_t>(1, 4096 / c->B));
+    copy_kernel<T><<<dim3(blocks, (unsigned)c->B, (unsigned)count), 256, 0, stream>>>(all, c->L, c->lengths);
+}
+
+struct Inputs {
+    View q, k, v;
+};
+
+// q, k and v as the sweeps read them: in place, or copied into (or already in) a forward's workspace
+template <typename T>
+Inputs inputs(const pathsig_linattn *c, const void *q, const void *k, const void *v, char *ws, bool there, hipStream_t stream) {
+    const int64_t group = c->H / c->Hkv;
+    if (!copied(c)) return {view(q, c->q_stride, 1), view(k, c->k_stride, group), view(v, c->v_stride, group)};
+    const ForwardLayout l = forward_layout(c);
+    const int64_t K = padded(c, c->Dk), V = padded(c, c->Dv);
+    if (!there) {
+        const int H = (int)c->H, Hkv = (int)c->Hkv, Dk = (int)c->Dk, Dv = (int)c->Dv;
+        const Copy list[3] = {{q, ws + l.q, c->q_stride[0], c->q_stride[1], c->q_stride[2], H, Dk, (int)K},
+                              {k, ws + l.k, c->k_stride[0], c->k_stride[1], c->k_stride[2], Hkv, Dk, (int)K},
+                              {v, ws + l.v, c->v_stride[0], c->v_stride[1], c->v_stride[2], Hkv, Dv, (int)V}};
+        copy<T>(c, list, 3, stream);
+    }
+    return {dense(ws + l.q, c->L, c->H, K, 1), dense(ws + l.k, c->L, c->Hkv, K, group), dense(ws + l.v, c->L, c->Hkv, V, group)};
+}
+
+// pointers that are read in whole units where they are not copied
+bool aligned(const pathsig_linattn *c, const void *q, const void *k, const void *v) {
+    if (copied(c) || (aligned16(q) && aligned16(k) && aligned16(v))) return true;
+    set_error("q, k and v must start at multiples of 16 bytes");
+    return false;
+}
+
+template <typename T>
+int forward_t(const pathsig_linattn *c, const void *q, const void *k, const void *v, const float *state, void *out, float *final_state,
+              char *ws, hipStream_t stream) {
+    Sweep a = sweep_of(c);
+    const Inputs in = inputs<T>(c, q, k, v, ws, false, stream);
+    a.q = in.q;
+    a.k = in.k;
+    a.v = in.v;
+    a.first = state;
+    a.last = final_state;
+    a.out = out;
+    a.out_scale = c->scale;
+    a.exact_state = final_state || c->learned_decay;
+    fold<T>(a, (float *)(ws + forward_layout(c).starts), stream);
+    chunks<T>(a, false, stream);
+    return launch_status("linear attention");
+}
+
+struct BackwardLayout {
+    size_t forward, ends, grad_out, wide_k, wide_v, decay, total;  // byte offsets
+};
+
 int64_t decay_partials(const pathsig_linattn *c) {
     int64_t piece;
     int pieces, run;
     cut(c, &piece, &pieces, &run);
-    return pieces / run * ceil_div(c->Dv, 128) * c->B;
+    return pieces / run * ceil_div(c->Dk, 128) * ceil_div(c->Dv, 128) * c->B;
 }
 
 BackwardLayout backward_layout(const pathsig_linattn *c, bool want_decay) {
     BackwardLayout l = {};
     const size_t tokens = (size_t)c->B * c->L * c->H;
-    l.starts = place(l.total, starts_bytes(c));
+    l.forward = place(l.total, forward_layout(c).total);
     l.ends = place(l.total, starts_bytes(c));
+    if (padded(c, c->Dv) != c->Dv) l.grad_out = place(l.total, tokens * padded(c, c->Dv) * element_of(c));
     if (c->H != c->Hkv) {
         l.wide_k = place(l.total, tokens * c->Dk * sizeof(float));
         l.wide_v = place(l.total, tokens * c->Dv * sizeof(float));
@@ -303,13 +399,20 @@ BackwardLayout backward_layout(const pathsig_linattn *c, bool want_decay) {
 }
 
 template <typename T>
-int backward_t(const pathsig_linattn *c, const void *q, const void *k, const void *v, const float *state, const float *kept,
+int backward_t(const pathsig_linattn *c, const void *q, const void *k, const void *v, const float *state, const char *kept,
                const void *grad_out, const float *grad_final, void *grad_q, void *grad_k, void *grad_v, float *grad_decay,
                float *grad_state, char *ws, hipStream_t stream) {
     const int64_t group = c->H / c->Hkv;
-    const View vq = view(q, c->q_stride, 1, sizeof(T)), vk = view(k, c->k_stride, group, sizeof(T)),
-               vv = view(v, c->v_stride, group, sizeof(T)), vdo = dense(grad_out, c->L, c->H, c->Dv, sizeof(T));
     const BackwardLayout l = backward_layout(c, grad_decay != nullptr);
+    char *const from_forward = kept ? const_cast<char *>(kept) : ws + l.forward;
+    const Inputs in = inputs<T>(c, q, k, v, from_forward, kept != nullptr, stream);
+    const View vq = in.q, vk = in.k, vv = in.v;
+    View vdo = dense(grad_out, c->L, c->H, c->Dv, 1);
+    if (const int64_t V = padded(c, c->Dv); V != c->Dv) {
+        const Copy one = {grad_out, ws + l.grad_out, vdo.sb, vdo.st, vdo.sh, (int)c->H, (int)c->Dv, (int)V};
+        copy<T>(c, &one, 1, stream);
+        vdo = dense(ws + l.grad_out, c->L, c->H, V, 1);
+    }
     // the forward's states in front of the pieces
     Sweep forward = sweep_of(c);
     forward.q = vq;
@@ -319,12 +422,13 @@ int backward_t(const pathsig_linattn *c, const void *q, const void *k, const voi
     forward.out_scale = c->scale;
     forward.exact_state = grad_decay != nullptr;
     if (kept)
-        forward.starts = const_cast<float *>(kept);
+        forward.starts = (float *)from_forward;
     else
-        fold<T>(forward, (float *)(ws + l.starts), stream);
+        fold<T>(forward, (float *)from_forward, stream);
     // dq: the forward with (do, v, k) and the transposed states
     Sweep a = forward;
     std::swap(a.Dk, a.Dv);
+    std::swap(a.Kp, a.Vp);
     a.q = vdo;
     a.k = vv;
     a.v = vk;
@@ -350,6 +454,7 @@ int backward_t(const pathsig_linattn *c, const void *q, const void *k, const voi
     // dk: backwards in time with (v, do, q), from the same states, transposed
     a = back;
     std::swap(a.Dk, a.Dv);
+    std::swap(a.Kp, a.Vp);
     a.q = vv;
     a.k = vdo;
     a.v = vq;
@@ -378,9 +483,9 @@ template <typename T>
 int step_t(const pathsig_linattn *c, const void *q, const void *k, const void *v, float *state, void *out, hipStream_t stream) {
     Sweep a = sweep_of(c);
     const int64_t group = c->H / c->Hkv;
-    a.q = view(q, c->q_stride, 1, sizeof(T));
-    a.k = view(k, c->k_stride, group, sizeof(T));
-    a.v = view(v, c->v_stride, group, sizeof(T));
+    a.q = view(q, c->q_stride, 1);
+    a.k = view(k, c->k_stride, group);
+    a.v = view(v, c->v_stride, group);
     a.out = out;
     a.out_scale = c->scale;
     const dim3 grid((unsigned)c->H, (unsigned)c->B);
@@ -405,7 +510,7 @@ extern "C" {
 
 size_t pathsig_linattn_forward_workspace(const pathsig_linattn *call) {
     if (check_call(call) != PATHSIG_OK) return 0;
-    return starts_bytes(call);
+    return forward_layout(call).total;
 }
 
 int pathsig_linattn_forward(const pathsig_linattn *call, const void *q, const void *k, const void *v, const float *state,
@@ -421,8 +526,9 @@ int pathsig_linattn_forward(const pathsig_linattn *call, const void *q, const vo
         set_error("linear attention: workspace of %zu bytes needed, got %zu", need, workspace ? workspace_bytes : (size_t)0);
         return PATHSIG_ERR_WORKSPACE;
     }
-    if (call->dtype == PATHSIG_F32) return forward_t<float>(call, q, k, v, state, out, final_state, (float *)workspace, (hipStream_t)stream);
-    return forward_t<bf16>(call, q, k, v, state, out, final_state, (float *)workspace, (hipStream_t)stream);
+    if (!aligned(call, q, k, v)) return PATHSIG_ERR_ARGUMENT;
+    if (call->dtype == PATHSIG_F32) return forward_t<float>(call, q, k, v, state, out, final_state, (char *)workspace, (hipStream_t)stream);
+    return forward_t<bf16>(call, q, k, v, state, out, final_state, (char *)workspace, (hipStream_t)stream);
 }
 
 size_t pathsig_linattn_backward_workspace(const pathsig_linattn *call, int want_log_decay) {
@@ -443,8 +549,8 @@ int pathsig_linattn_backward(const pathsig_linattn *call, const void *q, const v
         set_error("grad_log_decay is asked for, but learned_decay is not set");
         return PATHSIG_ERR_ARGUMENT;
     }
-    if (kept && kept_bytes != starts_bytes(call)) {
-        set_error("kept: the forward's workspace has %zu bytes, got %zu", starts_bytes(call), kept_bytes);
+    if (kept && kept_bytes != forward_layout(call).total) {
+        set_error("kept: the forward's workspace has %zu bytes, got %zu", forward_layout(call).total, kept_bytes);
         return PATHSIG_ERR_ARGUMENT;
     }
     const size_t need = backward_layout(call, grad_log_decay != nullptr).total;
@@ -457,10 +563,14 @@ int pathsig_linattn_backward(const pathsig_linattn *call, const void *q, const v
         decay_sum_kernel<<<(unsigned)call->H, 64, 0, (hipStream_t)stream>>>(nullptr, 0, (int)call->H, grad_log_decay);
         return launch_status("linear attention, backward");
     }
+    if (!aligned(call, q, k, v) || (padded(call, call->Dv) == call->Dv && !aligned16(grad_out))) {
+        set_error("q, k, v and grad_out must start at multiples of 16 bytes");
+        return PATHSIG_ERR_ARGUMENT;
+    }
     if (call->dtype == PATHSIG_F32)
-        return backward_t<float>(call, q, k, v, state, (const float *)kept, grad_out, grad_final_state, grad_q, grad_k, grad_v,
+        return backward_t<float>(call, q, k, v, state, (const char *)kept, grad_out, grad_final_state, grad_q, grad_k, grad_v,
                                  grad_log_decay, grad_state, (char *)workspace, (hipStream_t)stream);
-    return backward_t<bf16>(call, q, k, v, state, (const float *)kept, grad_out, grad_final_state, grad_q, grad_k, grad_v,
+    return backward_t<bf16>(call, q, k, v, state, (const char *)kept, grad_out, grad_final_state, grad_q, grad_k, grad_v,
                             grad_log_decay, grad_state, (char *)workspace, (hipStream_t)stream);
 }
 

@@ -7,12 +7,12 @@
 namespace psig {
 namespace seq {
 
-// a [B, L, heads, D] tensor; heads[h / group] is read for head h
+// A [B, L, heads, D] tensor; heads[h / group] is read for head h.  Rows start at multiples of 16 bytes and hold whole units of 16
+// bytes: tensors that do not lie so are copied first, with zeros behind the last channel.
 struct View {
     const void *p;
     int64_t sb, st, sh;
     int group;
-    int vectors;  // rows start at multiples of 16 bytes
 };
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -32,7 +32,7 @@ struct Sweep {
     const float *log_decay;
     const int32_t *lengths;
     int64_t B, L;
-    int H, Dk, Dv;
+    int H, Dk, Dv, Kp, Vp;  // Kp, Vp: channels of a row of q and k, and of v, in whole units
     float in_scale, out_scale;
     int reverse;
     int exact_state;       // the state is wanted in 32 bits, not only the answers
@@ -76,8 +76,9 @@ __device__ __forceinline__ Range range_of(const Sweep &a, int64_t n, int s, int 
 template <typename T, int DKT>
 void launch_chunks(const Sweep &a, bool fold, hipStream_t stream);
 
-// The gradient of the decays: partial sums [pieces][slices][B][H], slices = ceil(Dv / 128).  a: the sweep forwards in time; back: the
+// The gradient of the decays: partial sums [runs][slices][B][H], slices = decay_slices().  a: the sweep forwards in time; back: the
 // one backwards in time with the same rows and columns, whose states are the gradients of a's.
+inline int decay_slices(const Sweep &a) { return (int)(ceil_div(a.Dk, 128) * ceil_div(a.Dv, 128)); }
 template <typename T, int DKT>
 void launch_decay(const Sweep &a, const Sweep &back, const View &grad_out, float *partial, hipStream_t stream);
 

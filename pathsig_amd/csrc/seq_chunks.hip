@@ -171,13 +171,12 @@ struct Fetch {
     static_assert(THREADS % L::kUnits == 0, "a thread's units lie in one column");
     u32x4 x[kEach];
 
-    // p: the tile's first row and channel.  The rows before `pad` are zeros and not read, as are channels from `channels` on.
-    // st: from row to row, backwards in time negative.  VECTORS: whole units at addresses of whole units.
-    template <bool VECTORS>
+    // p: the tile's first row and channel.  The rows before `pad` are zeros and not read, as are channels from `channels` on, a
+    // multiple of a unit.  st: from row to row, backwards in time negative.
     __device__ __forceinline__ void load(const T *p, int st, int channels, int pad) {
         const int row0 = threadIdx.x / L::kUnits, c = threadIdx.x % L::kUnits * L::kPerUnit;
         const int offset = row0 * st + c;
-        if (VECTORS && kTotal % THREADS == 0 && pad <= 0 && channels >= D) {
+        if (kTotal % THREADS == 0 && pad <= 0 && channels >= D) {
 #pragma unroll
             for (int u = 0; u < kEach; ++u) x[u] = *(const u32x4 *)(p + (int64_t)u * kRowsApart * st + offset);
             return;
@@ -187,16 +186,7 @@ struct Fetch {
             const int row = row0 + u * kRowsApart;
             x[u] = u32x4{0, 0, 0, 0};
             if ((kTotal % THREADS && row >= ROWS) || row < pad || c >= channels) continue;
-            const T *const q = p + (int64_t)u * kRowsApart * st + offset;
-            if constexpr (VECTORS) {
-                x[u] = *(const u32x4 *)q;
-            } else {
-                Pack<T, L::kPerUnit> one = {};
-#pragma unroll
-                for (int e = 0; e < L::kPerUnit; ++e)
-                    if (c + e < channels) one.v[e] = q[e];
-                x[u] = __builtin_bit_cast(u32x4, one);
-            }
+            x[u] = *(const u32x4 *)(p + (int64_t)u * kRowsApart * st + offset);
         }
     }
     __device__ __forceinline__ void store(char *lds) const {
@@ -234,16 +224,16 @@ constexpr int chunk_tiles(int DKT, int NW) {
 
 // The state in front of a piece (FOLD: zero): this lane's column dv, rows in accumulator order.
 template <int DKT, int NW, bool FOLD>
-__device__ __forceinline__ void load_state(f32x16 (&S)[DKT], const Sweep &a, int64_t b, int h, int64_t n, int piece, float g2, int dv0,
-                                           int dv, int half) {
+__device__ __forceinline__ void load_state(f32x16 (&S)[DKT], const Sweep &a, int64_t b, int h, int64_t n, int piece, float g2, int dk0,
+                                           int dv0, int dv, int half) {
     const int64_t plane = (int64_t)a.Dk * a.Dv, head = (b * a.H + h) * plane, between = a.B * a.H * plane;
 #pragma unroll
     for (int t = 0; t < DKT; ++t) S[t] = f32x16{};
     if (FOLD) return;
-    const bool joined = a.pieces > kJoinInside, whole = a.Dk == 32 * DKT && dv0 + 32 * NW <= a.Dv;
+    const bool joined = a.pieces > kJoinInside, whole = dk0 + 32 * DKT <= a.Dk && dv0 + 32 * NW <= a.Dv;
     const int row = (int)a.row, column = (int)a.column;
     // one base for all lanes and 32-bit offsets; rows and columns behind the last are zeros, their addresses are kept inside
-    const uint32_t offset = whole ? dv * column + 4 * half * row : min(dv, a.Dv - 1) * column;
+    const uint32_t offset = whole ? dv * column + (dk0 + 4 * half) * row : min(dv, a.Dv - 1) * column;
     // the state in front of the first token (s = -1) and what the pieces up to this one add, or all of that at once
     for (int s = joined ? piece - 1 : a.first ? -1 : 0; s < piece; ++s) {
         const float *const p = (s < 0 && !joined ? a.first : a.starts + (s + 1) * between) + head;
@@ -273,7 +263,7 @@ __device__ __forceinline__ void load_state(f32x16 (&S)[DKT], const Sweep &a, int
             for (int t = 0; t < DKT; ++t)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int dk = 32 * t + acc_row(r, half);
+                    const int dk = dk0 + 32 * t + acc_row(r, half);
                     const float y = p[offset + (uint32_t)(min(dk, a.Dk - 1) * row)];
                     x[t][r] = dk < a.Dk && dv < a.Dv ? y : 0.f;
                 }
@@ -284,7 +274,7 @@ __device__ __forceinline__ void load_state(f32x16 (&S)[DKT], const Sweep &a, int
 }
 
 // TERMS: of l^(C-1-j) v_j in the state's update.
-template <typename T, typename O, int DKT, int NW, int TERMS, bool FOLD, bool VECTORS>
+template <typename T, typename O, int DKT, int NW, int TERMS, bool FOLD>
 __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_kernel(const Sweep a, int slices) {
     constexpr int DK = 32 * DKT, DV = 32 * NW, CT = chunk_tiles<T>(DKT, NW), C = 32 * CT, THREADS = 64 * NW;
     // fetched a chunk ahead, where registers allow it
@@ -322,7 +312,7 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
     if (begin >= end && !owns_end && !FOLD) return;
 
     f32x16 S[DKT];
-    load_state<DKT, NW, FOLD>(S, a, b, h, n, piece, g2, dv0, dv, half);
+    load_state<DKT, NW, FOLD>(S, a, b, h, n, piece, g2, 0, dv0, dv, half);
 
     // Factors of a lane's registers, in LDS (they would fill the registers, and are read once a chunk): l^(C - 1 - j) for the state's
     // update; for scores l^(31 - j), which l^(i + 1) completes in the tile off the diagonal, and l^(i - j) in those on it (j after i
@@ -354,11 +344,11 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
     // (where registers do not hold a whole chunk, the tensors pass through them one after the other)
     auto fetch = [&](int64_t at, int pad) {
         const int64_t t = a.reverse ? n - 1 - at : at;
-        fk.template load<VECTORS>(kp + t * a.k.st, sign * (int)a.k.st, a.Dk, pad);
+        fk.load(kp + t * a.k.st, sign * (int)a.k.st, a.Kp, pad);
         if (!kAhead) fk.store(lds_k);
-        fv.template load<VECTORS>(vp + t * a.v.st, sign * (int)a.v.st, a.Dv - dv0, pad);
+        fv.load(vp + t * a.v.st, sign * (int)a.v.st, a.Vp - dv0, pad);
         if (!kAhead) fv.store(lds_v);
-        if (!FOLD) fq.template load<VECTORS>(qp + t * a.q.st, sign * (int)a.q.st, a.Dk, pad);
+        if (!FOLD) fq.load(qp + t * a.q.st, sign * (int)a.q.st, a.Kp, pad);
         if (!kAhead && !FOLD) fq.store(lds_q);
     };
     auto store = [&]() {
@@ -498,7 +488,7 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
                         const int d = dv0 + 32 * wave + 8 * g + 4 * half;
-                        if constexpr (VECTORS) {
+                        if (a.Dv % 4 == 0) {  // (rows of whole fours start at multiples of four)
                             if (d < a.Dv) {
                                 Pack<O, 4> four;
 #pragma unroll
@@ -542,7 +532,7 @@ __device__ __forceinline__ float sum16(f32x16 x) {
     return s;
 }
 
-template <typename T, int DKT, int NW, bool VECTORS>
+template <typename T, int DKT, int NW>
 __global__ __launch_bounds__(64 * NW, DKT == 1 ? 2 : 1) void decay_kernel(const Sweep a, const Sweep back, const View grad, float *partial,
                                                          int slices) {
     constexpr int DK = 32 * DKT, DV = 32 * NW, THREADS = 64 * NW, TERMS = sizeof(T) == 2 ? 3 : 1;
@@ -561,20 +551,22 @@ __global__ __launch_bounds__(64 * NW, DKT == 1 ? 2 : 1) void decay_kernel(const 
     char *const lds_k = lds, *const lds_q = lds + kKBytes, *const lds_v = lds_q + kKBytes, *const lds_o = lds_v + kVBytes;
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, ln = lane & 31;
+    // Rows of the state are dealt to blocks like its columns: every term is a sum over both (inside a chunk, of products of a sum over
+    // rows with one over columns)
     const int slice = blockIdx.x % slices, h = blockIdx.x / slices, piece = blockIdx.y * a.run;
     const int64_t b = blockIdx.z;
-    const int dv0 = slice * DV, dv = dv0 + 32 * wave + ln;
+    const int across = (a.Dv + DV - 1) / DV, dk0 = slice / across * DK, dv0 = slice % across * DV, dv = dv0 + 32 * wave + ln;
     const int64_t n = length_of(a.lengths, b, a.L);
     const auto [begin, end] = range_of(a, n, piece, a.run);
     const float g2 = decay_of(a.log_decay, h) * kLog2e;
 
     f32x16 S[DKT], D[DKT];
-    load_state<DKT, NW, false>(S, a, b, h, n, piece, g2, dv0, dv, half);
+    load_state<DKT, NW, false>(S, a, b, h, n, piece, g2, dk0, dv0, dv, half);
 #pragma unroll
     for (int t = 0; t < DKT; ++t) D[t] = f32x16{};
-    const T *const kp = (const T *)a.k.p + b * a.k.sb + (h / a.k.group) * a.k.sh;
+    const T *const kp = (const T *)a.k.p + b * a.k.sb + (h / a.k.group) * a.k.sh + dk0;
     const T *const vp = (const T *)a.v.p + b * a.v.sb + (h / a.v.group) * a.v.sh + dv0;
-    const T *const qp = (const T *)a.q.p + b * a.q.sb + (h / a.q.group) * a.q.sh;
+    const T *const qp = (const T *)a.q.p + b * a.q.sb + (h / a.q.group) * a.q.sh + dk0;
     const T *const op = (const T *)grad.p + b * grad.sb + (h / grad.group) * grad.sh + dv0;
     const int chunks = (int)((end - begin + C - 1) / C);
     int64_t r0 = end - (int64_t)chunks * C;
@@ -601,13 +593,13 @@ __global__ __launch_bounds__(64 * NW, DKT == 1 ? 2 : 1) void decay_kernel(const 
     Fetch<T, DV, C, THREADS> fv, fo;
     // (where registers do not hold a whole chunk, the tensors pass through them one after the other)
     auto fetch = [&](int64_t at, int pad) {
-        fk.template load<VECTORS>(kp + at * a.k.st, (int)a.k.st, a.Dk, pad);
+        fk.load(kp + at * a.k.st, (int)a.k.st, a.Kp - dk0, pad);
         if (!kAhead) fk.store(lds_k);
-        fq.template load<VECTORS>(qp + at * a.q.st, (int)a.q.st, a.Dk, pad);
+        fq.load(qp + at * a.q.st, (int)a.q.st, a.Kp - dk0, pad);
         if (!kAhead) fq.store(lds_q);
-        fv.template load<VECTORS>(vp + at * a.v.st, (int)a.v.st, a.Dv - dv0, pad);
+        fv.load(vp + at * a.v.st, (int)a.v.st, a.Vp - dv0, pad);
         if (!kAhead) fv.store(lds_v);
-        fo.template load<VECTORS>(op + at * grad.st, (int)grad.st, a.Dv - dv0, pad);
+        fo.load(op + at * grad.st, (int)grad.st, a.Vp - dv0, pad);
         if (!kAhead) fo.store(lds_o);
     };
     auto store = [&]() {
@@ -737,7 +729,7 @@ __global__ __launch_bounds__(64 * NW, DKT == 1 ? 2 : 1) void decay_kernel(const 
     }
     total *= a.out_scale;
     // the gradient of the state behind the piece
-    load_state<DKT, NW, false>(S, back, b, h, n, a.pieces - piece - a.run, g2, dv0, dv, half);
+    load_state<DKT, NW, false>(S, back, b, h, n, a.pieces - piece - a.run, g2, dk0, dv0, dv, half);
 #pragma unroll
     for (int t = 0; t < DKT; ++t) total += sum16(D[t] * S[t]);
 #pragma unroll
@@ -749,60 +741,45 @@ __global__ __launch_bounds__(64 * NW, DKT == 1 ? 2 : 1) void decay_kernel(const 
     partial[(((int64_t)blockIdx.y * slices + slice) * a.B + b) * a.H + h] = (float)total;
 }
 
-// Whole units of 16 bytes everywhere: all rows start at addresses of units, and heads have whole units of channels (a head that
-// ends inside a unit would read its neighbour's channels, or a view's hidden ones).
-bool whole_units(const Sweep &a, int element, bool more = true) {
-    const int E = 16 / element;
-    return more && (a.q.vectors || !a.q.p) && a.k.vectors && a.v.vectors && a.Dk % E == 0 && a.Dv % E == 0 && aligned16(a.out);
-}
-
-template <typename T, int DKT, int NW, int TERMS, bool VECTORS>
+template <typename T, int DKT, int NW, int TERMS>
 void launch_width(const Sweep &a, bool fold, hipStream_t stream) {
     const int slices = (int)ceil_div(a.Dv, 32 * NW);
     const dim3 grid((unsigned)(slices * a.H), (unsigned)(fold ? a.pieces - a.run : a.pieces / a.run), (unsigned)a.B), block(64 * NW);
     if (fold)
-        chunk_kernel<T, T, DKT, NW, TERMS, true, VECTORS><<<grid, block, 0, stream>>>(a, slices);
+        chunk_kernel<T, T, DKT, NW, TERMS, true><<<grid, block, 0, stream>>>(a, slices);
     else if (a.out_float && sizeof(T) == 2)
-        chunk_kernel<T, float, DKT, NW, TERMS, false, VECTORS><<<grid, block, 0, stream>>>(a, slices);
+        chunk_kernel<T, float, DKT, NW, TERMS, false><<<grid, block, 0, stream>>>(a, slices);
     else
-        chunk_kernel<T, T, DKT, NW, TERMS, false, VECTORS><<<grid, block, 0, stream>>>(a, slices);
+        chunk_kernel<T, T, DKT, NW, TERMS, false><<<grid, block, 0, stream>>>(a, slices);
 }
 
 // A state that is handed out in 32 bits is summed from all bits of its terms.  For one that only answers, through a copy in the type
 // of the products, two terms of bf16 are enough; one would be off by as much as the copy is (root mean square of the error of an
 // answer 2.7e-3 of its size with one, 2.3e-3 with two or three, 1.7e-3 of them its own rounding; 16 x 4096 tokens, 16 heads of 128).
-template <typename T, int DKT, int NW, bool VECTORS>
+template <typename T, int DKT, int NW>
 void launch_terms(const Sweep &a, bool fold, hipStream_t stream) {
     if constexpr (sizeof(T) == 2) {
-        if (a.exact_state) return launch_width<T, DKT, NW, 3, VECTORS>(a, fold, stream);
-        return launch_width<T, DKT, NW, 2, VECTORS>(a, fold, stream);
+        if (a.exact_state) return launch_width<T, DKT, NW, 3>(a, fold, stream);
+        launch_width<T, DKT, NW, 2>(a, fold, stream);
+    } else {
+        launch_width<T, DKT, NW, 1>(a, fold, stream);
     }
-    launch_width<T, DKT, NW, 1, VECTORS>(a, fold, stream);
-}
-
-template <typename T, int DKT, int NW>
-void launch_aligned(const Sweep &a, bool fold, hipStream_t stream) {
-    if (whole_units(a, sizeof(T))) return launch_terms<T, DKT, NW, true>(a, fold, stream);
-    launch_terms<T, DKT, NW, false>(a, fold, stream);
 }
 
 template <typename T, int DKT, int NW>
 void launch_decay_width(const Sweep &a, const Sweep &back, const View &grad, float *partial, hipStream_t stream) {
-    const int slices = (int)ceil_div(a.Dv, 32 * NW);
+    const int slices = decay_slices(a);
     const dim3 grid((unsigned)(slices * a.H), (unsigned)(a.pieces / a.run), (unsigned)a.B), block(64 * NW);
-    if (whole_units(a, sizeof(T), grad.vectors))
-        decay_kernel<T, DKT, NW, true><<<grid, block, 0, stream>>>(a, back, grad, partial, slices);
-    else
-        decay_kernel<T, DKT, NW, false><<<grid, block, 0, stream>>>(a, back, grad, partial, slices);
+    decay_kernel<T, DKT, NW><<<grid, block, 0, stream>>>(a, back, grad, partial, slices);
 }
 
 }  // namespace
 
 template <typename T, int DKT>
 void launch_chunks(const Sweep &a, bool fold, hipStream_t stream) {
-    if (a.Dv <= 32) return launch_aligned<T, DKT, 1>(a, fold, stream);
-    if (a.Dv <= 64) return launch_aligned<T, DKT, 2>(a, fold, stream);
-    launch_aligned<T, DKT, 4>(a, fold, stream);
+    if (a.Dv <= 32) return launch_terms<T, DKT, 1>(a, fold, stream);
+    if (a.Dv <= 64) return launch_terms<T, DKT, 2>(a, fold, stream);
+    launch_terms<T, DKT, 4>(a, fold, stream);
 }
 
 template <typename T, int DKT>
@@ -814,8 +791,10 @@ void launch_decay(const Sweep &a, const Sweep &back, const View &grad_out, float
 
 template void launch_chunks<float, PSIG_KEY_TILES>(const Sweep &, bool, hipStream_t);
 template void launch_chunks<bf16, PSIG_KEY_TILES>(const Sweep &, bool, hipStream_t);
+#if PSIG_KEY_TILES <= 4  // (wider states are dealt to blocks by 128 rows)
 template void launch_decay<float, PSIG_KEY_TILES>(const Sweep &, const Sweep &, const View &, float *, hipStream_t);
 template void launch_decay<bf16, PSIG_KEY_TILES>(const Sweep &, const Sweep &, const View &, float *, hipStream_t);
+#endif
 
 }  // namespace seq
 }  // namespace psig

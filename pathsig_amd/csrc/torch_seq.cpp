@@ -30,10 +30,12 @@ void check_like(const Tensor &t, const char *what, const Tensor &like, const cha
     TORCH_CHECK(t.device() == like.device(), what, " must be on the device of ", like_name);
 }
 
-// the channels of a head side by side, and tokens no further apart than the kernels' offsets reach
-Tensor side_by_side(const Tensor &t) {
-    const bool near = t.dim() < 4 || t.size(1) <= 1 || t.stride(1) <= PATHSIG_MAX_TOKEN_STRIDE;
-    return near && (t.size(-1) == 1 || t.stride(-1) == 1) ? t : t.contiguous();
+// The channels of a head side by side, tokens no further apart than the kernels' offsets reach, and a start at a multiple of 16
+// bytes (of sequences, whose rows are read in such units).
+Tensor side_by_side(const Tensor &t, bool sequence) {
+    const bool near = !sequence || t.size(1) <= 1 || t.stride(1) <= PATHSIG_MAX_TOKEN_STRIDE;
+    const Tensor as = near && (t.size(-1) == 1 || t.stride(-1) == 1) ? t : t.contiguous();
+    return sequence && (uintptr_t)ptr(as) % 16 ? as.clone(at::MemoryFormat::Contiguous) : as;
 }
 
 // ---- linear attention ---------------------------------------------------------------------------------------------
@@ -81,9 +83,9 @@ AttentionCall attention_call(const Tensor &q, const Tensor &k, const Tensor &v, 
     check_like(log_decay, "log_decay", q, "q");
     TORCH_CHECK(log_decay.scalar_type() == at::kFloat, "log_decay must be float32");
     TORCH_CHECK(log_decay.dim() == 1 && log_decay.size(0) == a.c.H, "log_decay must be [heads of q]");
-    a.q = side_by_side(q);
-    a.k = side_by_side(k);
-    a.v = side_by_side(v);
+    a.q = side_by_side(q, token);
+    a.k = side_by_side(k, token);
+    a.v = side_by_side(v, token);
     a.log_decay = log_decay.contiguous();
     if (state.defined()) {
         check_like(state, "state", q, "q");
@@ -135,7 +137,7 @@ Gradients attention_backward(const Tensor &grad_out_in, const Tensor &grad_last_
     check_like(grad_out_in, "grad_out", q, "q");
     TORCH_CHECK(grad_out_in.scalar_type() == q.scalar_type(), "grad_out must have same dtype as q");
     TORCH_CHECK(grad_out_in.sizes() == at::IntArrayRef({a.c.B, a.c.L, a.c.H, a.c.Dv}), "grad_out must be [B, L, H, Dv]");
-    Tensor grad_out = grad_out_in.contiguous(), grad_last;
+    Tensor grad_out = side_by_side(grad_out_in.contiguous(), true), grad_last;
     if (grad_last_in.defined()) {
         check_like(grad_last_in, "grad_state", q, "q");
         TORCH_CHECK(grad_last_in.scalar_type() == at::kFloat, "grad_state must be float32");
