@@ -533,7 +533,7 @@ __device__ __forceinline__ float sum16(f32x16 x) {
 }
 
 template <typename T, int DKT, int NW>
-__global__ __launch_bounds__(64 * NW, DKT == 1 ? 2 : 1) void decay_kernel(const Sweep a, const Sweep back, const View grad, float *partial,
+__global__ __launch_bounds__(64 * NW, DKT == 1 || (DKT == 2 && sizeof(T) == 4) ? 2 : 1) void decay_kernel(const Sweep a, const Sweep back, const View grad, float *partial,
                                                          int slices) {
     constexpr int DK = 32 * DKT, DV = 32 * NW, THREADS = 64 * NW, TERMS = sizeof(T) == 2 ? 3 : 1;
     constexpr int CT = chunk_tiles<T>(DKT, NW), C = 32 * CT;

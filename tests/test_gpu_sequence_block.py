@@ -12,6 +12,17 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda"
 
 
+@pytest.fixture(autouse=True)
+def float32_by_default():
+    """Tensors made here without a type are float32, whatever the tests before left as the default."""
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(torch.float32)
+    yield
+    torch.set_default_dtype(before)
+
+
+
+
 class Block(nn.Module):
     def __init__(self, C, H, Dk, Dv, learn_decay):
         super().__init__()

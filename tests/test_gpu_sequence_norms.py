@@ -16,6 +16,17 @@ from tests import sequence_reference as ref
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+
+
+@pytest.fixture(autouse=True)
+def float32_by_default():
+    """Tensors made here without a type are float32, whatever the tests before left as the default."""
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(torch.float32)
+    yield
+    torch.set_default_dtype(before)
+
+
 BF16, F32 = torch.bfloat16, torch.float32
 NAMES = ("x", "weight", "gate", "residual", "scale", "next_weight")
 COLUMNS = ("weight", "scale", "next_weight")
