@@ -200,6 +200,15 @@ struct Fetch {
     }
 };
 
+// What `rounded` leaves of x; nothing of what has no finite remainder
+template <typename T>
+__device__ __forceinline__ Frag<T> remainder(f32x8 x) {
+    f32x8 left = x - widened(rounded<T>(x));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) left[e] = fabsf(left[e]) <= 3.402823466e38f ? left[e] : 0.f;
+    return rounded<T>(left);
+}
+
 // f x in COUNT terms of the type of the products; three of bf16 hold all 24 bits
 template <typename T, int COUNT>
 __device__ __forceinline__ void split_scaled(f32x8 x, const f32x8 &f, Frag<T> (&out)[COUNT]) {
@@ -287,7 +296,8 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
     __shared__ __align__(16) char lds[kKBytes * (FOLD ? 1 : 2) + kVBytes];
     __shared__ __align__(16) f32x4 table_left[CT][4][2], table_later[4][2], table_diagonal[FOLD ? 1 : 4][64];
     // rounded scores as operands, or the parts of a tile's sums
-    __shared__ __align__(16) Frag<T> scores[FOLD || kParts > 1 ? 1 : kTiles][2][64];
+    constexpr int kSecond = CT > 1 ? 0 : 1;  // where their second terms lie (see `brief`)
+    __shared__ __align__(16) Frag<T> scores[FOLD || kParts > 1 ? 1 : kTiles + (sizeof(T) == 2 ? kSecond : 0)][2][64];
     __shared__ __align__(16) f32x4 sums[!FOLD && kParts > 1 ? kParts : 1][4][64];
     char *const lds_k = lds, *const lds_v = lds + kKBytes, *const lds_q = lds_v + kVBytes;
 
@@ -341,6 +351,9 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
     Fetch<T, DV, C, THREADS> fv;
     const int chunks = (int)((max(end - begin, (int64_t)0) + C - 1) / C);
     int64_t r0 = end - (int64_t)chunks * C;  // of the chunk being worked on; before `begin` where the first is not full
+    // Up to 32 tokens: an answer may be one score times one row, whose rounding no sum averages out, so scores have a second term.
+    // They all are in the last tile: the others are skipped, and where there are any the first one's place holds the second terms.
+    const bool brief = !FOLD && sizeof(T) == 2 && end - begin <= 32;
     // (where registers do not hold a whole chunk, the tensors pass through them one after the other)
     auto fetch = [&](int64_t at, int pad) {
         const int64_t t = a.reverse ? n - 1 - at : at;
@@ -395,6 +408,7 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
                 }
             } else {
                 for (int tile = wave; tile < kTiles; tile += NW) {
+                    if (brief && tile < kTiles - 1) continue;
                     const int i = tile > 0, j = tile > 1;
                     f32x16 P = {};
                     const char *const kt = lds_k + j * 32 * KTile::kRow, *const qt = lds_q + i * 32 * KTile::kRow;
@@ -411,6 +425,10 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
                     }
                     scores[tile][0][lane] = rounded<T>(half_of<0>(P));
                     scores[tile][1][lane] = rounded<T>(half_of<1>(P));
+                    if (brief) {
+                        scores[kSecond][0][lane] = remainder<T>(half_of<0>(P));
+                        scores[kSecond][1][lane] = remainder<T>(half_of<1>(P));
+                    }
                 }
             }
             // answers from the state
@@ -474,12 +492,21 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
                         for (int e = 0; e < 4; ++e) P[r4 / 2][r4 % 2 * 4 + e] = acc_row(4 * r4 + e, half) <= ln ? x[e] : 0.f;
                     }
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) out[i] = mma(vt[0][s], rounded<T>(P[s]), out[i]);
+                    for (int s = 0; s < 2; ++s) {
+                        out[i] = mma(vt[0][s], rounded<T>(P[s]), out[i]);
+                        if (brief) out[i] = mma(vt[0][s], remainder<T>(P[s]), out[i]);
+                    }
                 } else {
 #pragma unroll
                     for (int j = 0; j <= i; ++j)
 #pragma unroll
-                        for (int s = 0; s < 2; ++s) out[i] = mma(vt[j][s], scores[i + j][s][lane], out[i]);
+                        for (int s = 0; s < 2; ++s) {
+                            if (brief && j < i)
+                                out[i] = mma(vt[CT - 1][s], scores[0][s][lane], out[i]);
+                            else
+                                out[i] = mma(vt[j][s], scores[i + j][s][lane], out[i]);
+                            if (brief && CT == 1) out[i] = mma(vt[0][s], scores[kSecond][s][lane], out[i]);
+                        }
                 }
                 const int row = 32 * i + ln;
                 if (row >= pad) {

@@ -456,3 +456,31 @@ def test_offsets_past_32_bits():
         err = (out[-1:].float() - want.float())
         assert float(err.square().mean().sqrt()) <= 2 ** -7 * float(want.float().square().mean().sqrt())
         assert (out[:-1] == 0).all()
+
+
+@pytest.mark.parametrize("Dk, Dv", [(18, 10), (64, 128), (128, 20), (128, 128), (256, 24), (256, 128)])
+@pytest.mark.parametrize("L", [1, 2, 7, 32])
+def test_scores_of_a_few_tokens_are_not_rounded_to_the_type(L, Dk, Dv):
+    """bfloat16 answers and gradients of up to 32 tokens without a state are rounded once, at the end: half a step 2^-8 of the
+    value.  With A as above, before that: scores in two terms, 2^-16 A; sums of up to 256 + 32 terms in 32 bits, 2^-15 A; powers
+    of the decay, 2^-20 A: below 2^-14 A together.  (A score rounded to the type would be another 2^-8 |o| off where L is 1.)"""
+    from pathsig_amd import sequence
+    a = _inputs(3, L, 4, 4, Dk, Dv, BF16, seed=60 + L, state=False)
+    leaves = [a[n].detach().requires_grad_(True) for n in ("q", "k", "v")]
+    out = sequence.linear_attention(*leaves, a["g"])
+    out.backward(a["do"])
+    exact = [_double(a[n]) for n in ("q", "k", "v", "g")]
+    do = _double(a["do"])
+    want, size = ref.attention(*exact, do=do), ref.attention_bound(*exact, do=do)
+    for name, got in (("out", out), ("q", leaves[0].grad), ("k", leaves[1].grad), ("v", leaves[2].grad)):
+        key = name if name in want else "d" + name
+        off = (got.detach().double() - want[key]).abs()
+        assert bool((off <= 2.0 ** -8 * want[key].abs() + 2.0 ** -14 * size[key]).all()), (name, off.max().item())
+
+
+def test_an_infinite_score_of_a_few_tokens_stays_infinite():
+    from pathsig_amd import sequence
+    q = torch.full((1, 2, 1, 8), 2.0 ** 127, dtype=BF16, device=DEV)
+    v = torch.ones(1, 2, 1, 8, dtype=BF16, device=DEV)
+    out = sequence.linear_attention(q, q, v, torch.zeros(1, dtype=F32, device=DEV))
+    assert bool(torch.isposinf(out).all())
