@@ -56,6 +56,12 @@ __global__ __launch_bounds__(256) void join_kernel(const Sweep a) {
     }
 }
 
+// The state in front of the first token, for a call that writes the last state over it: with few pieces every block of a sweep reads
+// the first one, in no order with the block that writes the last.
+__global__ void copy_state_kernel(const float *from, float *to, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) to[i] = from[i];
+}
+
 // The parts of a head's gradient, in a fixed order and in 64 bits; a few thousand numbers at most, bound by the launch.
 __global__ void decay_sum_kernel(const float *partial, int64_t rows, int H, float *out) {
     const int h = blockIdx.x;
@@ -371,7 +377,13 @@ int forward_t(const pathsig_linattn *c, const void *q, const void *k, const void
     a.out = out;
     a.out_scale = c->scale;
     a.exact_state = final_state || c->learned_decay;
-    fold<T>(a, (float *)(ws + forward_layout(c).starts), stream);
+    float *const starts = (float *)(ws + forward_layout(c).starts);
+    if (state && state == final_state && a.pieces > 1 && a.pieces <= kJoinInside) {
+        const int64_t n = c->B * c->H * c->Dk * c->Dv;  // the first entry of `starts`, which only more pieces fill
+        copy_state_kernel<<<(unsigned)std::min<int64_t>(ceil_div(n, 256), 4096), 256, 0, stream>>>(state, starts, n);
+        a.first = starts;
+    }
+    fold<T>(a, starts, stream);
     chunks<T>(a, false, stream);
     return launch_status("linear attention");
 }
@@ -550,6 +562,10 @@ int pathsig_linattn_backward(const pathsig_linattn *call, const void *q, const v
     }
     if (grad_log_decay && !call->learned_decay) {
         set_error("grad_log_decay is asked for, but learned_decay is not set");
+        return PATHSIG_ERR_ARGUMENT;
+    }
+    if (grad_state && (grad_state == grad_final_state || grad_state == state)) {
+        set_error("grad_state must not be the buffer of grad_final_state or state, which are read after it is written");
         return PATHSIG_ERR_ARGUMENT;
     }
     if (kept && kept_bytes != forward_layout(call).total) {
