@@ -19,16 +19,19 @@
 // worked on; between the two everything that reads tiles happens; after the second the next chunk's tiles are stored while the
 // answers are finished from registers and scores.
 //
-// Rounding in bf16: scores and the state's copy for the products with V and Q (half a step of bf16 a term, like the rounding of the
-// answers).  The state itself stays in 32 bits, and so does what is added to it: l^(C-1-j) v_j is split into terms of bf16, three of
-// which hold all 24 bits (launch_terms).
+// Rounding in bf16: scores and the state's copy for the products with V and Q are split into two terms of bf16 each, which are off by
+// 2^-16 of them: an answer is rounded once, at its end.  (With one term they are off by as much as that rounding: root mean square
+// of the error 2.35e-3 of the answers against 1.66e-3; a sweep of 16 x 4096 tokens of 16 heads of 128 takes 283 us with one and
+// 325 with two.)  The state itself stays in 32 bits, and so does what is added to it: l^(C-1-j) v_j is split too, three terms hold all
+// 24 bits (launch_terms).
 //
 // A first chunk that is not full is filled from the front with tokens of zeros, so that the factors l^(C-1-j) hold for every
 // chunk and none of them is a quotient.
 //
 // Bound by memory first: 16 x 4096 tokens of 16 heads of 128 in bf16 are 1.07 GB to read and write, 210 us at the rate of a large
-// copy (5.1 TB/s); the sweep takes 290 in two pieces, two blocks to a compute unit with 48 KB each on their way (without loads and
-// stores 150: 46 to 78 matrix instructions and about 400 vector ones a chunk and wave).  In one piece, one block to a unit, 356.
+// copy (5.1 TB/s); the sweep takes 325 in two pieces, two blocks to a compute unit with 48 KB each on their way: 76 to 100 matrix
+// instructions and about 500 vector ones a chunk and wave, which loads and stores do not hide altogether (with scores and the state's
+// copy in one term, 22 matrix instructions less, it was 283, and 150 without loads and stores).
 #include <algorithm>
 
 #include "seq_attention.hpp"
@@ -40,6 +43,7 @@ namespace {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // eight elements of an operand, a lane's share of sixteen steps of the contracted index
@@ -200,16 +204,37 @@ struct Fetch {
     }
 };
 
-// What `rounded` leaves of x; nothing of what has no finite remainder
-template <typename T>
-__device__ __forceinline__ Frag<T> remainder(f32x8 x) {
-    f32x8 left = x - widened(rounded<T>(x));
+// x - hi of eight elements, hi being x rounded: exact, a product with minus one added in 32 bits.  Where hi is infinite or no number
+// the remainder, and that of the element beside it, is zero (the median of NaN, zero and NaN), so that an infinity is not taken
+// from itself.
+__device__ __forceinline__ f32x8 remainder(f32x8 x, bf16x8 hi) {
+    uint32_t low = 0xbf80u, high = 0xbf800000u;  // minus one beside zero
+    asm("" : "+s"(low), "+s"(high));             // (in registers: as an inline constant the compiler puts it into both halves)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) left[e] = fabsf(left[e]) <= 3.402823466e38f ? left[e] : 0.f;
-    return rounded<T>(left);
+    for (int e = 0; e < 8; e += 2) {
+        const bf16x2 pair = {hi[e], hi[e + 1]};
+        x[e] = __builtin_amdgcn_fdot2_f32_bf16(pair, __builtin_bit_cast(bf16x2, low), x[e], false);
+        x[e + 1] = __builtin_amdgcn_fdot2_f32_bf16(pair, __builtin_bit_cast(bf16x2, high), x[e + 1], false);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_fmed3f(x[e], 0.f, x[e]);
+    return x;
 }
 
-// f x in COUNT terms of the type of the products; three of bf16 hold all 24 bits
+// x in COUNT terms of the type of the products; three of bf16 hold all 24 bits
+template <typename T, int COUNT>
+__device__ __forceinline__ void split(f32x8 x, Frag<T> (&out)[COUNT]) {
+    out[0] = rounded<T>(x);
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 1; i < COUNT; ++i) {
+            x = remainder(x, out[i - 1]);
+            out[i] = rounded<T>(x);
+        }
+    }
+}
+
+// f x in terms
 template <typename T, int COUNT>
 __device__ __forceinline__ void split_scaled(f32x8 x, const f32x8 &f, Frag<T> (&out)[COUNT]) {
 #pragma unroll
@@ -295,9 +320,9 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
     constexpr int kKBytes = C * KTile::kRow, kVBytes = C * VTile::kRow;
     __shared__ __align__(16) char lds[kKBytes * (FOLD ? 1 : 2) + kVBytes];
     __shared__ __align__(16) f32x4 table_left[CT][4][2], table_later[4][2], table_diagonal[FOLD ? 1 : 4][64];
-    // rounded scores as operands, or the parts of a tile's sums
-    constexpr int kSecond = CT > 1 ? 0 : 1;  // where their second terms lie (see `brief`)
-    __shared__ __align__(16) Frag<T> scores[FOLD || kParts > 1 ? 1 : kTiles + (sizeof(T) == 2 ? kSecond : 0)][2][64];
+    // scores as operands, in terms, or the parts of a tile's sums
+    constexpr int kTerms = sizeof(T) == 2 ? 2 : 1;
+    __shared__ __align__(16) Frag<T> scores[FOLD || kParts > 1 ? 1 : kTiles][2][kTerms][64];
     __shared__ __align__(16) f32x4 sums[!FOLD && kParts > 1 ? kParts : 1][4][64];
     char *const lds_k = lds, *const lds_v = lds + kKBytes, *const lds_q = lds_v + kVBytes;
 
@@ -351,9 +376,6 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
     Fetch<T, DV, C, THREADS> fv;
     const int chunks = (int)((max(end - begin, (int64_t)0) + C - 1) / C);
     int64_t r0 = end - (int64_t)chunks * C;  // of the chunk being worked on; before `begin` where the first is not full
-    // Up to 32 tokens: an answer may be one score times one row, whose rounding no sum averages out, so scores have a second term.
-    // They all are in the last tile: the others are skipped, and where there are any the first one's place holds the second terms.
-    const bool brief = !FOLD && sizeof(T) == 2 && end - begin <= 32;
     // (where registers do not hold a whole chunk, the tensors pass through them one after the other)
     auto fetch = [&](int64_t at, int pad) {
         const int64_t t = a.reverse ? n - 1 - at : at;
@@ -408,7 +430,6 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
                 }
             } else {
                 for (int tile = wave; tile < kTiles; tile += NW) {
-                    if (brief && tile < kTiles - 1) continue;
                     const int i = tile > 0, j = tile > 1;
                     f32x16 P = {};
                     const char *const kt = lds_k + j * 32 * KTile::kRow, *const qt = lds_q + i * 32 * KTile::kRow;
@@ -423,11 +444,12 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
 #pragma unroll
                         for (int r = 0; r < 16; ++r) P[r] *= table_later[r / 4][half][r % 4] * since;
                     }
-                    scores[tile][0][lane] = rounded<T>(half_of<0>(P));
-                    scores[tile][1][lane] = rounded<T>(half_of<1>(P));
-                    if (brief) {
-                        scores[kSecond][0][lane] = remainder<T>(half_of<0>(P));
-                        scores[kSecond][1][lane] = remainder<T>(half_of<1>(P));
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        Frag<T> terms[kTerms];
+                        split<T>(s ? half_of<1>(P) : half_of<0>(P), terms);
+#pragma unroll
+                        for (int e = 0; e < kTerms; ++e) scores[tile][s][e][lane] = terms[e];
                     }
                 }
             }
@@ -436,9 +458,15 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
             for (int i = 0; i < CT; ++i) out[i] = f32x16{};
 #pragma unroll
             for (int kk = 0; kk < DK / 16; ++kk) {
-                const Frag<T> st = rounded<T>(kk % 2 ? half_of<1>(S[kk / 2]) : half_of<0>(S[kk / 2]));
+                Frag<T> st[kTerms];
+                split<T>(kk % 2 ? half_of<1>(S[kk / 2]) : half_of<0>(S[kk / 2]), st);
+                Frag<T> q[CT];
 #pragma unroll
-                for (int i = 0; i < CT; ++i) out[i] = mma(st, KTile::row(lds_q, row_base, i, kk), out[i]);
+                for (int i = 0; i < CT; ++i) q[i] = KTile::row(lds_q, row_base, i, kk);
+#pragma unroll
+                for (int e = 0; e < kTerms; ++e)
+#pragma unroll
+                    for (int i = 0; i < CT; ++i) out[i] = mma(st[e], q[i], out[i]);
             }
         }
 
@@ -493,20 +521,18 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
                     }
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
-                        out[i] = mma(vt[0][s], rounded<T>(P[s]), out[i]);
-                        if (brief) out[i] = mma(vt[0][s], remainder<T>(P[s]), out[i]);
+                        Frag<T> terms[kTerms];
+                        split<T>(P[s], terms);
+#pragma unroll
+                        for (int e = 0; e < kTerms; ++e) out[i] = mma(vt[0][s], terms[e], out[i]);
                     }
                 } else {
 #pragma unroll
                     for (int j = 0; j <= i; ++j)
 #pragma unroll
-                        for (int s = 0; s < 2; ++s) {
-                            if (brief && j < i)
-                                out[i] = mma(vt[CT - 1][s], scores[0][s][lane], out[i]);
-                            else
-                                out[i] = mma(vt[j][s], scores[i + j][s][lane], out[i]);
-                            if (brief && CT == 1) out[i] = mma(vt[0][s], scores[kSecond][s][lane], out[i]);
-                        }
+                        for (int s = 0; s < 2; ++s)
+#pragma unroll
+                            for (int e = 0; e < kTerms; ++e) out[i] = mma(vt[j][s], scores[i + j][s][e][lane], out[i]);
                 }
                 const int row = 32 * i + ln;
                 if (row >= pad) {
@@ -780,9 +806,8 @@ void launch_width(const Sweep &a, bool fold, hipStream_t stream) {
         chunk_kernel<T, T, DKT, NW, TERMS, false><<<grid, block, 0, stream>>>(a, slices);
 }
 
-// A state that is handed out in 32 bits is summed from all bits of its terms.  For one that only answers, through a copy in the type
-// of the products, two terms of bf16 are enough; one would be off by as much as the copy is (root mean square of the error of an
-// answer 2.7e-3 of its size with one, 2.3e-3 with two or three, 1.7e-3 of them its own rounding; 16 x 4096 tokens, 16 heads of 128).
+// A state that is handed out in 32 bits is summed from all bits of its terms.  For one that only answers, through a copy in two terms of
+// the type of the products, two terms of bf16 are enough; one would be off by as much as the rounding of an answer is.
 template <typename T, int DKT, int NW>
 void launch_terms(const Sweep &a, bool fold, hipStream_t stream) {
     if constexpr (sizeof(T) == 2) {

@@ -7,7 +7,8 @@ import ctypes
 import pytest
 import torch
 
-from tests.test_gpu_sequence_attention import _inputs
+from tests import sequence_reference as ref
+from tests.test_gpu_sequence_attention import _double, _inputs, _run
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -73,3 +74,25 @@ def test_last_state_over_the_first(shape, pieces, dtype):
     # what a backward takes over is the same: the states in front of the second piece and all that follow
     state = 4 * both.numel()
     assert torch.equal(ws_both[state:_pieces(lib, c) * state], ws[state:_pieces(lib, c) * state])
+
+
+# ---- precision ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("shape", [
+    # B, L, H, Hkv, Dk, Dv
+    (2, 33, 2, 1, 24, 40), (2, 64, 2, 2, 128, 128), (2, 65, 4, 2, 64, 128), (3, 100, 2, 2, 18, 10), (2, 130, 2, 2, 128, 20),
+    (1, 700, 4, 2, 128, 128), (2, 200, 2, 1, 256, 24), (2, 90, 2, 2, 256, 200), (2, 40, 2, 1, 64, 16), (2, 300, 2, 1, 32, 32)])
+def test_scores_and_states_in_bfloat16_keep_two_terms(shape):
+    """bfloat16 answers and gradients are rounded once, at the end: half a step 2^-8 of the value.  With A the sum of the absolute values
+    of the terms, before that: scores, the copy of the state and what is added to the state in two terms, 2^-16 A each, below
+    2^-14 A together with what the last rounding makes of it; sums in 32 bits and powers of the decay as for float32,
+    2^-24 (2 L + Dk + 64) A."""
+    a = _inputs(*shape, BF16, seed=300)
+    args = [_double(a[n]) for n in ("q", "k", "v", "g", "s0")] + [None, None, _double(a["do"]), _double(a["ds"])]
+    want, bound = ref.attention(*args), ref.attention_bound(*args)
+    got = _run(a)
+    for n in ("out", "dq", "dk", "dv"):
+        off = (got[n].double() - want[n]).abs()
+        tol = 2 ** -8 * want[n].abs() + (2 ** -14 + 2 ** -24 * (2 * shape[1] + max(shape[4:]) + 64)) * bound[n]
+        assert (off <= tol).all(), (n, float((off / tol).max()))
+        if off.numel() > 2000:  # a rounding to the nearest alone: steps of 2^-7 at most, a third of whose half squared is the mean
+            assert float(off.square().mean().sqrt()) <= 12 ** -0.5 * 2 ** -7 * float(want[n].square().mean().sqrt()), n
