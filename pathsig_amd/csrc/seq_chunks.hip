@@ -239,11 +239,7 @@ template <typename T, int COUNT>
 __device__ __forceinline__ void split_scaled(f32x8 x, const f32x8 &f, Frag<T> (&out)[COUNT]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] *= f[e];
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i) {
-        out[i] = rounded<T>(x);
-        if (i + 1 < COUNT) x -= widened(out[i]);
-    }
+    split<T>(x, out);
 }
 
 // Bytes that a thread fetches of a chunk of 32 tiles tokens.

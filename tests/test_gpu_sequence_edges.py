@@ -96,3 +96,16 @@ def test_scores_and_states_in_bfloat16_keep_two_terms(shape):
         assert (off <= tol).all(), (n, float((off / tol).max()))
         if off.numel() > 2000:  # a rounding to the nearest alone: steps of 2^-7 at most, a third of whose half squared is the mean
             assert float(off.square().mean().sqrt()) <= 12 ** -0.5 * 2 ** -7 * float(want[n].square().mean().sqrt()), n
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_an_infinite_value_stays_infinite_in_the_state(dtype):
+    from pathsig_amd import sequence
+    a = _inputs(2, 150, 2, 1, 24, 40, dtype, seed=310)
+    a["k"] = torch.where(a["k"] == 0, torch.ones_like(a["k"]), a["k"])
+    a["v"][0, 20, 0, 3], a["v"][0, 149, 0, 5], a["v"][1, 70, 0, 0] = float("inf"), float("-inf"), float("inf")
+    _, last = sequence.linear_attention(a["q"], a["k"], a["v"], torch.full((2,), -0.01, device=DEV), state=a["s0"], return_state=True)
+    want = torch.isinf(torch.zeros_like(last))
+    want[0, :, :, 3] = want[0, :, :, 5] = want[1, :, :, 0] = True
+    assert torch.equal(torch.isinf(last), want) and not last.isnan().any()
+    assert torch.equal(last[0, :, :, 5] > 0, (a["k"][0, 149] < 0).expand(2, 24))
