@@ -5,6 +5,8 @@
 #include <tuple>
 #include <vector>
 
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
+
 #include "torch_common.hpp"
 
 namespace psig_torch {
@@ -596,4 +598,7 @@ TORCH_LIBRARY_IMPL(pathsig, Autograd, m) {
     m.impl("linear_attention", &psig_torch::linear_attention_autograd);
     m.impl("linear_attention_step", &psig_torch::linear_attention_step_autograd);
     m.impl("norm_join", &psig_torch::norm_join_autograd);
+    // (without these, a gradient of a gradient would go on without their part of it, with a warning alone)
+    m.impl("linear_attention_backward", torch::autograd::autogradNotImplementedFallback());
+    m.impl("norm_join_backward", torch::autograd::autogradNotImplementedFallback());
 }

@@ -109,3 +109,22 @@ def test_an_infinite_value_stays_infinite_in_the_state(dtype):
     want[0, :, :, 3] = want[0, :, :, 5] = want[1, :, :, 0] = True
     assert torch.equal(torch.isinf(last), want) and not last.isnan().any()
     assert torch.equal(last[0, :, :, 5] > 0, (a["k"][0, 149] < 0).expand(2, 24))
+
+
+# ---- gradients ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gradients_of_gradients_are_refused(dtype):
+    """A penalty on a gradient, which reaches the leaves through the output as well; a graph that nobody goes back through changes
+    nothing."""
+    from pathsig_amd import sequence
+    a = _inputs(2, 40, 2, 1, 16, 24, dtype, seed=320)
+    leaves = [a[n].requires_grad_(True) for n in ("q", "k", "v", "g", "s0")]
+    x, w = a["q"].detach().requires_grad_(True), torch.ones(16, device=DEV, requires_grad=True)
+    for out, of in ((sequence.linear_attention(*leaves[:4], state=leaves[4]), leaves), (sequence.norm_before(x, w), (x, w))):
+        plain = torch.autograd.grad(out.float().sum(), of, retain_graph=True)
+        grads = torch.autograd.grad(out.float().sum(), of, create_graph=True)
+        for one, other in zip(plain, grads):
+            assert torch.equal(one, other)
+        for grad in grads:
+            with pytest.raises(RuntimeError, match="not implemented"):
+                (out.float().sum() + grad.float().pow(2).sum()).backward(retain_graph=True)

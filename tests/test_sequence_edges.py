@@ -1,11 +1,13 @@
-"""Sequence operators at the edges of what their documents allow, without a GPU: buffers that a call of the C ABI must not share."""
+"""Sequence operators at the edges of what their documents allow, without a GPU: buffers that a call of the C ABI must not share,
+gradients of gradients."""
 from __future__ import annotations
 
 import ctypes
 
 import pytest
+import torch
 
-from pathsig_amd import _load
+from pathsig_amd import _load, sequence
 
 ERR_ARG = -1
 
@@ -31,3 +33,35 @@ def test_gradient_of_the_state_over_what_is_read(lib, state, above):
     rc = lib.pathsig_linattn_backward(ctypes.byref(_attention()), 256, 256, 256, state, None, 0, 256, above, 256, 256, 256, None, 512, None, 0,
                                       None)
     assert rc == ERR_ARG and b"grad_state" in lib.pathsig_last_error()
+
+
+def _meta(*shape):
+    return torch.empty(*shape, device="meta", requires_grad=True)
+
+
+def _attention_out():
+    q, k, v, g, s = _meta(2, 5, 4, 8), _meta(2, 5, 2, 8), _meta(2, 5, 2, 12), _meta(4), _meta(2, 4, 8, 12)
+    return (q, k, v, g, s), sequence.linear_attention(q, k, v, g, state=s)
+
+
+def _after_out():
+    x, w, gate, r, s, nw = _meta(6, 16), _meta(16), _meta(6, 16), _meta(6, 16), _meta(16), _meta(16)
+    return (x, w, gate, s, nw, r), sequence.norm_after(x, w, gate=gate, residual=r, scale=s, next_weight=nw)[1]
+
+
+def _before_out():
+    x, w = _meta(6, 16), _meta(16)
+    return (x, w), sequence.norm_before(x, w)
+
+
+@pytest.mark.parametrize("make", [_attention_out, _after_out, _before_out])
+def test_gradients_of_gradients_are_refused(make):
+    """A penalty on a gradient, which reaches the leaves through the output as well."""
+    leaves, out = make()
+    grads = torch.autograd.grad(out.sum(), leaves, create_graph=True)
+    for grad in grads:
+        penalty = out.sum() + grad.pow(2).sum()
+        with pytest.raises(RuntimeError, match="not implemented"):
+            penalty.backward(retain_graph=True)
+    leaves, out = make()
+    assert not any(grad.requires_grad for grad in torch.autograd.grad(out.sum(), leaves))
