@@ -154,9 +154,14 @@ Gradients attention_backward(const Tensor &grad_out_in, const Tensor &grad_last_
                                : at::empty({0}, a.log_decay.options());
     const size_t ws_bytes = pathsig_linattn_backward_workspace(&a.c, want_decay);
     Tensor ws = scratch(ws_bytes, a.q);
-    check_rc(pathsig_linattn_backward(&a.c, ptr(a.q), ptr(a.k), ptr(a.v), (const float *)ptr(a.state), ptr(kept),
-                                      kept.defined() ? (size_t)kept.numel() : 0, ptr(grad_out), (const float *)ptr(grad_last), ptr(dq), ptr(dk), ptr(dv), (float *)ptr(ddecay),
-                                      (float *)ptr(dstate), ptr(ws), ws_bytes, stream_of(a.q)));
+    // The forward's workspace holds copies of q, k and v where they did not lie in whole units.  Hooks on saved tensors may hand them
+    // back in other strides: a workspace that is not this call's is left, and worked out again.
+    const size_t kept_bytes = pathsig_linattn_forward_workspace(&a.c);
+    const bool use = kept.defined() && kept.is_contiguous() && (size_t)kept.nbytes() == kept_bytes && kept.device() == q.device() &&
+                     (uintptr_t)ptr(kept) % 16 == 0;
+    check_rc(pathsig_linattn_backward(&a.c, ptr(a.q), ptr(a.k), ptr(a.v), (const float *)ptr(a.state), use ? ptr(kept) : nullptr,
+                                      use ? kept_bytes : 0, ptr(grad_out), (const float *)ptr(grad_last), ptr(dq), ptr(dk), ptr(dv),
+                                      (float *)ptr(ddecay), (float *)ptr(dstate), ptr(ws), ws_bytes, stream_of(a.q)));
     return {dq, dk, dv, ddecay, dstate};
 }
 

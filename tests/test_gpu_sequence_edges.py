@@ -128,3 +128,30 @@ def test_gradients_of_gradients_are_refused(dtype):
         for grad in grads:
             with pytest.raises(RuntimeError, match="not implemented"):
                 (out.float().sum() + grad.float().pow(2).sum()).backward(retain_graph=True)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("L", [40, 500])
+def test_hooks_that_hand_saved_tensors_back_in_other_strides(L, dtype):
+    """Views of a projection whose rows are no whole units of 16 bytes are copied by the forward; activations that were kept on the
+    host come back contiguous, with rows of whole units, and need no copy."""
+    from pathsig_amd import sequence
+    B, H, Dk, Dv = 2, 2, 16, 24
+    a = _inputs(B, L, H, H, Dk, Dv, dtype, seed=330)
+    wide = torch.cat([a[n].flatten(2) for n in ("q", "k", "v")] + [torch.zeros(B, L, 3, dtype=dtype, device=DEV)], dim=-1)
+    q, k, v, _ = wide.requires_grad_(True).split((H * Dk, H * Dk, H * Dv, 3), dim=-1)
+    g, s0 = a["g"].requires_grad_(True), a["s0"].requires_grad_(True)
+
+    def gradients():
+        out, last = sequence.linear_attention(*(t.unflatten(-1, (H, -1)) for t in (q, k, v)), g, state=s0, return_state=True)
+        return torch.autograd.grad((out, last), (wide, g, s0), (a["do"], a["ds"]), retain_graph=True)
+    want = gradients()
+    for hooks in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.save_on_cpu(pin_memory=True),
+                  torch.autograd.graph.saved_tensors_hooks(lambda t: t.contiguous(), lambda t: t),
+                  # no unit of the workspace at its place
+                  torch.autograd.graph.saved_tensors_hooks(
+                      lambda t: torch.cat([t.flatten()[:1], t.flatten()])[1:].view(t.shape) if t.numel() else t, lambda t: t)):
+        with hooks:
+            got = gradients()
+        for one, other in zip(got, want):
+            assert torch.equal(one, other)
