@@ -106,7 +106,8 @@ def _wants_grad(*tensors) -> bool:
 # ------------------------------------------------------------------------------------------------
 class LinearAttention(nn.Module):
     """`linear_attention` with the decays of its heads: exp(log_decay) = 1 - 2^-e with e spread evenly over [first, last] (the
-    memory of a head is about 2^e tokens), or as given.  `learn_decay` makes them a parameter."""
+    memory of a head is about 2^e tokens), or as given.  `learn_decay` makes them a parameter.  They stay float32 where the module
+    is converted to another type."""
 
     def __init__(self, *, num_heads: int, log_decay=None, decay_exponents=(2.0, 9.0), learn_decay: bool = False, scale=None):
         super().__init__()
@@ -126,6 +127,17 @@ class LinearAttention(nn.Module):
             self.log_decay = nn.Parameter(log_decay)
         else:
             self.register_buffer("log_decay", log_decay)
+
+    def _apply(self, fn, recurse=True):
+        # (a slow decay in bfloat16 would be none: 1 - 2^-9 rounds to 1)
+        decays = (self.log_decay, self.log_decay.grad)
+
+        def keep_float(t):
+            new = fn(t)
+            if new.dtype == t.dtype or not any(t is d for d in decays):
+                return new
+            return t.to(new.device)
+        return super()._apply(keep_float, recurse)
 
     def forward(self, q, k, v, *, state=None, lengths=None, return_state=False):
         return linear_attention(q, k, v, self.log_decay, state=state, lengths=lengths, scale=self.scale,

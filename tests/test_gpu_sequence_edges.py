@@ -155,3 +155,27 @@ def test_hooks_that_hand_saved_tensors_back_in_other_strides(L, dtype):
             got = gradients()
         for one, other in zip(got, want):
             assert torch.equal(one, other)
+
+
+# ---- modules ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("learn", [False, True])
+def test_a_whole_block_converted_to_bfloat16(learn):
+    """The block of test_gpu_sequence_block.py converted as models are, decays and all: what converting its other parts one by one
+    gives, in training and token by token."""
+    import copy
+    from tests.test_gpu_sequence_block import Block
+    torch.manual_seed(5)
+    parts = Block(64, 4, 16, 16, learn)
+    whole = copy.deepcopy(parts).to(BF16)
+    for m in (parts.before, parts.project, parts.heads, parts.join, parts.after):
+        m.to(BF16)
+    x = torch.randn(2, 80, 64, device=DEV).to(BF16)
+    results = []
+    for block in (whole, parts):
+        assert block.attend.log_decay.dtype == F32
+        out, normed, last = block(x)
+        grads = torch.autograd.grad(out.float().sum() + normed.float().square().sum() + last.sum(), list(block.parameters()))
+        with torch.no_grad():
+            results.append([out, normed, last, *grads, *block.step(x[:, 0], last.clone())])
+    for one, other in zip(*results):
+        assert one.dtype == other.dtype and torch.equal(one, other)

@@ -1,5 +1,5 @@
 """Sequence operators at the edges of what their documents allow, without a GPU: buffers that a call of the C ABI must not share,
-gradients of gradients."""
+gradients of gradients, modules in other types."""
 from __future__ import annotations
 
 import ctypes
@@ -65,3 +65,32 @@ def test_gradients_of_gradients_are_refused(make):
             penalty.backward(retain_graph=True)
     leaves, out = make()
     assert not any(grad.requires_grad for grad in torch.autograd.grad(out.sum(), leaves))
+
+
+@pytest.mark.parametrize("learn", [False, True])
+def test_decays_stay_float32_in_a_module_of_another_type(learn):
+    """Conversions of a whole model leave the decays' values and type alone, alone or within another module, and their gradient."""
+    class OnTheHost(sequence.LinearAttention):
+        def __init__(self):
+            torch.nn.Module.__init__(self)
+            self.num_heads, self.scale = 3, None
+            self.inner = torch.nn.Linear(4, 4)
+            if learn:
+                self.log_decay = torch.nn.Parameter(torch.tensor([-0.5, -2.0 ** -9, -1e-5]))
+                self.log_decay.grad = torch.tensor([1.0, 1 + 2.0 ** -20, 3.0])
+            else:
+                self.register_buffer("log_decay", torch.tensor([-0.5, -2.0 ** -9, -1e-5]))
+
+    for convert in (lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.to("cpu", torch.float64),
+                    lambda m: m.type(torch.bfloat16), lambda m: m.float(), lambda m: m.bfloat16().float()):
+        attend, other = OnTheHost(), torch.nn.Linear(4, 4)
+        want, leaf = attend.log_decay.detach().clone(), attend.log_decay
+        convert(torch.nn.Sequential(other, attend))
+        assert attend.log_decay.dtype == torch.float32 and torch.equal(attend.log_decay, want)
+        assert attend.inner.weight.dtype == other.weight.dtype
+        assert ("log_decay" in dict(attend.named_parameters())) == learn and "log_decay" in attend.state_dict()
+        if learn:
+            assert attend.log_decay is leaf
+            assert attend.log_decay.grad.dtype == torch.float32 and float(attend.log_decay.grad[1]) == 1 + 2.0 ** -20
+    attend = OnTheHost().to("meta", torch.bfloat16)
+    assert attend.log_decay.device.type == "meta" and attend.log_decay.dtype == torch.float32
