@@ -431,8 +431,10 @@ struct NormFunction : public torch::autograd::Function<NormFunction<DIRECT>> {
             std::tie(out, next, stats) = op.call(x, maybe_weight, maybe_gate, maybe_residual, maybe_scale, maybe_next_weight, eps,
                                                  activation, true);
         }
-        // (the residual is only read again where the second norm's input is rebuilt)
-        ctx->save_for_backward({x, weight, gate, residual, scale, next_weight, stats});
+        // The residual is read again where the second norm's input is rebuilt.  Without that norm its gradient is the one from above,
+        // and it may change after the call.
+        ctx->save_for_backward({x, weight, gate, next_weight.defined() ? residual : Tensor(), scale, next_weight, stats});
+        ctx->saved_data["residual"] = residual.defined();
         ctx->saved_data["eps"] = eps;
         ctx->saved_data["activation"] = activation;
         ctx->set_materialize_grads(false);
@@ -464,9 +466,11 @@ struct NormFunction : public torch::autograd::Function<NormFunction<DIRECT>> {
             g = op.call(or_none(grad_out), or_none(grad_next), s[0], or_none(s[1]), or_none(s[2]), or_none(s[3]), or_none(s[4]),
                         or_none(s[5]), s[6], eps, activation);
         }
-        const Tensor all[] = {std::get<0>(g), std::get<1>(g), std::get<2>(g), std::get<3>(g), std::get<4>(g), std::get<5>(g)};
+        const bool residual = ctx->saved_data["residual"].toBool();
+        const Tensor all[] = {std::get<0>(g), std::get<1>(g), std::get<2>(g), s[3].defined() ? std::get<3>(g) : grad_out, std::get<4>(g),
+                              std::get<5>(g)};
         for (int i = 0, present = 0; i < 6; ++i)  // (autograd counts the inputs that are there)
-            if (s[i].defined() && ctx->needs_input_grad(present++)) out[i] = all[i];
+            if ((i == 3 ? residual : s[i].defined()) && ctx->needs_input_grad(present++)) out[i] = all[i];
         return out;
     }
 };

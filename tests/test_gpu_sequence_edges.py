@@ -179,3 +179,39 @@ def test_a_whole_block_converted_to_bfloat16(learn):
             results.append([out, normed, last, *grads, *block.step(x[:, 0], last.clone())])
     for one, other in zip(*results):
         assert one.dtype == other.dtype and torch.equal(one, other)
+
+
+# ---- norms --------------------------------------------------------------------------------------------------------
+def _norm_inputs(dtype, *shape):
+    g = torch.Generator().manual_seed(400)
+    make = lambda *s: torch.randn(*s, generator=g).to(DEV, dtype).requires_grad_(True)  # noqa: E731
+    return {"x": make(*shape), "gate": make(*shape), "residual": make(*shape), "weight": make(shape[-1]), "scale": make(shape[-1])}
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_residual_that_changes_after_the_call(dtype):
+    """Without a second norm the backward does not read the residual: a stream of features may be added to in place."""
+    from pathsig_amd import sequence
+    a = _norm_inputs(dtype, 5, 96)
+    up = torch.randn(5, 96, device=DEV).to(dtype)
+    x, rest = a["x"], {n: a[n] for n in ("gate", "residual", "scale")}
+    want = torch.autograd.grad(sequence.norm_after(x, a["weight"], **rest), (x, *rest.values(), a["weight"]), up)
+    assert torch.equal(want[2], up)
+    stream = a["residual"] * 1
+    out = sequence.norm_after(x, a["weight"], gate=a["gate"], residual=stream, scale=a["scale"])
+    with torch.no_grad():
+        stream.add_(1)
+    got = torch.autograd.grad(out, (x, a["gate"], a["residual"], a["scale"], a["weight"]), up)
+    for one, other in zip(got, want):
+        assert torch.equal(one, other)
+    # with a second norm it does, and autograd says so
+    stream = a["residual"] * 1
+    out, nxt = sequence.norm_after(x, a["weight"], residual=stream, next_weight=a["weight"])
+    with torch.no_grad():
+        stream.add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(nxt, x, up)
+    # a residual of fewer axes: the sum over the rows
+    one = a["residual"][0].detach().requires_grad_(True)
+    (got,) = torch.autograd.grad(sequence.norm_after(x, residual=one), one, up)
+    assert got.shape == one.shape and torch.equal(got, up.sum(0))
