@@ -279,7 +279,8 @@ int pathsig_linattn_forward(const pathsig_linattn *call, const void *q, const vo
  * states between pieces of long sequences, copies), or NULL, and the backward works it out again.
  *   grad_out is a dense [B, L, H, Dv], grad_final_state [B, H, Dk, Dv] float32 or NULL (zero).
  *   grad_q [B, L, H, Dk], grad_k [B, L, Hkv, Dk], grad_v [B, L, Hkv, Dv] dense, in the type of q (sums over the heads that share
- *   a key); grad_log_decay [H] and grad_state [B, H, Dk, Dv] float32, each NULL where it is not wanted.  No gradient that is written
+ *   a key); grad_log_decay [H] and grad_state [B, H, Dk, Dv] float32; each NULL where it is not wanted, and then not worked out
+ *   (grad_state comes with grad_v, from one sweep).  No gradient that is written
  *   may lie over a buffer that is read (grad_state over grad_final_state or state is refused).
  */
 size_t pathsig_linattn_backward_workspace(const pathsig_linattn *call, int want_log_decay);

@@ -413,6 +413,16 @@ BackwardLayout backward_layout(const pathsig_linattn *c, bool want_decay) {
     return l;
 }
 
+// the same states with rows and columns exchanged, for the answers of a sweep alone
+Sweep transposed(Sweep a) {
+    std::swap(a.Dk, a.Dv);
+    std::swap(a.Kp, a.Vp);
+    std::swap(a.row, a.column);
+    a.last = nullptr;
+    a.exact_state = 0;
+    return a;
+}
+
 template <typename T>
 int backward_t(const pathsig_linattn *c, const void *q, const void *k, const void *v, const float *state, const char *kept,
                const void *grad_out, const float *grad_final, void *grad_q, void *grad_k, void *grad_v, float *grad_decay,
@@ -438,19 +448,17 @@ int backward_t(const pathsig_linattn *c, const void *q, const void *k, const voi
     forward.exact_state = grad_decay != nullptr;
     if (kept)
         forward.starts = (float *)from_forward;
-    else
+    else if (grad_q || grad_decay)
         fold<T>(forward, (float *)from_forward, stream);
     // dq: the forward with (do, v, k) and the transposed states
-    Sweep a = forward;
-    std::swap(a.Dk, a.Dv);
-    std::swap(a.Kp, a.Vp);
-    a.q = vdo;
-    a.k = vv;
-    a.v = vk;
-    std::swap(a.row, a.column);
-    a.out = grad_q;
-    a.exact_state = 0;
-    chunks<T>(a, false, stream);
+    if (grad_q) {
+        Sweep a = transposed(forward);
+        a.q = vdo;
+        a.k = vv;
+        a.v = vk;
+        a.out = grad_q;
+        chunks<T>(a, false, stream);
+    }
     // dv: backwards in time with (k, q, do)
     Sweep back = sweep_of(c);
     back.q = vk;
@@ -463,29 +471,27 @@ int backward_t(const pathsig_linattn *c, const void *q, const void *k, const voi
     back.out_float = group > 1;
     back.out = group > 1 ? (void *)(ws + l.wide_v) : grad_v;
     back.exact_state = grad_state || grad_decay;
-    fold<T>(back, (float *)(ws + l.ends), stream);
-    back.exact_state = grad_state != nullptr;
-    chunks<T>(back, false, stream);
+    if (grad_k || grad_v || grad_state || grad_decay) fold<T>(back, (float *)(ws + l.ends), stream);
+    const int64_t rows = c->B * c->L;
+    auto sum_heads = [&](size_t wide, void *out, int64_t D) {
+        if (group == 1 || rows == 0) return;
+        const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(rows * c->Hkv * D, 256), 4096);
+        group_sum_kernel<T><<<blocks, 256, 0, stream>>>((const float *)(ws + wide), (T *)out, rows, (int)c->Hkv, (int)group, (int)D);
+    };
+    if (grad_v || grad_state) {
+        back.exact_state = grad_state != nullptr;
+        chunks<T>(back, false, stream);
+        sum_heads(l.wide_v, grad_v, c->Dv);
+    }
     // dk: backwards in time with (v, do, q), from the same states, transposed
-    a = back;
-    std::swap(a.Dk, a.Dv);
-    std::swap(a.Kp, a.Vp);
-    a.q = vv;
-    a.k = vdo;
-    a.v = vq;
-    std::swap(a.row, a.column);
-    a.last = nullptr;
-    a.out = group > 1 ? (void *)(ws + l.wide_k) : grad_k;
-    a.exact_state = 0;
-    chunks<T>(a, false, stream);
-    if (group > 1) {
-        const int64_t rows = c->B * c->L;
-        const unsigned blocks_k = (unsigned)std::min<int64_t>(ceil_div(rows * c->Hkv * c->Dk, 256), 4096);
-        const unsigned blocks_v = (unsigned)std::min<int64_t>(ceil_div(rows * c->Hkv * c->Dv, 256), 4096);
-        if (rows > 0) {
-            group_sum_kernel<T><<<blocks_k, 256, 0, stream>>>((const float *)(ws + l.wide_k), (T *)grad_k, rows, (int)c->Hkv, (int)group, (int)c->Dk);
-            group_sum_kernel<T><<<blocks_v, 256, 0, stream>>>((const float *)(ws + l.wide_v), (T *)grad_v, rows, (int)c->Hkv, (int)group, (int)c->Dv);
-        }
+    if (grad_k) {
+        Sweep a = transposed(back);
+        a.q = vv;
+        a.k = vdo;
+        a.v = vq;
+        a.out = group > 1 ? (void *)(ws + l.wide_k) : grad_k;
+        chunks<T>(a, false, stream);
+        sum_heads(l.wide_k, grad_k, c->Dk);
     }
     if (grad_decay) {
         decay<T>(forward, back, vdo, (float *)(ws + l.decay), stream);
@@ -556,8 +562,12 @@ int pathsig_linattn_backward(const pathsig_linattn *call, const void *q, const v
                              void *grad_k, void *grad_v, float *grad_log_decay, float *grad_state, void *workspace,
                              size_t workspace_bytes, void *stream) {
     if (const int rc = check_call(call)) return rc;
-    if (call->B > 0 && call->L > 0 && (!q || !k || !v || !grad_out || !grad_q || !grad_k || !grad_v)) {
-        set_error("q, k, v, grad_out, grad_q, grad_k and grad_v must not be NULL");
+    if (call->B > 0 && call->L > 0 && (!q || !k || !v || !grad_out)) {
+        set_error("q, k, v and grad_out must not be NULL");
+        return PATHSIG_ERR_ARGUMENT;
+    }
+    if (call->B > 0 && call->L > 0 && grad_state && !grad_v) {
+        set_error("grad_state comes with grad_v, which must not be NULL");
         return PATHSIG_ERR_ARGUMENT;
     }
     if (grad_log_decay && !call->learned_decay) {

@@ -1,6 +1,7 @@
 // Registration of the sequence operators (linear attention with decays, norms before and after a block) with the torch
 // dispatcher: schemas, argument checks, device implementations over the C ABI of pathsig_hip.h, autograd nodes, and the
 // functions that plain eager calls take past the dispatcher.  They have no counterpart in the reference.
+#include <array>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -129,13 +130,17 @@ std::tuple<Tensor, Tensor, Tensor> attention_forward(const Tensor &q, const Tens
 
 using Gradients = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
 
-// the gradients of log_decay and state are empty tensors where they are not wanted
+// which gradients are asked for; empty tensors stand for the others
+struct Wanted {
+    bool q = true, k = true, v = true, decay = false, state = false;
+};
+
 Gradients attention_backward(const Tensor &grad_out_in, const Tensor &grad_last_in, const Tensor &q, const Tensor &k,
                              const Tensor &v, const Tensor &log_decay, const Tensor &state, const Tensor &lengths,
-                             const Tensor &kept, double scale, bool want_decay, bool want_state) {
+                             const Tensor &kept, double scale, const Wanted &want) {
     c10::DeviceGuard guard(q.device());
     AttentionCall a = attention_call(q, k, v, log_decay, state, lengths, scale, true);
-    a.c.learned_decay = want_decay;
+    a.c.learned_decay = want.decay;
     check_like(grad_out_in, "grad_out", q, "q");
     TORCH_CHECK(grad_out_in.scalar_type() == q.scalar_type(), "grad_out must have same dtype as q");
     TORCH_CHECK(grad_out_in.sizes() == at::IntArrayRef({a.c.B, a.c.L, a.c.H, a.c.Dv}), "grad_out must be [B, L, H, Dv]");
@@ -146,13 +151,15 @@ Gradients attention_backward(const Tensor &grad_out_in, const Tensor &grad_last_
         TORCH_CHECK(grad_last_in.sizes() == at::IntArrayRef({a.c.B, a.c.H, a.c.Dk, a.c.Dv}), "grad_state must be [B, H, Dk, Dv]");
         grad_last = grad_last_in.contiguous();
     }
-    Tensor dq = at::empty({a.c.B, a.c.L, a.c.H, a.c.Dk}, a.q.options());
-    Tensor dk = at::empty({a.c.B, a.c.L, a.c.Hkv, a.c.Dk}, a.q.options());
-    Tensor dv = at::empty({a.c.B, a.c.L, a.c.Hkv, a.c.Dv}, a.q.options());
-    Tensor ddecay = at::empty({want_decay ? a.c.H : 0}, a.log_decay.options());
-    Tensor dstate = want_state ? at::empty({a.c.B, a.c.H, a.c.Dk, a.c.Dv}, a.log_decay.options())
-                               : at::empty({0}, a.log_decay.options());
-    const size_t ws_bytes = pathsig_linattn_backward_workspace(&a.c, want_decay);
+    auto gradient = [](bool wanted, at::IntArrayRef shape, const Tensor &like) {
+        return at::empty(wanted ? shape : at::IntArrayRef({0}), like.options());
+    };
+    const Tensor dq = gradient(want.q, {a.c.B, a.c.L, a.c.H, a.c.Dk}, a.q), dk = gradient(want.k, {a.c.B, a.c.L, a.c.Hkv, a.c.Dk}, a.q),
+                 // (from the sweep of the state's gradient)
+                 dv = gradient(want.v || want.state, {a.c.B, a.c.L, a.c.Hkv, a.c.Dv}, a.q),
+                 ddecay = gradient(want.decay, {a.c.H}, a.log_decay),
+                 dstate = gradient(want.state, {a.c.B, a.c.H, a.c.Dk, a.c.Dv}, a.log_decay);
+    const size_t ws_bytes = pathsig_linattn_backward_workspace(&a.c, want.decay);
     Tensor ws = scratch(ws_bytes, a.q);
     // The forward's workspace holds copies of q, k and v where they did not lie in whole units.  Hooks on saved tensors may hand them
     // back in other strides: a workspace that is not this call's is left, and worked out again.
@@ -188,7 +195,7 @@ Gradients linear_attention_backward_hip(const Tensor &grad_out, const MaybeTenso
                                         const Tensor &v, const Tensor &log_decay, const MaybeTensor &state,
                                         const MaybeTensor &lengths, double scale, bool want_log_decay, bool want_state) {
     return attention_backward(grad_out, or_undefined(grad_state), q, k, v, log_decay, or_undefined(state), or_undefined(lengths),
-                              Tensor(), scale, want_log_decay, want_state);
+                              Tensor(), scale, {true, true, true, want_log_decay, want_state});
 }
 
 bool any_grad(std::initializer_list<const Tensor *> all) {
@@ -243,23 +250,24 @@ struct AttentionFunction : public torch::autograd::Function<AttentionFunction<DI
         const double scale = ctx->saved_data["scale"].toDouble();
         Tensor grad_out = grads[0];
         if (!grad_out.defined()) grad_out = at::zeros({q.size(0), q.size(1), q.size(2), v.size(3)}, q.options());
-        const bool want_decay = ctx->needs_input_grad(3), want_state = state.defined() && ctx->needs_input_grad(4);
+        const Wanted want{ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2), ctx->needs_input_grad(3),
+                          state.defined() && ctx->needs_input_grad(4)};
         bool direct = DIRECT && !at::GradMode::is_enabled();
         for (const Tensor *t : {(const Tensor *)&grad_out, &q, &k, &v, &log_decay}) direct = direct && plain(*t);
         for (const Tensor *t : {&state, &lengths, &kept, &grad_last}) direct = direct && (!t->defined() || plain(*t));
         Gradients g;
         if (direct) {
-            g = attention_backward(grad_out, grad_last, q, k, v, log_decay, state, lengths, kept, scale, want_decay, want_state);
+            g = attention_backward(grad_out, grad_last, q, k, v, log_decay, state, lengths, kept, scale, want);
         } else {
             static auto op = typed_op<AttentionBackwardOp>("pathsig::linear_attention_backward");
-            g = op.call(grad_out, or_none(grad_last), q, k, v, log_decay, or_none(state), or_none(lengths), scale, want_decay,
-                        want_state);
+            g = op.call(grad_out, or_none(grad_last), q, k, v, log_decay, or_none(state), or_none(lengths), scale, want.decay,
+                        want.state);
         }
-        if (ctx->needs_input_grad(0)) out[0] = std::get<0>(g);
-        if (ctx->needs_input_grad(1)) out[1] = std::get<1>(g);
-        if (ctx->needs_input_grad(2)) out[2] = std::get<2>(g);
-        if (want_decay) out[3] = std::get<3>(g);
-        if (want_state) out[4] = std::get<4>(g);
+        if (want.q) out[0] = std::get<0>(g);
+        if (want.k) out[1] = std::get<1>(g);
+        if (want.v) out[2] = std::get<2>(g);
+        if (want.decay) out[3] = std::get<3>(g);
+        if (want.state) out[4] = std::get<4>(g);
         return out;
     }
 };
@@ -359,10 +367,10 @@ std::tuple<Tensor, Tensor, Tensor> norm_forward(const Tensor &x, const Tensor &w
 
 using NormGradients = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
 
-// gradients of x, weight, gate, residual, scale, next_weight; an empty tensor for what is not there
+// gradients of x, weight, gate, residual, scale, next_weight, those that are wanted; an empty tensor for what is not, or is not there
 NormGradients norm_backward(const Tensor &grad_out, const Tensor &grad_next, const Tensor &x, const Tensor &weight,
                             const Tensor &gate, const Tensor &residual, const Tensor &scale, const Tensor &next_weight,
-                            const Tensor &stats, double eps, int64_t activation) {
+                            const Tensor &stats, double eps, int64_t activation, const std::array<bool, 6> &want) {
     c10::DeviceGuard guard(x.device());
     const NormCall a = norm_call(x, weight, gate, residual, scale, next_weight, eps, activation);
     Tensor up[2];
@@ -378,15 +386,15 @@ NormGradients norm_backward(const Tensor &grad_out, const Tensor &grad_next, con
     TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.dim() == 2 && stats.size(0) == 2 &&
                     stats.size(1) == a.c.rows,
                 "statistics must be the forward's");
-    auto like = [](const Tensor &t, const Tensor &other) {
-        return t.defined() ? at::empty(t.sizes(), other.options()) : at::empty({0}, other.options());
-    };
-    const Tensor dx = at::empty(a.shape, x.options()), dgate = like(gate, x), dresidual = like(residual, x);
     const at::TensorOptions params = x.options().dtype(a.c.param_dtype == PATHSIG_F32 ? at::kFloat : x.scalar_type());
-    auto column = [&](const Tensor &t) { return at::empty({t.defined() ? a.c.C : 0}, params); };
-    const Tensor dweight = column(weight), dscale = column(scale), dnext = column(next_weight);
+    auto rows = [&](const Tensor &t, bool wanted) {
+        return at::empty(wanted && t.defined() ? at::IntArrayRef(a.shape) : at::IntArrayRef({0}), x.options());
+    };
+    auto column = [&](const Tensor &t, bool wanted) { return at::empty({wanted && t.defined() ? a.c.C : 0}, params); };
+    const Tensor dx = rows(x, want[0]), dweight = column(weight, want[1]), dgate = rows(gate, want[2]), dresidual = rows(residual, want[3]),
+                 dscale = column(scale, want[4]), dnext = column(next_weight, want[5]);
     const size_t ws_bytes = pathsig_norm_backward_workspace(&a.c);
-    Tensor ws = weight.defined() || scale.defined() || next_weight.defined() ? scratch(ws_bytes, x) : Tensor();
+    Tensor ws = dweight.numel() + dscale.numel() + dnext.numel() > 0 ? scratch(ws_bytes, x) : Tensor();
     check_rc(pathsig_norm_backward(&a.c, (const float *)ptr(stats), ptr(up[0]), ptr(up[1]), ptr(dx), ptr(dgate), ptr(dresidual),
                                    ptr(dweight), ptr(dscale), ptr(dnext), ptr(ws), ws.defined() ? ws_bytes : 0, stream_of(x)));
     return {dx, dweight, dgate, dresidual, dscale, dnext};
@@ -406,7 +414,8 @@ NormGradients norm_join_backward_hip(const MaybeTensor &grad_out, const MaybeTen
                                      const MaybeTensor &scale, const MaybeTensor &next_weight, const Tensor &stats, double eps,
                                      int64_t activation) {
     return norm_backward(or_undefined(grad_out), or_undefined(grad_next), x, or_undefined(weight), or_undefined(gate),
-                         or_undefined(residual), or_undefined(scale), or_undefined(next_weight), stats, eps, activation);
+                         or_undefined(residual), or_undefined(scale), or_undefined(next_weight), stats, eps, activation,
+                         {true, true, true, true, true, true});
 }
 
 using NormOp = std::tuple<Tensor, Tensor, Tensor>(const Tensor &, const MaybeTensor &, const MaybeTensor &, const MaybeTensor &,
@@ -458,19 +467,22 @@ struct NormFunction : public torch::autograd::Function<NormFunction<DIRECT>> {
         bool direct = DIRECT && !at::GradMode::is_enabled();
         for (const Tensor &t : s) direct = direct && (!t.defined() || plain(t));
         for (const Tensor *t : {&grad_out, &grad_next}) direct = direct && (!t->defined() || plain(*t));
+        const bool residual = ctx->saved_data["residual"].toBool();
+        std::array<bool, 6> want{};
+        for (int i = 0, present = 0; i < 6; ++i)  // (autograd counts the inputs that are there)
+            want[i] = (i == 3 ? residual : s[i].defined()) && ctx->needs_input_grad(present++);
         NormGradients g;
         if (direct) {
-            g = norm_backward(grad_out, grad_next, s[0], s[1], s[2], s[3], s[4], s[5], s[6], eps, activation);
+            g = norm_backward(grad_out, grad_next, s[0], s[1], s[2], s[3], s[4], s[5], s[6], eps, activation, want);
         } else {
             static auto op = typed_op<NormBackwardOp>("pathsig::norm_join_backward");
             g = op.call(or_none(grad_out), or_none(grad_next), s[0], or_none(s[1]), or_none(s[2]), or_none(s[3]), or_none(s[4]),
                         or_none(s[5]), s[6], eps, activation);
         }
-        const bool residual = ctx->saved_data["residual"].toBool();
         const Tensor all[] = {std::get<0>(g), std::get<1>(g), std::get<2>(g), s[3].defined() ? std::get<3>(g) : grad_out, std::get<4>(g),
                               std::get<5>(g)};
-        for (int i = 0, present = 0; i < 6; ++i)  // (autograd counts the inputs that are there)
-            if ((i == 3 ? residual : s[i].defined()) && ctx->needs_input_grad(present++)) out[i] = all[i];
+        for (int i = 0; i < 6; ++i)
+            if (want[i]) out[i] = all[i];
         return out;
     }
 };

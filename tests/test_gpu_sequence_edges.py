@@ -215,3 +215,72 @@ def test_a_residual_that_changes_after_the_call(dtype):
     one = a["residual"][0].detach().requires_grad_(True)
     (got,) = torch.autograd.grad(sequence.norm_after(x, residual=one), one, up)
     assert got.shape == one.shape and torch.equal(got, up.sum(0))
+
+
+# ---- gradients that nobody asks for -------------------------------------------------------------------------------
+def _subsets(names):
+    return [[n for i, n in enumerate(names) if bits >> i & 1] for bits in range(1, 2 ** len(names))]
+
+
+@pytest.mark.parametrize("dtype,shape", [(F32, (2, 300, 4, 2, 24, 32)), (BF16, (2, 300, 4, 2, 24, 32)), (BF16, (3, 45, 2, 2, 18, 10)), (F32, (2, 0, 2, 1, 8, 8))])
+def test_each_gradient_of_attention_alone(shape, dtype):
+    """Whatever part of the gradients is asked for, it is the same as in all of them."""
+    from pathsig_amd import sequence
+    a = _inputs(*shape, dtype, seed=340)
+    lengths = torch.tensor([shape[1] - 7, 3, 0][:shape[0]], device=DEV)
+    names = ("q", "k", "v", "g", "s0")
+    bound = ref.attention_bound(*(_double(a[n]) for n in names), lengths, None, _double(a["do"]), _double(a["ds"]))
+    want = None
+    for some in [list(names)] + _subsets(names):
+        leaves = {n: a[n].detach().requires_grad_(n in some) for n in names}
+        outs = sequence.linear_attention(*(leaves[n] for n in names[:4]), state=leaves["s0"], lengths=lengths, return_state=True)
+        got = dict(zip(some, torch.autograd.grad(outs, [leaves[n] for n in some], (a["do"], a["ds"]))))
+        want = want or got
+        for n in some:
+            if dtype == F32 or ("g" in some and "s0" in some):
+                assert torch.equal(got[n], want[n]), (some, n)
+                continue
+            # states that are not wanted in 32 bits carry a term of bfloat16 less: both sides are off by one rounding, 2^-8 of the value,
+            # and 2^-14 A (test_scores_and_states_in_bfloat16_keep_two_terms); what is in 32 bits, by the states' terms, 2^-16 A, at most
+            off, A = (got[n].double() - want[n].double()).abs(), bound["d" + n]
+            u = 2 ** -8 if got[n].dtype == BF16 else 2 ** -23
+            assert (off <= 2 * (u * want[n].double().abs() + 2 ** -14 * A)).all(), (some, n)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", [(40, 96), (5, 1030)])
+def test_each_gradient_of_norms_alone(shape, dtype):
+    from pathsig_amd import sequence
+    a = _norm_inputs(dtype, *shape)
+    a["next_weight"] = (a["weight"] * 0.5).detach()
+    do, dn = (torch.randn(*shape, device=DEV).to(dtype) for _ in range(2))
+    for last in (False, True):
+        names = [n for n in a if last or n != "next_weight"]
+        want = None
+        for some in [names] + _subsets(names):
+            leaves = {n: a[n].detach().requires_grad_(n in some) for n in names}
+            outs = sequence.norm_after(leaves["x"], leaves["weight"], **{n: leaves[n] for n in names if n not in ("x", "weight")})
+            got = dict(zip(some, torch.autograd.grad(outs, [leaves[n] for n in some], (do, dn) if last else do)))
+            want = want or got
+            for n in some:
+                assert torch.equal(got[n], want[n]), (some, n)
+
+
+def test_c_abi_without_some_of_the_gradients():
+    a = _inputs(2, 700, 4, 2, 32, 48, BF16, seed=350)
+    lib, c = _call(a)
+    size = lib.pathsig_linattn_backward_workspace(ctypes.byref(c), 0)
+    ws = torch.empty(size, dtype=torch.uint8, device=DEV)
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+    def backward(*which):
+        got = [torch.full_like(a[n], float("nan")) if i in which else None for i, n in enumerate(("q", "k", "v"))]
+        rc = lib.pathsig_linattn_backward(ctypes.byref(c), *(_pointer(a[n]) for n in ("q", "k", "v", "s0")), None, 0, _pointer(a["do"]),
+                                          _pointer(a["ds"]), *map(_pointer, got), None, None, _pointer(ws), size, stream)
+        assert rc == 0, lib.pathsig_last_error()
+        return got
+    want = backward(0, 1, 2)
+    assert not any(t.isnan().any() for t in want)
+    for which in ((0,), (1,), (2,), (0, 2), (1, 2), ()):
+        for i, t in enumerate(backward(*which)):
+            assert t is None or torch.equal(t, want[i])

@@ -9,7 +9,7 @@ import torch
 
 from pathsig_amd import _load, sequence
 
-ERR_ARG = -1
+ERR_ARG, ERR_WORKSPACE = -1, -3
 
 
 @pytest.fixture(scope="module")
@@ -33,6 +33,17 @@ def test_gradient_of_the_state_over_what_is_read(lib, state, above):
     rc = lib.pathsig_linattn_backward(ctypes.byref(_attention()), 256, 256, 256, state, None, 0, 256, above, 256, 256, 256, None, 512, None, 0,
                                       None)
     assert rc == ERR_ARG and b"grad_state" in lib.pathsig_last_error()
+
+
+def test_gradients_that_are_not_wanted_may_be_missing(lib):
+    """Their buffers are not asked for; the gradient of the state is worked out with that of the values."""
+    call = _attention(L=65536)
+    need = lib.pathsig_linattn_backward_workspace(ctypes.byref(call), 0)
+    for grads in ((None, None, None), (256, None, None), (None, 256, None), (None, None, 256)):
+        rc = lib.pathsig_linattn_backward(ctypes.byref(call), 256, 256, 256, None, None, 0, 256, None, *grads, None, None, 256, need - 1, None)
+        assert rc == ERR_WORKSPACE  # (nothing is launched; missing buffers would be named before)
+    rc = lib.pathsig_linattn_backward(ctypes.byref(call), 256, 256, 256, None, None, 0, 256, None, 256, 256, None, None, 512, 256, need, None)
+    assert rc == ERR_ARG and b"grad_v" in lib.pathsig_last_error()
 
 
 def _meta(*shape):
