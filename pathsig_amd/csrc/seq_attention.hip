@@ -48,7 +48,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Sweep a) {
         for (int j = 0; j < kBatch; ++j) {
             if (s0 + j >= a.pieces) break;
             const Range before = range_of(a, n, s0 + j - 1);
-            const float f = exp2f(g2 * (float)(before.end - before.begin));
+            // (nothing of the zeros in front of the first token, whatever the decay)
+            const float f = s0 + j == 1 && !a.first ? 0.f : exp2f(g2 * (float)(before.end - before.begin));
 #pragma unroll
             for (int e = 0; e < V; ++e) x.v[e] = x.v[e] * f + add[j].v[e];
             *(P *)(p + (s0 + j) * stride) = x;

@@ -84,6 +84,11 @@ __device__ __forceinline__ f32x8 half_of(f32x16 x) {
         return __builtin_shufflevector(x, x, 8, 9, 10, 11, 12, 13, 14, 15);
 }
 
+// the same in all lanes, in a scalar register
+__device__ __forceinline__ float uniform(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
+
 // row of accumulator register r
 __device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r / 4) + 4 * half + r % 4; }
 
@@ -265,10 +270,11 @@ __device__ __forceinline__ void load_state(f32x16 (&S)[DKT], const Sweep &a, int
     // one base for all lanes and 32-bit offsets; rows and columns behind the last are zeros, their addresses are kept inside
     const uint32_t offset = whole ? dv * column + (dk0 + 4 * half) * row : min(dv, a.Dv - 1) * column;
     // the state in front of the first token (s = -1) and what the pieces up to this one add, or all of that at once
-    for (int s = joined ? piece - 1 : a.first ? -1 : 0; s < piece; ++s) {
+    const int s0 = joined ? piece - 1 : a.first ? -1 : 0;
+    for (int s = s0; s < piece; ++s) {
         const float *const p = (s < 0 && !joined ? a.first : a.starts + (s + 1) * between) + head;
-        float f = 0.f;
-        if (s >= 0 && !joined) {
+        float f = 0.f;  // (of the zeros in front of the first, whatever the decay)
+        if (s > s0) {
             const Range r = range_of(a, n, s);
             f = exp2f(g2 * (float)(r.end - r.begin));
         }
@@ -345,6 +351,15 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
     f32x16 S[DKT];
     load_state<DKT, NW, FOLD>(S, a, b, h, n, piece, g2, 0, dv0, dv, half);
 
+    const int chunks = (int)((max(end - begin, (int64_t)0) + C - 1) / C);
+    int64_t r0 = end - (int64_t)chunks * C;  // of the chunk being worked on; before `begin` where the first is not full
+    // A decay above 1 may have powers that overflow where a chunk is full, and would make NaN of the zeros of padding.  A single chunk
+    // has no factors for tokens of padding and for gaps that no two of its tokens have, and a state of zeros in front of it stays one.
+    // (Behind a padded chunk, a full one has those gaps.)
+    const bool grows = g2 > 0.f && chunks == 1;
+    const int padded = grows ? (int)(begin - r0) : 0, most = C - padded;
+    const float g_state = uniform(grows && (FOLD || (piece == 0 && !a.first)) ? 0.f : g2);
+
     // Factors of a lane's registers, in LDS (they would fill the registers, and are read once a chunk): l^(C - 1 - j) for the state's
     // update; for scores l^(31 - j), which l^(i + 1) completes in the tile off the diagonal, and l^(i - j) in those on it (j after i
     // is masked where it is used)
@@ -354,15 +369,16 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
         for (int r = 0; r < 16; ++r) {
             const int j = acc_row(r, half);
             if (ln == 0) {
-                table_later[r / 4][half][r % 4] = exp2f(g2 * (float)(31 - j));
+                table_later[r / 4][half][r % 4] = j < padded ? 0.f : exp2f(g2 * (float)(31 - j));
 #pragma unroll
                 for (int t = 0; t < CT; ++t)
-                    table_left[t][r / 4][half][r % 4] = a.in_scale * exp2f(g2 * (float)(C - 1 - 32 * t - j + a.reverse));
+                    table_left[t][r / 4][half][r % 4] =
+                        32 * t + j < padded ? 0.f : a.in_scale * exp2f(g2 * (float)(C - 1 - 32 * t - j + a.reverse));
             }
-            if constexpr (!FOLD) table_diagonal[r / 4][lane][r % 4] = both * exp2f(g2 * (float)max(ln - j, 0));
+            if constexpr (!FOLD) table_diagonal[r / 4][lane][r % 4] = ln - j < most ? both * exp2f(g2 * (float)max(ln - j, 0)) : 0.f;
         }
     }
-    const float since = both * exp2f(g2 * (float)(ln + 1));
+    const float since = ln + 1 < most ? both * exp2f(g2 * (float)(ln + 1)) : 0.f;
 
     const T *const kp = (const T *)a.k.p + b * a.k.sb + (h / a.k.group) * a.k.sh;
     const T *const vp = (const T *)a.v.p + b * a.v.sb + (h / a.v.group) * a.v.sh + dv0;
@@ -370,8 +386,6 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
     const int sign = a.reverse ? -1 : 1;
     Fetch<T, DK, C, THREADS> fk, fq;
     Fetch<T, DV, C, THREADS> fv;
-    const int chunks = (int)((max(end - begin, (int64_t)0) + C - 1) / C);
-    int64_t r0 = end - (int64_t)chunks * C;  // of the chunk being worked on; before `begin` where the first is not full
     // (where registers do not hold a whole chunk, the tensors pass through them one after the other)
     auto fetch = [&](int64_t at, int pad) {
         const int64_t t = a.reverse ? n - 1 - at : at;
@@ -468,7 +482,7 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
 
         // the state after the chunk
         Frag<T> vt[CT][2];
-        const float whole = exp2f(g2 * (float)(C - pad));
+        const float whole = exp2f(g_state * (float)(C - pad));
 #pragma unroll
         for (int t = 0; t < DKT; ++t) S[t] *= whole;
 #pragma unroll
@@ -503,7 +517,7 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
 #pragma unroll
             for (int i = 0; i < CT; ++i) {
                 // (rows of padding have answers that no one reads; their exponent is kept from turning around)
-                out[i] *= a.out_scale * exp2f(g2 * (float)max(32 * i + ln + 1 - a.reverse - pad, 0));
+                out[i] *= a.out_scale * exp2f(g_state * (float)max(32 * i + ln + 1 - a.reverse - pad, 0));
                 if constexpr (kParts > 1) {
                     f32x8 P[2];
 #pragma unroll
@@ -594,8 +608,9 @@ __global__ __launch_bounds__(64 * NW, DKT == 1 || (DKT == 2 && sizeof(T) == 4) ?
     constexpr int kKBytes = C * KTile::kRow, kVBytes = C * VTile::kRow;
     __shared__ __align__(16) char lds[2 * kKBytes + 2 * kVBytes];
     __shared__ double meet[NW];
-    // Factors by token of a chunk: l^(i+1) and l^(C-1-j), and by lane and register gap l^gap in tiles on the diagonal and off it
-    // (accumulator order, zero where j is not before i)
+    // Factors by token of a chunk: l^(i+1) and l^(C-1-j), and by lane and register gap l^gap / kGap in tiles on the diagonal and off it
+    // (accumulator order, zero where j is not before i; kGap is above all gaps, so that no factor overflows where the power does not)
+    constexpr float kGap = 64.f;
     __shared__ __align__(16) f32x4 table_since[C / 4], table_left[C / 4], table_gap[CT][4][64];
     char *const lds_k = lds, *const lds_q = lds + kKBytes, *const lds_v = lds_q + kKBytes, *const lds_o = lds_v + kVBytes;
 
@@ -623,19 +638,24 @@ __global__ __launch_bounds__(64 * NW, DKT == 1 || (DKT == 2 && sizeof(T) == 4) ?
     int k_bases_of_lane[KTile::kColumnBases], v_bases_of_lane[VTile::kColumnBases];
     KTile::column_bases(k_bases_of_lane, lane);
     VTile::column_bases(v_bases_of_lane, lane);
-    if (threadIdx.x < C) table_left[threadIdx.x / 4][threadIdx.x % 4] = exp2f(g2 * (float)(C - 1 - (int)threadIdx.x));
+    // (as in chunk_kernel)
+    const bool grows = g2 > 0.f && chunks == 1;
+    const int padded = grows ? (int)(begin - r0) : 0, most = C - padded;
+    const float g_state = uniform(grows && piece == 0 && !a.first ? 0.f : g2);
+    if (threadIdx.x < C)
+        table_left[threadIdx.x / 4][threadIdx.x % 4] = (int)threadIdx.x < padded ? 0.f : exp2f(g2 * (float)(C - 1 - (int)threadIdx.x));
     if (wave < CT) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int gap = 32 * wave + ln - acc_row(r, half);
-            table_gap[wave][r / 4][lane][r % 4] = gap > 0 ? (float)gap * exp2f(g2 * (float)gap) : 0.f;
+            table_gap[wave][r / 4][lane][r % 4] = gap > 0 && gap < most ? (float)gap / kGap * exp2f(g2 * (float)gap) : 0.f;
         }
     }
     if (NW == 1 && CT == 2) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int gap = 32 + ln - acc_row(r, half);
-            table_gap[CT - 1][r / 4][lane][r % 4] = (float)gap * exp2f(g2 * (float)gap);
+            table_gap[CT - 1][r / 4][lane][r % 4] = gap < most ? (float)gap / kGap * exp2f(g2 * (float)gap) : 0.f;
         }
     }
     Fetch<T, DK, C, THREADS> fk, fq;
@@ -664,7 +684,7 @@ __global__ __launch_bounds__(64 * NW, DKT == 1 || (DKT == 2 && sizeof(T) == 4) ?
         __syncthreads();
         // (tokens of padding are rows of zeros: their factor is kept from turning around)
         if (c < 2 && threadIdx.x < C)
-            table_since[threadIdx.x / 4][threadIdx.x % 4] = exp2f(g2 * (float)max((int)threadIdx.x + 1 - pad, 0));
+            table_since[threadIdx.x / 4][threadIdx.x % 4] = exp2f(g_state * (float)max((int)threadIdx.x + 1 - pad, 0));
         if (kAhead)
             store();
         else
@@ -708,7 +728,7 @@ __global__ __launch_bounds__(64 * NW, DKT == 1 || (DKT == 2 && sizeof(T) == 4) ?
                         sum += i > j || acc_row(4 * r4 + e, half) < ln ? f[e] * x : 0.f;
                     }
                 }
-                chunk += sum;
+                chunk += kGap * sum;
             }
 
         // through the states, some tiles of rows at a time
@@ -720,16 +740,16 @@ __global__ __launch_bounds__(64 * NW, DKT == 1 || (DKT == 2 && sizeof(T) == 4) ?
             for (int t = 0; t < kBlock; ++t) G[t] = G1[t] = f32x16{};
 #pragma unroll
             for (int kk = 0; kk < 2 * CT; ++kk) {
-                f32x8 f, f1;
+                // (the power first, then its exponent: their product may overflow where that with a small element does not)
+                f32x8 o = widened(VTile::column(lds_o, v_bases, 0, kk)), o1;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    f[e] = table_since[4 * kk + 2 * (e / 4) + half][e % 4];
-                    f1[e] = (float)(16 * kk + acc_row(e, half) + 1 - pad) * f[e];
+                    o[e] *= table_since[4 * kk + 2 * (e / 4) + half][e % 4];
+                    o1[e] = (float)(16 * kk + acc_row(e, half) + 1 - pad) * o[e];
                 }
-                const f32x8 o = widened(VTile::column(lds_o, v_bases, 0, kk));
                 Frag<T> x[TERMS], x1[TERMS];
-                split_scaled<T>(o, f, x);
-                split_scaled<T>(o, f1, x1);
+                split<T>(o, x);
+                split<T>(o1, x1);
 #pragma unroll
                 for (int t = 0; t < kBlock; ++t) {
                     const Frag<T> q = KTile::column(lds_q, k_bases, t0 + t, kk);
@@ -746,7 +766,7 @@ __global__ __launch_bounds__(64 * NW, DKT == 1 || (DKT == 2 && sizeof(T) == 4) ?
         }
         total += chunk;
 
-        const float count = (float)(C - pad), whole = exp2f(g2 * count);
+        const float count = (float)(C - pad), whole = exp2f(g_state * count);
 #pragma unroll
         for (int t = 0; t < DKT; ++t) {
             D[t] = whole * (D[t] + count * S[t]);
@@ -754,16 +774,15 @@ __global__ __launch_bounds__(64 * NW, DKT == 1 || (DKT == 2 && sizeof(T) == 4) ?
         }
 #pragma unroll
         for (int kk = 0; kk < 2 * CT; ++kk) {
-            f32x8 f, f1;
+            f32x8 v = widened(VTile::column(lds_v, v_bases, 0, kk)), v1;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                f[e] = table_left[4 * kk + 2 * (e / 4) + half][e % 4];
-                f1[e] = (float)(C - 1 - 16 * kk - acc_row(e, half)) * f[e];
+                v[e] *= table_left[4 * kk + 2 * (e / 4) + half][e % 4];
+                v1[e] = (float)(C - 1 - 16 * kk - acc_row(e, half)) * v[e];
             }
-            const f32x8 v = widened(VTile::column(lds_v, v_bases, 0, kk));
             Frag<T> x[TERMS], x1[TERMS];
-            split_scaled<T>(v, f, x);
-            split_scaled<T>(v, f1, x1);
+            split<T>(v, x);
+            split<T>(v1, x1);
 #pragma unroll
             for (int t = 0; t < DKT; ++t) {
                 const Frag<T> k = KTile::column(lds_k, k_bases, t, kk);

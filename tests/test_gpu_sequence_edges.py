@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from tests import sequence_reference as ref
-from tests.test_gpu_sequence_attention import _double, _inputs, _run
+from tests.test_gpu_sequence_attention import _compare, _double, _inputs, _run
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -284,3 +284,32 @@ def test_c_abi_without_some_of_the_gradients():
     for which in ((0,), (1,), (2,), (0, 2), (1, 2), ()):
         for i, t in enumerate(backward(*which)):
             assert t is None or torch.equal(t, want[i])
+
+
+# ---- decays above 1 -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("state", [False, True])
+@pytest.mark.parametrize("g,L", [(1.5, 42), (1.5, 33), (2.0, 32), (3.0, 20), (6.0, 9), (12.0, 5), (60.0, 1), (0.9, 70), (0.3, 200), (0.1, 640)])
+def test_states_that_grow(g, L, state, dtype):
+    """Positive log-decays are no memory that fades, but a learned one may become positive: as long as its powers over the tokens there
+    are stay finite (here e^64), so do all results, whatever powers a whole chunk would have.  Tolerances as in
+    test_gpu_sequence_attention.py."""
+    for shape in ((2, L, 4, 2, 24, 40), (1, L, 4, 4, 130, 20)):
+        a = _inputs(*shape, dtype, seed=360, state=state)
+        a["g"] = torch.tensor([g, g / 2, 0.0, -g], device=DEV)
+        got = _run(a)
+        _compare(got, a, rms=False)
+        a["g"] = torch.full((4,), g, device=DEV)
+        lengths = torch.tensor([L, max(L - 3, 1)][:shape[0]], device=DEV)
+        _compare(_run(a, lengths=lengths), a, lengths=lengths, rms=False)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("g,L", [(60.0, 2), (30.0, 3), (2.8, 32), (1.42, 63)])
+def test_a_power_that_no_two_tokens_have(g, L, dtype):
+    """From a state of zeros the largest power is that between the first token and the last: one more may overflow."""
+    a = _inputs(2, L, 2, 1, 24, 40, dtype, seed=370, state=False)
+    a["g"] = torch.full((2,), g, device=DEV)
+    a["v"], a["ds"] = a["v"] * 2.0 ** -20, a["ds"] * 2.0 ** -20  # (the sums below stay finite too)
+    a["do"] = a["do"] * 2.0 ** -20
+    _compare(_run(a), a, rms=False)
