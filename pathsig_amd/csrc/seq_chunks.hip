@@ -309,10 +309,10 @@ __device__ __forceinline__ void load_state(f32x16 (&S)[DKT], const Sweep &a, int
     }
 }
 
-// TERMS: of l^(C-1-j) v_j in the state's update.
-template <typename T, typename O, int DKT, int NW, int TERMS, bool FOLD>
+// CT: tiles of 32 tokens to a chunk.  TERMS: of l^(C-1-j) v_j in the state's update.
+template <typename T, typename O, int DKT, int NW, int CT, int TERMS, bool FOLD>
 __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_kernel(const Sweep a, int slices) {
-    constexpr int DK = 32 * DKT, DV = 32 * NW, CT = chunk_tiles<T>(DKT, NW), C = 32 * CT, THREADS = 64 * NW;
+    constexpr int DK = 32 * DKT, DV = 32 * NW, C = 32 * CT, THREADS = 64 * NW;
     // fetched a chunk ahead, where registers allow it
     constexpr bool kAhead = fetched(sizeof(T), CT, DKT, NW) <= 320;
     // Scores: tiles (j, i) = (0, 0), (0, 1), (1, 1) are dealt to the waves; a single tile is split along the channels instead
@@ -321,10 +321,16 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
     using VTile = Tile<T, DV>;
     constexpr int kKBytes = C * KTile::kRow, kVBytes = C * VTile::kRow;
     __shared__ __align__(16) char lds[kKBytes * (FOLD ? 1 : 2) + kVBytes];
-    __shared__ __align__(16) f32x4 table_left[CT][4][2], table_later[4][2], table_diagonal[FOLD ? 1 : 4][64];
-    // scores as operands, in terms, or the parts of a tile's sums
+    // Tables of factors.  The small ones lie where that of the diagonal tiles has the last four j of too small an i, which nothing reads:
+    // with them beside it a block of 64 x 64 would have 384 bytes too many for four blocks to a compute unit.
+    __shared__ __align__(16) f32x4 table_diagonal[FOLD ? 1 : 4][64];
+    f32x4 (&table_left)[CT][4][2] = *(f32x4 (*)[CT][4][2])&table_diagonal[FOLD ? 0 : 3][32];
+    f32x4 (&table_later)[4][2] = *(f32x4 (*)[4][2])&table_diagonal[FOLD ? 0 : 3][32 + 8 * CT];
+    constexpr int kSmall = 8 * CT + 8;
+    static_assert(kSmall <= 28, "the unit of (r / 4, lane) = (3, 32 + i) has j = 28 .. 31 of token i");
+    // scores as operands, in terms (a wave alone keeps them), or the parts of a tile's sums
     constexpr int kTerms = sizeof(T) == 2 ? 2 : 1;
-    __shared__ __align__(16) Frag<T> scores[FOLD || kParts > 1 ? 1 : kTiles][2][kTerms][64];
+    __shared__ __align__(16) Frag<T> scores[FOLD || kParts > 1 || NW == 1 ? 1 : kTiles][2][kTerms][64];
     __shared__ __align__(16) f32x4 sums[!FOLD && kParts > 1 ? kParts : 1][4][64];
     char *const lds_k = lds, *const lds_v = lds + kKBytes, *const lds_q = lds_v + kVBytes;
 
@@ -375,7 +381,10 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
                     table_left[t][r / 4][half][r % 4] =
                         32 * t + j < padded ? 0.f : a.in_scale * exp2f(g2 * (float)(C - 1 - 32 * t - j + a.reverse));
             }
-            if constexpr (!FOLD) table_diagonal[r / 4][lane][r % 4] = ln - j < most ? both * exp2f(g2 * (float)max(ln - j, 0)) : 0.f;
+            if constexpr (!FOLD) {
+                if (r < 12 || lane < 32 || ln >= kSmall)
+                    table_diagonal[r / 4][lane][r % 4] = ln - j < most ? both * exp2f(g2 * (float)max(ln - j, 0)) : 0.f;
+            }
         }
     }
     const float since = ln + 1 < most ? both * exp2f(g2 * (float)(ln + 1)) : 0.f;
@@ -428,6 +437,7 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
 
         // scores
         f32x16 out[FOLD ? 1 : CT];
+        Frag<T> own[NW == 1 && !FOLD ? kTiles : 1][2][kTerms];
         if constexpr (!FOLD) {
             if constexpr (kParts > 1) {
                 if (wave < kParts) {
@@ -439,7 +449,7 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
                     for (int r4 = 0; r4 < 4; ++r4) sums[wave][r4][lane] = f32x4{P[4 * r4], P[4 * r4 + 1], P[4 * r4 + 2], P[4 * r4 + 3]};
                 }
             } else {
-                for (int tile = wave; tile < kTiles; tile += NW) {
+                auto score = [&](int tile, auto keep) {
                     const int i = tile > 0, j = tile > 1;
                     f32x16 P = {};
                     const char *const kt = lds_k + j * 32 * KTile::kRow, *const qt = lds_q + i * 32 * KTile::kRow;
@@ -459,8 +469,15 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
                         Frag<T> terms[kTerms];
                         split<T>(s ? half_of<1>(P) : half_of<0>(P), terms);
 #pragma unroll
-                        for (int e = 0; e < kTerms; ++e) scores[tile][s][e][lane] = terms[e];
+                        for (int e = 0; e < kTerms; ++e) keep(s, e, terms[e]);
                     }
+                };
+                if constexpr (NW == 1) {
+#pragma unroll
+                    for (int tile = 0; tile < kTiles; ++tile) score(tile, [&](int s, int e, Frag<T> x) { own[tile][s][e] = x; });
+                } else {
+                    for (int tile = wave; tile < kTiles; tile += NW)
+                        score(tile, [&](int s, int e, Frag<T> x) { scores[tile][s][e][lane] = x; });
                 }
             }
             // answers from the state
@@ -468,9 +485,8 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
             for (int i = 0; i < CT; ++i) out[i] = f32x16{};
 #pragma unroll
             for (int kk = 0; kk < DK / 16; ++kk) {
-                Frag<T> st[kTerms];
+                Frag<T> st[kTerms], q[CT];
                 split<T>(kk % 2 ? half_of<1>(S[kk / 2]) : half_of<0>(S[kk / 2]), st);
-                Frag<T> q[CT];
 #pragma unroll
                 for (int i = 0; i < CT; ++i) q[i] = KTile::row(lds_q, row_base, i, kk);
 #pragma unroll
@@ -542,7 +558,8 @@ __global__ __launch_bounds__(64 * NW, DKT <= 4 && NW >= DKT ? 2 : 1) void chunk_
 #pragma unroll
                         for (int s = 0; s < 2; ++s)
 #pragma unroll
-                            for (int e = 0; e < kTerms; ++e) out[i] = mma(vt[j][s], scores[i + j][s][e][lane], out[i]);
+                            for (int e = 0; e < kTerms; ++e)
+                                out[i] = mma(vt[j][s], NW == 1 ? own[NW == 1 ? i + j : 0][s][e] : scores[NW == 1 ? 0 : i + j][s][e][lane], out[i]);
                 }
                 const int row = 32 * i + ln;
                 if (row >= pad) {
@@ -809,16 +826,24 @@ __global__ __launch_bounds__(64 * NW, DKT == 1 || (DKT == 2 && sizeof(T) == 4) ?
     partial[(((int64_t)blockIdx.y * slices + slice) * a.B + b) * a.H + h] = (float)total;
 }
 
+template <typename T, int DKT, int NW, int CT, int TERMS>
+void launch_sweep(const Sweep &a, dim3 grid, int slices, hipStream_t stream) {
+    if (a.out_float && sizeof(T) == 2)
+        chunk_kernel<T, float, DKT, NW, CT, TERMS, false><<<grid, 64 * NW, 0, stream>>>(a, slices);
+    else
+        chunk_kernel<T, T, DKT, NW, CT, TERMS, false><<<grid, 64 * NW, 0, stream>>>(a, slices);
+}
+
+// Sequences of up to 32 tokens take chunks of 32 where longer ones have 64, half of which would be padding (1024 x 20 tokens, 16 heads
+// of 64, from a state to a state: 155 us, in chunks of 64 238; 2048 x 8 tokens in training 630 and 1238).
 template <typename T, int DKT, int NW, int TERMS>
 void launch_width(const Sweep &a, bool fold, hipStream_t stream) {
+    constexpr int CT = chunk_tiles<T>(DKT, NW);
     const int slices = (int)ceil_div(a.Dv, 32 * NW);
-    const dim3 grid((unsigned)(slices * a.H), (unsigned)(fold ? a.pieces - a.run : a.pieces / a.run), (unsigned)a.B), block(64 * NW);
-    if (fold)
-        chunk_kernel<T, T, DKT, NW, TERMS, true><<<grid, block, 0, stream>>>(a, slices);
-    else if (a.out_float && sizeof(T) == 2)
-        chunk_kernel<T, float, DKT, NW, TERMS, false><<<grid, block, 0, stream>>>(a, slices);
-    else
-        chunk_kernel<T, T, DKT, NW, TERMS, false><<<grid, block, 0, stream>>>(a, slices);
+    const dim3 grid((unsigned)(slices * a.H), (unsigned)(fold ? a.pieces - a.run : a.pieces / a.run), (unsigned)a.B);
+    if (fold) return chunk_kernel<T, T, DKT, NW, CT, TERMS, true><<<grid, 64 * NW, 0, stream>>>(a, slices);
+    if (CT > 1 && a.L <= 32) return launch_sweep<T, DKT, NW, 1, TERMS>(a, grid, slices, stream);
+    launch_sweep<T, DKT, NW, CT, TERMS>(a, grid, slices, stream);
 }
 
 // A state that is handed out in 32 bits is summed from all bits of its terms.  For one that only answers, through a copy in two terms of

@@ -313,3 +313,16 @@ def test_a_power_that_no_two_tokens_have(g, L, dtype):
     a["v"], a["ds"] = a["v"] * 2.0 ** -20, a["ds"] * 2.0 ** -20  # (the sums below stay finite too)
     a["do"] = a["do"] * 2.0 ** -20
     _compare(_run(a), a, rms=False)
+
+
+# ---- every width of the state in chunks of each length ------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("L", [19, 32, 33, 97])
+@pytest.mark.parametrize("Dk", [24, 64, 128, 200])
+@pytest.mark.parametrize("Dv", [32, 56, 128, 200])
+def test_widths_and_lengths(L, Dk, Dv, dtype):
+    """Up to 32 tokens, more, and more than a chunk, with sequences that end early and one without tokens; tolerances as in
+    test_gpu_sequence_attention.py."""
+    a = _inputs(4, L, 2, 1, Dk, Dv, dtype, seed=380)
+    lengths = torch.tensor([L, L - 1, 0, L // 2], device=DEV)
+    _compare(_run(a, lengths=lengths), a, lengths=lengths)
