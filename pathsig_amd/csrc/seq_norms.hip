@@ -114,29 +114,47 @@ __device__ __forceinline__ float row_sum(float x, float *slot) {
     return x;
 }
 
-// (the hardware's reciprocal, off by one unit in the last place at most; a division would take ten instructions)
-__device__ __forceinline__ float logistic(float g) { return __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
+// 1 / (1 + e^-g) and 1 minus it, which is not taken as a difference: behind g = 16 none of its digits would be left.  For rows in 32
+// bits to a few units in the last place: the hardware's power of two, times 1 + r for what x = -g log2 e was rounded by.  For rows in
+// bfloat16 without that, off by |g| units, 2^-17 at most where the answer is rounded to 2^-9.
+struct Logistic {
+    float up, down;
+};
+template <typename T>
+__device__ __forceinline__ Logistic logistic(float g) {
+    constexpr float kLog2e = 1.44269502162933349609375f, kLn2 = 0.693147182464599609375f, kLn2Rest = -1.904654299957767e-9f;
+    const float x = -g * kLog2e;
+    float t = __builtin_amdgcn_exp2f(x);
+    if constexpr (sizeof(T) == 4) {
+        const float r = fmaf(-x, kLn2Rest, fmaf(-x, kLn2, -g));
+        t *= 1.f + __builtin_amdgcn_fmed3f(r, 0.f, r);  // (zero instead of NaN where g is infinite)
+    }
+    const float up = __builtin_amdgcn_rcpf(1.f + t);
+    return {up, fminf(t, 1e38f) * up};  // (where t is infinite `up` is zero, and so is all that either is used for)
+}
 
+template <typename T>
 __device__ __forceinline__ float gate_value(float g, int activation) {
     if (activation == PATHSIG_GATE_LINEAR) return g;
-    const float s = logistic(g);
+    const float s = logistic<T>(g).up;
     return activation == PATHSIG_GATE_SILU ? g * s : s;
 }
 
 // value and derivative
+template <typename T>
 __device__ __forceinline__ void gate_both(float g, int activation, float &u, float &du) {
     if (activation == PATHSIG_GATE_LINEAR) {
         u = g;
         du = 1.f;
         return;
     }
-    const float s = logistic(g);
+    const Logistic s = logistic<T>(g);
     if (activation == PATHSIG_GATE_SILU) {
-        u = g * s;
-        du = s + u * (1.f - s);
+        u = g * s.up;
+        du = s.up + u * s.down;
     } else {
-        u = s;
-        du = s * (1.f - s);
+        u = s.up;
+        du = s.up * s.down;
     }
 }
 
@@ -164,7 +182,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void norm_forward_kernel(const Nor
     if (a.gate) {
         load_row<T, TPR, EPT, E>(w, (const T *)a.gate + row * a.gate_stride, t, C);
 #pragma unroll
-        for (int e = 0; e < EPT; ++e) x[e] *= gate_value(w[e], a.activation);
+        for (int e = 0; e < EPT; ++e) x[e] *= gate_value<T>(w[e], a.activation);
     }
     if (a.scale) {
         load_param<T, TPR, EPT, E>(w, a.scale, a.float_params, t, C, 1.f);
@@ -209,7 +227,9 @@ __global__ __launch_bounds__(TPR > 256 ? 1024 : threads_of(TPR), backward_waves(
     const int t = kRows > 1 ? threadIdx.x % TPR : threadIdx.x;
     const int C = a.C;
     float sum_w[EPT] = {}, sum_s[EPT] = {}, sum_n[EPT] = {};
-    // The tensors of a row are loaded while the row before is worked on.
+    // The tensors of a row are loaded while the row before is worked on; not those of wide rows in 32 bits, for which the 128 registers
+    // of a thread there are too few (8192 x 4096: with 100 to 120 bytes of them spilled 406 to 514 us a step, without 333).
+    constexpr bool kAhead = !(sizeof(T) == 4 && TPR > 256);
     RawRow<T, TPR, EPT, E> raw_x, raw_d, raw_u, raw_out, raw_n;
     float raw_r = 0.f, raw_r2 = 0.f;
     // (a row behind the last is one of zeros, which adds nothing)
@@ -228,14 +248,15 @@ __global__ __launch_bounds__(TPR > 256 ? 1024 : threads_of(TPR), backward_waves(
     };
     const int64_t step = (int64_t)gridDim.x * kRows;
     const int own = kRows > 1 ? threadIdx.x / TPR : 0;
-    fetch((int64_t)blockIdx.x * kRows + own);
+    if (kAhead) fetch((int64_t)blockIdx.x * kRows + own);
     // as many turns for every thread of a block: they meet at barriers
     for (int64_t first = (int64_t)blockIdx.x * kRows; first < a.rows; first += step) {
         const int64_t row = first + own;
         const bool live = row < a.rows;
+        if (!kAhead) fetch(row);
         RawRow<T, TPR, EPT, E> x = raw_x, d = raw_d, u = raw_u, residual = raw_out, n = raw_n;
         const float r = raw_r, r2 = raw_r2;
-        if (first + step < a.rows) fetch(row + step);
+        if (kAhead && first + step < a.rows) fetch(row + step);
         // (read again for every row, from the cache: held, the parameters would take 24 registers)
         const void *weight = a.weight, *scale = a.scale, *next_weight = a.next_weight;
         asm volatile("" : "+s"(weight), "+s"(scale), "+s"(next_weight));
@@ -254,7 +275,7 @@ __global__ __launch_bounds__(TPR > 256 ? 1024 : threads_of(TPR), backward_waves(
             float dot = 0.f;
 #pragma unroll
             for (int e = 0; e < EPT; ++e) {
-                const float g = a.gate ? gate_value(u.at(e), a.activation) : 1.f;
+                const float g = a.gate ? gate_value<T>(u.at(e), a.activation) : 1.f;
                 unit2[e] = ((a.residual ? residual.at(e) : 0.f) + unit[e] * w[e] * g * p[e]) * r2;
                 dn[e] = n.at(e);
                 sum_n[e] += dn[e] * unit2[e];
@@ -271,7 +292,7 @@ __global__ __launch_bounds__(TPR > 256 ? 1024 : threads_of(TPR), backward_waves(
 #pragma unroll
             for (int e = 0; e < EPT; ++e) {
                 float g, dg;
-                gate_both(u.at(e), a.activation, g, dg);
+                gate_both<T>(u.at(e), a.activation, g, dg);
                 const float normed = unit[e] * w[e];
                 sum_s[e] += up[e] * normed * g;
                 up[e] *= p[e];

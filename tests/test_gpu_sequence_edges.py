@@ -315,6 +315,42 @@ def test_a_power_that_no_two_tokens_have(g, L, dtype):
     _compare(_run(a), a, rms=False)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("activation", ["silu", "sigmoid"])
+def test_gates_to_the_last_places(activation, dtype):
+    """On a row of ones without eps the norm is 1 and the answer the gate's: an exponential (two units of 2^-23), a sum, a reciprocal and
+    two products, below 12 * 2^-24 of the value; of the derivative the same of the terms it adds up.  In bfloat16 the argument of
+    the exponential, up to 85 / ln 2 in size, is rounded to half a step 2^-24: below 2^-16 together, and the answer is rounded, 2^-8."""
+    from pathsig_amd import sequence
+    gate = torch.cat([torch.linspace(-85, 85, 3401), torch.linspace(-2, 2, 695)]).view(-1, 64).to(DEV, dtype).requires_grad_(True)
+    ones = torch.ones_like(gate)
+    out = sequence.norm_after(ones, gate=gate, activation=activation, eps=0.0)
+    (slope,) = torch.autograd.grad(out, gate, ones)
+    g = gate.detach().double()
+    up, down = 1 / (1 + (-g).exp()), 1 / (1 + g.exp())
+    value, terms = (g * up, (up, g * up * down)) if activation == "silu" else (up, (up * down, 0 * up))
+    u, last = (12 * 2 ** -24, 0.0) if dtype == F32 else (2 ** -16, (1 + 2 ** -16) * 2 ** -8)
+    assert ((out.detach().double() - value).abs() <= (u + last) * value.abs()).all()
+    off = (slope.double() - terms[0] - terms[1]).abs()
+    assert (off <= u * (terms[0].abs() + terms[1].abs()) + last * (terms[0] + terms[1]).abs()).all()
+
+
+def test_gates_at_their_ends():
+    """Gates behind the range of the exponential, and what is no number."""
+    from pathsig_amd import sequence
+    inf = float("inf")
+    for dtype in (F32, BF16):
+        gate = torch.tensor([[-300.0, 300.0, -inf, inf, float("nan"), 0.0, -90.0, 90.0]], device=DEV, dtype=dtype, requires_grad=True)
+        ones = torch.ones_like(gate)
+        out = sequence.norm_after(ones, gate=gate, activation="sigmoid", eps=0.0)
+        (slope,) = torch.autograd.grad(out, gate, ones)
+        assert out[0, 4].isnan() and slope[0, 4].isnan()
+        want = torch.tensor([0.0, 1.0, 0.0, 1.0, 0.5, 0.0, 1.0], device=DEV, dtype=dtype)
+        some = [0, 1, 2, 3, 5, 6, 7]
+        assert float((out.detach()[0, some] - want).abs().max()) <= 1e-38  # (e^-90 underflows)
+        assert float((slope[0, some] - want * (1 - want)).abs().max()) <= 1e-38
+
+
 # ---- every width of the state in chunks of each length ------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("L", [19, 32, 33, 97])
