@@ -382,51 +382,47 @@ __global__ __launch_bounds__(kColumnLanes * kColumnParts) void norm_columns_kern
     out[c] = from_float<P>(s);
 }
 
-struct RowShape {
-    int threads_per_row, elements;
-};
+// Elements that a thread holds, of rows of up to 8192 channels.
+constexpr int kElements = 8;
 
-// The fewest threads that hold a row with eight elements each, sixteen only for the widest rows.
-RowShape row_shape(int64_t C) {
-    static constexpr RowShape kShapes[] = {{8, 8}, {16, 8}, {32, 8}, {64, 8}, {128, 8}, {256, 8}, {512, 8}, {1024, 8}};
-    for (const RowShape &s : kShapes)
-        if (C <= (int64_t)s.threads_per_row * s.elements) return s;
-    return {0, 0};
+// The fewest threads that hold a row.
+int threads_per_row(int64_t C) {
+    int threads = 8;
+    while (threads < 1024 && (int64_t)threads * kElements < C) threads *= 2;
+    return threads;
 }
 
-int rows_per_block(const RowShape &s) { return threads_of(s.threads_per_row) / s.threads_per_row; }
+int rows_per_block(int threads) { return threads_of(threads) / threads; }
 
 // Blocks of the backward: as many as the device holds at once, and the rows dealt evenly to them.
 int64_t backward_blocks(int dtype, int64_t rows, int64_t C) {
-    const RowShape s = row_shape(C);
-    const int threads = threads_of(s.threads_per_row);
-    const int64_t groups = ceil_div(rows, rows_per_block(s));
-    const int waves = backward_waves(dtype == PATHSIG_F32 ? 4 : 2, s.threads_per_row);
+    const int per_row = threads_per_row(C), threads = threads_of(per_row);
+    const int64_t groups = ceil_div(rows, rows_per_block(per_row));
+    const int waves = backward_waves(dtype == PATHSIG_F32 ? 4 : 2, per_row);
     const int64_t most = (int64_t)256 * (256 * waves / threads);
     return ceil_div(groups, ceil_div(groups, most));
 }
 
-template <typename T, int TPR, int EPT, int E>
+template <typename T, int TPR, int E>
 void launch(const NormArgs &a, bool backward, int64_t blocks, hipStream_t stream) {
     constexpr int kThreads = threads_of(TPR);
     if (backward)
-        norm_backward_kernel<T, TPR, EPT, E><<<dim3((unsigned)blocks), dim3(kThreads), 0, stream>>>(a);
+        norm_backward_kernel<T, TPR, kElements, E><<<dim3((unsigned)blocks), dim3(kThreads), 0, stream>>>(a);
     else
-        norm_forward_kernel<T, TPR, EPT, E><<<dim3((unsigned)blocks), dim3(kThreads), 0, stream>>>(a);
+        norm_forward_kernel<T, TPR, kElements, E><<<dim3((unsigned)blocks), dim3(kThreads), 0, stream>>>(a);
 }
 
 template <typename T, int E>
 void dispatch(const NormArgs &a, bool backward, int64_t blocks, hipStream_t stream) {
-    const RowShape s = row_shape(a.C);
-    switch (s.threads_per_row * 100 + s.elements) {
-        case 808: return launch<T, 8, 8, E>(a, backward, blocks, stream);
-        case 1608: return launch<T, 16, 8, E>(a, backward, blocks, stream);
-        case 3208: return launch<T, 32, 8, E>(a, backward, blocks, stream);
-        case 6408: return launch<T, 64, 8, E>(a, backward, blocks, stream);
-        case 12808: return launch<T, 128, 8, E>(a, backward, blocks, stream);
-        case 25608: return launch<T, 256, 8, E>(a, backward, blocks, stream);
-        case 51208: return launch<T, 512, 8, E>(a, backward, blocks, stream);
-        default: return launch<T, 1024, 8, E>(a, backward, blocks, stream);
+    switch (threads_per_row(a.C)) {
+        case 8: return launch<T, 8, E>(a, backward, blocks, stream);
+        case 16: return launch<T, 16, E>(a, backward, blocks, stream);
+        case 32: return launch<T, 32, E>(a, backward, blocks, stream);
+        case 64: return launch<T, 64, E>(a, backward, blocks, stream);
+        case 128: return launch<T, 128, E>(a, backward, blocks, stream);
+        case 256: return launch<T, 256, E>(a, backward, blocks, stream);
+        case 512: return launch<T, 512, E>(a, backward, blocks, stream);
+        default: return launch<T, 1024, E>(a, backward, blocks, stream);
     }
 }
 
@@ -463,7 +459,7 @@ int check_norm(const pathsig_norm *c) {
         set_error("C must be at most %d (got %lld)", PATHSIG_MAX_NORM_CHANNELS, (long long)c->C);
         return PATHSIG_ERR_UNSUPPORTED;
     }
-    if (ceil_div(c->rows, rows_per_block(row_shape(c->C))) > 0x7fffffff) {
+    if (ceil_div(c->rows, rows_per_block(threads_per_row(c->C))) > 0x7fffffff) {
         set_error("too many rows (%lld)", (long long)c->rows);
         return PATHSIG_ERR_UNSUPPORTED;
     }
@@ -529,7 +525,7 @@ int pathsig_norm_forward(const pathsig_norm *call, void *out, void *next, float 
     a.out = out;
     a.next = next;
     a.stats = statistics;
-    run(a, call->dtype, false, ceil_div(a.rows, rows_per_block(row_shape(a.C))), (hipStream_t)stream);
+    run(a, call->dtype, false, ceil_div(a.rows, rows_per_block(threads_per_row(a.C))), (hipStream_t)stream);
     return launch_status("norm forward");
 }
 
