@@ -26,7 +26,7 @@ struct NormArgs {
     const void *grad_out, *grad_next;
     void *grad_x, *grad_gate, *grad_residual;
     float *partial;  // [3][blocks][C]: weight, scale, next_weight
-    int64_t rows, x_stride, gate_stride, residual_stride;
+    int64_t first_row, rows, x_stride, gate_stride, residual_stride;  // first_row: of a forward's launch
     int C, activation, float_params, want_weight, want_scale, want_next;
     float eps;
 };
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void norm_forward_kernel(const Nor
     constexpr int kRows = threads_of(TPR) / TPR;
     __shared__ float slots[2][16];
     const int t = threadIdx.x % TPR;
-    const int64_t row_or_behind = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
+    const int64_t row_or_behind = a.first_row + (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
     const bool live = row_or_behind < a.rows;  // (all threads of a block meet at barriers)
     const int64_t row = live ? row_or_behind : a.rows - 1;
     const int C = a.C;
@@ -525,7 +525,10 @@ int pathsig_norm_forward(const pathsig_norm *call, void *out, void *next, float 
     a.out = out;
     a.next = next;
     a.stats = statistics;
-    run(a, call->dtype, false, ceil_div(a.rows, rows_per_block(threads_per_row(a.C))), (hipStream_t)stream);
+    // (a launch has fewer than 2^32 threads)
+    const int64_t of_block = rows_per_block(threads_per_row(a.C)), most = ((int64_t)1 << 31) / threads_of(threads_per_row(a.C));
+    for (; a.first_row < a.rows; a.first_row += most * of_block)
+        run(a, call->dtype, false, std::min(ceil_div(a.rows - a.first_row, of_block), most), (hipStream_t)stream);
     return launch_status("norm forward");
 }
 

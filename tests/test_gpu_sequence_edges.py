@@ -362,3 +362,20 @@ def test_widths_and_lengths(L, Dk, Dv, dtype):
     a = _inputs(4, L, 2, 1, Dk, Dv, dtype, seed=380)
     lengths = torch.tensor([L, L - 1, 0, L // 2], device=DEV)
     _compare(_run(a, lengths=lengths), a, lengths=lengths)
+
+
+def test_rows_of_more_threads_than_a_launch_has():
+    """2^29 rows of one channel, eight threads each: the last rows are answered like the same ones alone, and get their gradients."""
+    from pathsig_amd import sequence
+    rows = 2 ** 29 + 3001
+    x = torch.full((rows, 1), 2.0, dtype=BF16, device=DEV)
+    x[-5000:] = torch.randn(5000, 1, device=DEV).to(BF16)
+    with torch.no_grad():
+        out = sequence.norm_before(x, eps=0.25)
+        assert torch.equal(out[-5000:], sequence.norm_before(x[-5000:], eps=0.25))
+        assert bool((out[:-5000] == (2.0 / 4.25 ** 0.5 * torch.ones(1, device=DEV)).to(BF16)).all())
+    x.requires_grad_(True)
+    (grad,) = torch.autograd.grad(sequence.norm_before(x, eps=0.25), x, out)
+    some = x.detach()[-5000:].requires_grad_(True)
+    (want,) = torch.autograd.grad(sequence.norm_before(some, eps=0.25), some, out[-5000:])
+    assert torch.equal(grad[-5000:], want)
