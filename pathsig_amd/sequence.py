@@ -39,6 +39,7 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, *, stat
     Returns out (B, L, H, Dv), with `return_state` also S after the last token of every sequence, (B, H, Dk, Dv) float32.
     """
     scale = max(q.shape[-1], 1) ** -0.5 if scale is None else float(scale)
+    return_state = bool(return_state)
     if not _is_compiling():
         out = _direct.linear_attention(q, k, v, log_decay, state, lengths, scale, return_state)
         if out is not None:

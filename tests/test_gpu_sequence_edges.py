@@ -379,3 +379,16 @@ def test_rows_of_more_threads_than_a_launch_has():
     some = x.detach()[-5000:].requires_grad_(True)
     (want,) = torch.autograd.grad(sequence.norm_before(some, eps=0.25), some, out[-5000:])
     assert torch.equal(grad[-5000:], want)
+
+
+def test_return_state_is_any_truth_value():
+    import numpy as np
+    from pathsig_amd import sequence
+    a = _inputs(1, 5, 2, 1, 8, 8, F32, seed=390)
+    args = [a[n] for n in ("q", "k", "v", "g")]
+    want = sequence.linear_attention(*args, return_state=True)
+    for yes in (1, np.True_, np.bool_(1)):
+        got = sequence.linear_attention(*args, return_state=yes)
+        assert isinstance(got, tuple) and all(torch.equal(x, y) for x, y in zip(got, want))
+    for no in (0, np.False_, None):
+        assert torch.equal(sequence.linear_attention(*args, return_state=no), want[0])
