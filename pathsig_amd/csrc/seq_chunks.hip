@@ -813,10 +813,12 @@ __global__ __launch_bounds__(64 * NW, DKT == 1 || (DKT == 2 && sizeof(T) == 4) ?
         }
     }
     total *= a.out_scale;
-    // the gradient of the state behind the piece
-    load_state<DKT, NW, false>(S, back, b, h, n, a.pieces - piece - a.run, g2, dk0, dv0, dv, half);
+    // the gradient of the state behind the piece; not where there is no token, whatever it is
+    if (chunks > 0) {
+        load_state<DKT, NW, false>(S, back, b, h, n, a.pieces - piece - a.run, g2, dk0, dv0, dv, half);
 #pragma unroll
-    for (int t = 0; t < DKT; ++t) total += sum16(D[t] * S[t]);
+        for (int t = 0; t < DKT; ++t) total += sum16(D[t] * S[t]);
+    }
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) total += __shfl_xor(total, m);
     if (lane == 0) meet[wave] = total;

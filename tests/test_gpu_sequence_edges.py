@@ -392,3 +392,19 @@ def test_return_state_is_any_truth_value():
         assert isinstance(got, tuple) and all(torch.equal(x, y) for x, y in zip(got, want))
     for no in (0, np.False_, None):
         assert torch.equal(sequence.linear_attention(*args, return_state=no), want[0])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("L", [20, 700])
+def test_what_a_sequence_without_tokens_holds_stays_there(L, dtype):
+    """The state of a place in the batch that nothing uses, and the gradient from above for it, may be no numbers."""
+    a = _inputs(3, L, 2, 1, 24, 40, dtype, seed=395)
+    lengths = torch.tensor([L, 0, L // 2], device=DEV)
+    want = _run(a, lengths=lengths)
+    for n in ("s0", "ds"):
+        a[n][1, :, :5], a[n][1, :, 5:] = float("nan"), float("inf")
+    got = _run(a, lengths=lengths)
+    assert torch.equal(got["dg"], want["dg"])
+    for n in ("out", "last", "dq", "dk", "dv", "ds0"):
+        assert torch.equal(got[n][::2], want[n][::2]), n
+    assert (got["out"][1] == 0).all() and torch.equal(got["last"][1, :, 5:], a["s0"][1, :, 5:])
