@@ -408,3 +408,50 @@ def test_what_a_sequence_without_tokens_holds_stays_there(L, dtype):
     for n in ("out", "last", "dq", "dk", "dv", "ds0"):
         assert torch.equal(got[n][::2], want[n][::2]), n
     assert (got["out"][1] == 0).all() and torch.equal(got["last"][1, :, 5:], a["s0"][1, :, 5:])
+
+
+# ---- plans of pieces ----------------------------------------------------------------------------------------------
+# Sequences are cut into pieces where there are few of them.  Up to four pieces are joined by the blocks that start from them, more by a
+# launch of their own; 171 to 256 heads of more than 64 channels are folded in halves and swept two pieces to a block.
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape,pieces", [
+    # B, L, H, Hkv, Dk, Dv: two pieces, three, four, more; rows times columns of the state no multiple of four; heads or rows that are no
+    # whole units of 16 bytes and are copied first
+    ((3, 250, 2, 1, 16, 128), 2), ((1, 192, 2, 1, 16, 16), 3), ((1, 500, 3, 3, 8, 8), 4), ((1, 2304, 1, 1, 16, 24), 36),
+    ((1, 900, 3, 1, 5, 7), None), ((2, 700, 2, 1, 18, 10), None), ((1, 300, 2, 2, 33, 65), None), ((1, 1500, 2, 2, 129, 3), None)])
+def test_pieces(shape, pieces, dtype):
+    a = _inputs(*shape, dtype, seed=410)
+    assert pieces is None or _pieces(*_call(a)) == pieces
+    _compare(_run(a), a, rms=False)
+    L = shape[1]
+    lengths = torch.tensor([L - 70, 65, 1][:shape[0]], device=DEV)
+    _compare(_run(a, lengths=lengths), a, lengths=lengths, rms=False)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("L,Dk,Dv,Hkv", [(616, 80, 72, 16), (617, 72, 80, 4), (640, 16, 96, 16), (1030, 128, 128, 16)])
+def test_two_pieces_to_a_block(L, Dk, Dv, Hkv, dtype):
+    """176 heads of sequences, folded in halves: all lengths alike, and sequences that end in each half, at its border and before it
+    begins."""
+    B, H = 11, 16
+    a = _inputs(B, L, H, Hkv, Dk, Dv, dtype, seed=420)
+    lib, c = _call(a)
+    assert _pieces(lib, c) == 4
+    _compare(_run(a), a)
+    piece = -(-(-(-L // 4)) // 64) * 64
+    lengths = torch.tensor([L, 0, 1, piece - 1, piece, piece + 1, 2 * piece - 3, 2 * piece, 2 * piece + 1, 3 * piece + 5, L - 1], device=DEV)
+    got = _run(a, lengths=lengths)
+    _compare(got, a, lengths=lengths)
+    dead = torch.arange(L, device=DEV)[None] >= lengths[:, None]
+    for n in ("out", "dq", "dk", "dv"):
+        assert (got[n][dead] == 0).all(), n
+
+
+@pytest.mark.parametrize("shape", [(2, 100, 4, 2, 24, 40), (1, 700, 4, 4, 64, 64), (2, 300, 2, 1, 130, 20), (2, 40, 3, 1, 18, 10), (1, 2304, 2, 2, 16, 24)])
+def test_decays_gradient_in_bfloat16_is_summed_in_32_bits(shape):
+    """Its terms enter in three parts of bfloat16, all their bits: the bound of float32."""
+    a = _inputs(*shape, BF16, seed=430)
+    args = [_double(a[n]) for n in ("q", "k", "v", "g", "s0")] + [None, None, _double(a["do"]), _double(a["ds"])]
+    want, bound = ref.attention(*args)["dg"], ref.attention_bound(*args)["dg"]
+    off = (_run(a)["dg"].double() - want).abs()
+    assert (off <= 2 ** -24 * (2 * shape[1] + max(shape[4:]) + 64) * bound).all(), float((off / bound).max())
