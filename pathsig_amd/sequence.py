@@ -131,11 +131,12 @@ class LinearAttention(nn.Module):
 
     def _apply(self, fn, recurse=True):
         # (a slow decay in bfloat16 would be none: 1 - 2^-9 rounds to 1)
-        decays = (self.log_decay, self.log_decay.grad)
+        decays = self._parameters.get("log_decay", self._buffers.get("log_decay"))
+        held = () if decays is None else (decays, decays.grad)
 
         def keep_float(t):
             new = fn(t)
-            if new.dtype == t.dtype or not any(t is d for d in decays):
+            if new.dtype == t.dtype or not any(t is h for h in held):
                 return new
             return t.to(new.device)
         return super()._apply(keep_float, recurse)
