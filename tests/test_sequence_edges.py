@@ -12,6 +12,15 @@ from pathsig_amd import _load, sequence
 ERR_ARG, ERR_WORKSPACE = -1, -3
 
 
+@pytest.fixture(autouse=True)
+def float32_by_default():
+    """Tensors made here without a type are float32, whatever the tests before left as the default."""
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(torch.float32)
+    yield
+    torch.set_default_dtype(before)
+
+
 @pytest.fixture(scope="module")
 def lib():
     return _load.lib()
