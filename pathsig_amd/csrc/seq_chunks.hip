@@ -21,17 +21,18 @@
 //
 // Rounding in bf16: scores and the state's copy for the products with V and Q are split into two terms of bf16 each, which are off by
 // 2^-16 of them: an answer is rounded once, at its end.  (With one term they are off by as much as that rounding: root mean square
-// of the error 2.35e-3 of the answers against 1.66e-3; a sweep of 16 x 4096 tokens of 16 heads of 128 takes 283 us with one and
-// 325 with two.)  The state itself stays in 32 bits, and so does what is added to it: l^(C-1-j) v_j is split too, three terms hold all
+// of the error 2.35e-3 of the answers against 1.66e-3; a sweep of 16 x 4096 tokens of 16 heads of 128 took 270 us with one and
+// takes 310 with two.)  The state itself stays in 32 bits, and so does what is added to it: l^(C-1-j) v_j is split too, three terms hold all
 // 24 bits (launch_terms).
 //
 // A first chunk that is not full is filled from the front with tokens of zeros, so that the factors l^(C-1-j) hold for every
 // chunk and none of them is a quotient.
 //
 // Bound by memory first: 16 x 4096 tokens of 16 heads of 128 in bf16 are 1.07 GB to read and write, 210 us at the rate of a large
-// copy (5.1 TB/s); the sweep takes 325 in two pieces, two blocks to a compute unit with 48 KB each on their way: 76 to 100 matrix
-// instructions and about 500 vector ones a chunk and wave, which loads and stores do not hide altogether (with scores and the state's
-// copy in one term, 22 matrix instructions less, it was 283, and 150 without loads and stores).
+// copy (5.1 TB/s); the sweep takes 310 in two pieces, two blocks to a compute unit with 48 KB each on their way.  What two waves to a
+// SIMD do not hide: 76 to 84 matrix instructions and about 790 vector ones a chunk and wave (a quarter of the time each), one after
+// the other between two barriers, and 24 of 256 registers that are spilled.  In one piece, one block to a unit, it took 356 where two
+// took 290.
 #include <algorithm>
 
 #include "seq_attention.hpp"
