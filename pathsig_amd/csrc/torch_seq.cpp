@@ -1,6 +1,7 @@
 // Registration of the sequence operators (linear attention with decays, norms before and after a block) with the torch
 // dispatcher: schemas, argument checks, device implementations over the C ABI of pathsig_hip.h, autograd nodes, and the
 // functions that plain eager calls take past the dispatcher.  They have no counterpart in the reference.
+#include <algorithm>
 #include <array>
 #include <optional>
 #include <tuple>
@@ -471,6 +472,10 @@ struct NormFunction : public torch::autograd::Function<NormFunction<DIRECT>> {
         std::array<bool, 6> want{};
         for (int i = 0, present = 0; i < 6; ++i)  // (autograd counts the inputs that are there)
             want[i] = (i == 3 ? residual : s[i].defined()) && ctx->needs_input_grad(present++);
+        if (want[3] && !s[3].defined() && std::count(want.begin(), want.end(), true) == 1) {
+            out[3] = grad_out;
+            return out;
+        }
         NormGradients g;
         if (direct) {
             g = norm_backward(grad_out, grad_next, s[0], s[1], s[2], s[3], s[4], s[5], s[6], eps, activation, want);
